@@ -328,6 +328,113 @@ int vk_conv3x3_resize_ac_forward_batched(vk_ctx* ctx, const vk_conv3x3* conv, si
                                          const float* bias, float* out);
 int vk_conv3x3_release(vk_conv3x3* conv);
 
+/* ------------------------------------------------- trainable block pieces
+ * The parts of a ViT block around its projections, with their gradients:
+ * attention that keeps its row statistics and its backward pass, rotary
+ * positions over several axes, and the residual step between two norms.  They
+ * have no counterpart in the reference, which runs the encoder forward only.
+ *  - Buffers are device pointers of the context's GPU; the element type is
+ *    given per call and decides the arithmetic (vk_set_math does not apply).
+ *  - They allocate nothing and use no workspace of the context, so a call can
+ *    be captured into a CUDA graph and replayed; what a call needs beside its
+ *    outputs is passed in and belongs to the caller.
+ *  - Every element of every output is written on every call, the same bits
+ *    each time (no atomics); outputs may not overlap inputs except where said.
+ *  - The calling thread's current device is left as it was. */
+#define VK_DTYPE_F32 0
+#define VK_DTYPE_BF16 1
+
+/* A [batch, heads, tokens, head_dim] tensor with any order of its first three
+ * dimensions; strides in elements, head_dim contiguous.  No element lies at two
+ * places: strides of dimensions longer than one are positive and none of them
+ * falls inside another's extent.  For attention `data` and these strides are
+ * multiples of 16 bytes. */
+typedef struct {
+  void* data;
+  int64_t batch_stride, head_stride, token_stride;
+} vk_heads;
+
+typedef struct {
+  int dtype; /* VK_DTYPE_F32: f32 arithmetic; VK_DTYPE_BF16: bf16 products, f32 sums */
+  size_t batch, heads, q_tokens, kv_tokens;
+  size_t head_dim;         /* 8, 16, 32 or 64                                        */
+  float scale;             /* of the scores, e.g. 1 / sqrt(head_dim); finite, > 0    */
+  const int32_t* q_lens;   /* device [batch]: sequence b has q_lens[b] queries and   */
+  const int32_t* kv_lens;  /* kv_lens[b] keys (clamped to 0..tokens); NULL: all      */
+} vk_attention_shape;
+
+/* out = softmax(scale q k^T) v over the valid keys, not causal; lse [batch,
+ * heads, q_tokens] (f32) = log of the row's sum of exponentials.  Queries past
+ * q_lens and rows without keys: out 0, lse -inf.  What lies past the lengths
+ * in q, k, v is never used (it may hold NaN). */
+int vk_attention_forward(vk_ctx* ctx, const vk_attention_shape* shape, const vk_heads* q, const vk_heads* k,
+                         const vk_heads* v, const vk_heads* out, float* lse);
+/* Gradients of vk_attention_forward for d_out, from its inputs, out and lse;
+ * the probabilities are recomputed.  Rows past the lengths get zeros.  delta
+ * [batch, heads, q_tokens] (f32) is scratch that belongs to this call until it
+ * has run; it receives the row sums of d_out * out. */
+int vk_attention_backward(vk_ctx* ctx, const vk_attention_shape* shape, const vk_heads* q, const vk_heads* k,
+                          const vk_heads* v, const vk_heads* out, const float* lse, const vk_heads* d_out,
+                          const vk_heads* dq, const vk_heads* dk, const vk_heads* dv, float* delta);
+
+/* Rotary positions over up to VK_ROPE_MAX_AXES axes (time, height, width, ...),
+ * vk_rope2d's rule with any widths: axis a owns the next sections[a] (even)
+ * elements of a head, element i of its first half pairs with element i of its
+ * second half, and the pair turns by position[a] * freq^(-2 i / sections[a]).
+ * Elements past the sections are copied. */
+#define VK_ROPE_MAX_AXES 4
+typedef struct {
+  int dtype;
+  size_t batch, heads, tokens, head_dim; /* head_dim <= 256 */
+  size_t axes;
+  size_t sections[VK_ROPE_MAX_AXES];
+  float freq;
+  int inverse;               /* turn back: the gradient of the forward rotation */
+  int positions_per_batch;   /* positions [batch, tokens, axes], else [tokens, axes] */
+} vk_rope_axes_shape;
+/* q -> q_out and, unless k is NULL, k -> k_out (the same pointer and strides:
+ * in place; other overlaps are not allowed).  positions int64 (device), any
+ * value below 2^53 in size; angles are taken in double precision. */
+int vk_rope_axes(vk_ctx* ctx, const vk_rope_axes_shape* shape, const vk_heads* q, const vk_heads* k,
+                 const int64_t* positions, const vk_heads* q_out, const vk_heads* k_out);
+
+/* The residual step between two norms, rows = groups * rows_per_group (a group
+ * is an image), everything [rows, cols] contiguous:
+ *   n = branch, or its LayerNorm (post_gamma, post_beta) where post_gamma is set
+ *   h = x + scale[col] * gate[group][col] * n       (NULL scale or gate: ones)
+ *   y = LayerNorm(h; gamma, beta)
+ * x and h have stream_dtype, branch and y branch_dtype; vectors and statistics
+ * are f32.  (stream, branch) is (f32, f32), (f32, bf16) or (bf16, bf16); y is
+ * taken from h before h is rounded.  cols <= 8192. */
+typedef struct {
+  int stream_dtype, branch_dtype;
+  size_t groups, rows_per_group, cols;
+  float eps;
+  const float *gamma, *beta;           /* [cols]         */
+  const float *scale;                  /* [cols] or NULL */
+  const float *gate;                   /* [groups, cols] or NULL */
+  const float *post_gamma, *post_beta; /* [cols], both or neither */
+} vk_residual_norm_shape;
+/* stats [rows, 2] receives (mean, 1 / sqrt(var + eps)) of h, post_stats those
+ * of branch (NULL without a norm of the branch).  h may be x. */
+int vk_residual_norm_forward(vk_ctx* ctx, const vk_residual_norm_shape* shape, const void* x, const void* branch,
+                             void* h, void* y, float* stats, float* post_stats);
+typedef struct {
+  void* d_x;      /* [rows, cols] stream_dtype: the gradient of x, may be d_h */
+  void* d_branch; /* [rows, cols] branch_dtype, may be d_y                    */
+  float *d_gamma, *d_beta;           /* [cols]                     */
+  float *d_scale;                    /* [cols], NULL iff scale is  */
+  float *d_gate;                     /* [groups, cols], NULL iff gate is */
+  float *d_post_gamma, *d_post_beta; /* [cols], NULL iff post_gamma is   */
+} vk_residual_norm_grads;
+/* d_h: the gradient that reaches h by its other use, the residual stream (NULL:
+ * none); d_y that of y.  workspace: vk_residual_norm_workspace(ctx, shape) bytes
+ * (16-byte aligned) that belong to this call until it has run. */
+int vk_residual_norm_backward(vk_ctx* ctx, const vk_residual_norm_shape* shape, const void* d_h, const void* d_y,
+                              const void* h, const void* branch, const float* stats, const float* post_stats,
+                              const vk_residual_norm_grads* grads, void* workspace, size_t workspace_bytes);
+int vk_residual_norm_workspace(vk_ctx* ctx, const vk_residual_norm_shape* shape, size_t* bytes);
+
 #ifdef __cplusplus
 }
 #endif

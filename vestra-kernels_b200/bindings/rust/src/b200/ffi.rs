@@ -19,6 +19,10 @@ pub const VK_MATH_F32: c_int = 0;
 pub const VK_MATH_BF16: c_int = 1;
 pub const VK_MATH_Q8_0: c_int = 2;
 
+pub const VK_DTYPE_F32: c_int = 0;
+pub const VK_DTYPE_BF16: c_int = 1;
+pub const VK_ROPE_MAX_AXES: usize = 4;
+
 #[repr(C)]
 pub struct VkCtx { _p: [u8; 0] }
 #[repr(C)]
@@ -29,6 +33,42 @@ pub struct VkEncoder { _p: [u8; 0] }
 pub struct VkConv3x3 { _p: [u8; 0] }
 #[repr(C)]
 pub struct VkPatchEmbed { _p: [u8; 0] }
+
+/// vk_heads: a [batch, heads, tokens, head_dim] tensor, strides in elements.
+#[repr(C)]
+pub struct VkHeads { pub data: *mut c_void, pub batch_stride: i64, pub head_stride: i64, pub token_stride: i64 }
+
+#[repr(C)]
+pub struct VkAttentionShape {
+    pub dtype: c_int,
+    pub batch: usize, pub heads: usize, pub q_tokens: usize, pub kv_tokens: usize, pub head_dim: usize,
+    pub scale: f32,
+    pub q_lens: *const i32, pub kv_lens: *const i32,
+}
+
+#[repr(C)]
+pub struct VkRopeAxesShape {
+    pub dtype: c_int,
+    pub batch: usize, pub heads: usize, pub tokens: usize, pub head_dim: usize,
+    pub axes: usize, pub sections: [usize; VK_ROPE_MAX_AXES],
+    pub freq: f32, pub inverse: c_int, pub positions_per_batch: c_int,
+}
+
+#[repr(C)]
+pub struct VkResidualNormShape {
+    pub stream_dtype: c_int, pub branch_dtype: c_int,
+    pub groups: usize, pub rows_per_group: usize, pub cols: usize,
+    pub eps: f32,
+    pub gamma: *const f32, pub beta: *const f32, pub scale: *const f32, pub gate: *const f32,
+    pub post_gamma: *const f32, pub post_beta: *const f32,
+}
+
+#[repr(C)]
+pub struct VkResidualNormGrads {
+    pub d_x: *mut c_void, pub d_branch: *mut c_void,
+    pub d_gamma: *mut f32, pub d_beta: *mut f32, pub d_scale: *mut f32, pub d_gate: *mut f32,
+    pub d_post_gamma: *mut f32, pub d_post_beta: *mut f32,
+}
 
 /// vk_layer_weights: host f32 arrays of one block, [K, N] weights.
 #[repr(C)]
@@ -108,4 +148,10 @@ extern "C" {
     pub fn vk_conv3x3_forward_batched(ctx: *mut VkCtx, conv: *const VkConv3x3, images: usize, input: *const f32, ih: usize, iw: usize, bias: *const f32, relu_input: c_int, out: *mut f32) -> c_int;
     pub fn vk_conv3x3_resize_ac_forward_batched(ctx: *mut VkCtx, conv: *const VkConv3x3, images: usize, input: *const f32, ih: usize, iw: usize, oh: usize, ow: usize, add: *const f32, bias: *const f32, out: *mut f32) -> c_int;
     pub fn vk_conv3x3_release(conv: *mut VkConv3x3) -> c_int;
+    pub fn vk_attention_forward(ctx: *mut VkCtx, shape: *const VkAttentionShape, q: *const VkHeads, k: *const VkHeads, v: *const VkHeads, out: *const VkHeads, lse: *mut f32) -> c_int;
+    pub fn vk_attention_backward(ctx: *mut VkCtx, shape: *const VkAttentionShape, q: *const VkHeads, k: *const VkHeads, v: *const VkHeads, out: *const VkHeads, lse: *const f32, d_out: *const VkHeads, dq: *const VkHeads, dk: *const VkHeads, dv: *const VkHeads, delta: *mut f32) -> c_int;
+    pub fn vk_rope_axes(ctx: *mut VkCtx, shape: *const VkRopeAxesShape, q: *const VkHeads, k: *const VkHeads, positions: *const i64, q_out: *const VkHeads, k_out: *const VkHeads) -> c_int;
+    pub fn vk_residual_norm_forward(ctx: *mut VkCtx, shape: *const VkResidualNormShape, x: *const c_void, branch: *const c_void, h: *mut c_void, y: *mut c_void, stats: *mut f32, post_stats: *mut f32) -> c_int;
+    pub fn vk_residual_norm_backward(ctx: *mut VkCtx, shape: *const VkResidualNormShape, d_h: *const c_void, d_y: *const c_void, h: *const c_void, branch: *const c_void, stats: *const f32, post_stats: *const f32, grads: *const VkResidualNormGrads, workspace: *mut c_void, workspace_bytes: usize) -> c_int;
+    pub fn vk_residual_norm_workspace(ctx: *mut VkCtx, shape: *const VkResidualNormShape, bytes: *mut usize) -> c_int;
 }

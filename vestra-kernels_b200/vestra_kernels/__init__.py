@@ -33,6 +33,9 @@ MATH_F32 = 0
 MATH_BF16 = 1
 MATH_Q8_0 = 2
 
+DTYPE_F32 = 0
+DTYPE_BF16 = 1
+
 QK8_0 = 32
 DA3_BASE_TOKENS = 865
 
@@ -92,6 +95,12 @@ SIGNATURES = {
     "vk_conv3x3_forward_batched": (_I, [_P, _P, _S, _P, _S, _S, _P, _I, _P]),
     "vk_conv3x3_resize_ac_forward_batched": (_I, [_P, _P, _S, _P, _S, _S, _S, _S, _P, _P, _P]),
     "vk_conv3x3_release": (_I, [_P]),
+    "vk_attention_forward": (_I, [_P] * 7),
+    "vk_attention_backward": (_I, [_P] * 12),
+    "vk_rope_axes": (_I, [_P] * 7),
+    "vk_residual_norm_forward": (_I, [_P] * 8),
+    "vk_residual_norm_backward": (_I, [_P] * 10 + [_S]),
+    "vk_residual_norm_workspace": (_I, [_P, _P, ctypes.POINTER(_S)]),
 }
 
 _lib = None
@@ -577,3 +586,255 @@ class Encoder:
                 self.handle = None
         except Exception:
             pass
+
+
+# ---------------------------------------------------------------- trainable block pieces
+ROPE_MAX_AXES = 4
+
+
+class _Heads(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("batch_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
+                ("token_stride", ctypes.c_int64)]
+
+
+class _AttentionShape(ctypes.Structure):
+    _fields_ = [("dtype", _I), ("batch", _S), ("heads", _S), ("q_tokens", _S), ("kv_tokens", _S), ("head_dim", _S),
+                ("scale", _F), ("q_lens", _P), ("kv_lens", _P)]
+
+
+class _RopeAxesShape(ctypes.Structure):
+    _fields_ = [("dtype", _I), ("batch", _S), ("heads", _S), ("tokens", _S), ("head_dim", _S), ("axes", _S),
+                ("sections", _S * ROPE_MAX_AXES), ("freq", _F), ("inverse", _I), ("positions_per_batch", _I)]
+
+
+class _ResidualNormShape(ctypes.Structure):
+    _fields_ = [("stream_dtype", _I), ("branch_dtype", _I), ("groups", _S), ("rows_per_group", _S), ("cols", _S),
+                ("eps", _F), ("gamma", _P), ("beta", _P), ("scale", _P), ("gate", _P), ("post_gamma", _P),
+                ("post_beta", _P)]
+
+
+class _ResidualNormGrads(ctypes.Structure):
+    _fields_ = [("d_x", _P), ("d_branch", _P), ("d_gamma", _P), ("d_beta", _P), ("d_scale", _P), ("d_gate", _P),
+                ("d_post_gamma", _P), ("d_post_beta", _P)]
+
+
+_on_stream = {}
+_on_stream_lock = threading.Lock()
+
+
+def _launch(name, device, ctx, *args) -> None:
+    """Calls an entry point on `ctx`, or on a context of `device` that follows torch's current stream there."""
+    fn = getattr(lib(), name)
+    if ctx is not None:
+        status = fn(ctx.handle, *args)
+    else:
+        import torch
+
+        # a NULL stream would mean the context's own: torch's default stream goes by its other name, cudaStreamLegacy (1)
+        stream = torch.cuda.current_stream(device).cuda_stream or 1
+        with _on_stream_lock:  # the stream and the call that is meant for it, whichever threads call
+            own = _on_stream.get(device)
+            if own is None:
+                with torch.cuda.device(device):
+                    own = _on_stream[device] = Context(device)
+            own.set_stream(stream)
+            status = fn(own.handle, *args)
+    if status != VK_OK:
+        raise VestraError(status, last_error())
+
+
+def _dtype_code(t, name):
+    import torch
+
+    if t.dtype == torch.float32:
+        return DTYPE_F32
+    if t.dtype == torch.bfloat16:
+        return DTYPE_BF16
+    raise TypeError(f"{name} must be float32 or bfloat16, got {t.dtype}")
+
+
+def _device_of(t, ctx):
+    import torch
+
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise TypeError("expected CUDA tensors")
+    if ctx is not None and ctx.device != t.device.index:
+        raise ValueError(f"the context is on device {ctx.device}, the tensors on device {t.device.index}")
+    return t.device.index
+
+
+def _view(t, name, shape, like):
+    """A vk_heads of a [batch, heads, tokens, head_dim] tensor of any strides but the last."""
+    if t.device != like.device or t.dtype != like.dtype:
+        raise TypeError(f"{name} must be {like.dtype} on {like.device}, got {t.dtype} on {t.device}")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
+    b, h, n, d = t.stride()
+    if d != 1 and shape[3] > 1:
+        raise ValueError(f"the last dimension of {name} must be contiguous")
+    return ctypes.byref(_Heads(t.data_ptr(), b, h, n))
+
+
+def _flat(t, name, shape, dtype, device):
+    """The pointer of a contiguous tensor of this shape and type, None for None."""
+    if t is None:
+        return None
+    if t.device.type != "cuda" or t.device.index != device or t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype} on cuda:{device}, got {t.dtype} on {t.device}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    return t.data_ptr()
+
+
+def _attention_shape(q, k, scale, q_lens, kv_lens, device):
+    import torch
+
+    if q.dim() != 4 or k.dim() != 4:
+        raise ValueError("q and k must be [batch, heads, tokens, head_dim]")
+    b, h, n, d = q.shape
+    return _AttentionShape(_dtype_code(q, "q"), b, h, n, k.shape[2], d, d ** -0.5 if scale is None else scale,
+                           _flat(q_lens, "q_lens", (b,), torch.int32, device),
+                           _flat(kv_lens, "kv_lens", (b,), torch.int32, device))
+
+
+def attention_forward(q, k, v, out, lse, scale=None, q_lens=None, kv_lens=None, ctx: Context | None = None) -> None:
+    """vk_attention_forward: softmax(scale q k^T) v and the rows' log-sum-exp.
+
+    q, out [batch, heads, q_tokens, head_dim] and k, v [batch, heads, kv_tokens, head_dim], f32 or bf16 CUDA tensors
+    with any order of the first three dimensions (a slice of a token-major QKV product transposed to it included);
+    lse f32 [batch, heads, q_tokens].  q_lens / kv_lens: int32 CUDA tensors [batch], the valid tokens of each
+    sequence.  Without a ctx the call runs on torch's current stream of the tensors' device."""
+    import torch
+
+    dev = _device_of(q, ctx)
+    shape = _attention_shape(q, k, scale, q_lens, kv_lens, dev)
+    qs, ks = tuple(q.shape), (*q.shape[:2], k.shape[2], q.shape[3])
+    _launch("vk_attention_forward", dev, ctx, ctypes.byref(shape), _view(q, "q", qs, q), _view(k, "k", ks, q),
+            _view(v, "v", ks, q), _view(out, "out", qs, q), _flat(lse, "lse", qs[:3], torch.float32, dev))
+
+
+def attention_backward(q, k, v, out, lse, d_out, dq, dk, dv, scale=None, q_lens=None, kv_lens=None, delta=None,
+                       ctx: Context | None = None) -> None:
+    """vk_attention_backward: the gradients dq, dk, dv of attention_forward for d_out, from its inputs, out and lse.
+
+    delta: f32 [batch, heads, q_tokens], scratch that receives the row sums of d_out * out; allocated on torch's
+    current stream where there is no ctx (with a ctx, whose stream may be another one, it is the caller's)."""
+    import torch
+
+    dev = _device_of(q, ctx)
+    shape = _attention_shape(q, k, scale, q_lens, kv_lens, dev)
+    qs, ks = tuple(q.shape), (*q.shape[:2], k.shape[2], q.shape[3])
+    if delta is None:
+        if ctx is not None:
+            raise ValueError("with a ctx, delta is given by the caller")
+        delta = torch.empty(qs[:3], dtype=torch.float32, device=q.device)
+    _launch("vk_attention_backward", dev, ctx, ctypes.byref(shape), _view(q, "q", qs, q), _view(k, "k", ks, q),
+            _view(v, "v", ks, q), _view(out, "out", qs, q), _flat(lse, "lse", qs[:3], torch.float32, dev),
+            _view(d_out, "d_out", qs, q), _view(dq, "dq", qs, q), _view(dk, "dk", ks, q), _view(dv, "dv", ks, q),
+            _flat(delta, "delta", qs[:3], torch.float32, dev))
+
+
+def rope_axes(q, k, positions, sections, freq, q_out, k_out, inverse: bool = False, ctx: Context | None = None) -> None:
+    """vk_rope_axes: rotary positions over up to four axes; axis a turns the next sections[a] elements of a head.
+
+    q, k (or None) [batch, heads, tokens, head_dim], f32 or bf16, any strides but the last; q_out, k_out may be q, k.
+    positions int64 [tokens, axes], or [batch, tokens, axes] for each batch entry's own.  inverse=True turns back,
+    which is the gradient."""
+    import torch
+
+    dev = _device_of(q, ctx)
+    if q.dim() != 4:
+        raise ValueError("q must be [batch, heads, tokens, head_dim]")
+    if not 1 <= len(sections) <= ROPE_MAX_AXES:
+        raise ValueError(f"1 to {ROPE_MAX_AXES} sections, got {len(sections)}")
+    b, h, n, d = qs = tuple(q.shape)
+    own = positions.dim() == 3
+    pos = _flat(positions, "positions", (b, n, len(sections)) if own else (n, len(sections)), torch.int64, dev)
+    shape = _RopeAxesShape(_dtype_code(q, "q"), b, h, n, d, len(sections),
+                           (_S * ROPE_MAX_AXES)(*sections), freq, int(inverse), int(own))
+    if (k is None) != (k_out is None):
+        raise ValueError("k and k_out go together")
+    _launch("vk_rope_axes", dev, ctx, ctypes.byref(shape), _view(q, "q", qs, q),
+            None if k is None else _view(k, "k", qs, q), pos, _view(q_out, "q_out", qs, q),
+            None if k is None else _view(k_out, "k_out", qs, q))
+
+
+def _residual_norm_shape(stream, branch, gamma, beta, eps, scale, gate, post_gamma, post_beta, device):
+    import torch
+
+    if stream.dim() != 3 or branch.dim() != 3:
+        raise ValueError("the stream and the branch must be [groups, rows, cols]")
+    g, t, c = stream.shape
+    f = torch.float32
+    return _ResidualNormShape(_dtype_code(stream, "the stream"), _dtype_code(branch, "the branch"), g, t, c, eps,
+                              _flat(gamma, "gamma", (c,), f, device), _flat(beta, "beta", (c,), f, device),
+                              _flat(scale, "scale", (c,), f, device), _flat(gate, "gate", (g, c), f, device),
+                              _flat(post_gamma, "post_gamma", (c,), f, device),
+                              _flat(post_beta, "post_beta", (c,), f, device))
+
+
+def residual_norm_forward(x, branch, gamma, beta, eps, h, y, stats, scale=None, gate=None, post_gamma=None,
+                          post_beta=None, post_stats=None, ctx: Context | None = None) -> None:
+    """vk_residual_norm_forward: h = x + scale * gate * n and y = LayerNorm(h; gamma, beta), with n = branch or its
+    LayerNorm (post_gamma, post_beta).
+
+    x, h [groups, rows, cols] in the residual stream's type, branch, y the same shape in the branch's: (f32, f32),
+    (f32, bf16) or (bf16, bf16), contiguous; vectors f32 [cols], gate f32 [groups, cols]; stats and post_stats f32
+    [groups, rows, 2] receive (mean, 1 / sqrt(var + eps)).  h may be x."""
+    import torch
+
+    dev = _device_of(x, ctx)
+    shape = _residual_norm_shape(x, branch, gamma, beta, eps, scale, gate, post_gamma, post_beta, dev)
+    s, rows, f = x.shape, (*x.shape[:2], 2), torch.float32
+    _launch("vk_residual_norm_forward", dev, ctx, ctypes.byref(shape), _flat(x, "x", s, x.dtype, dev),
+            _flat(branch, "branch", s, branch.dtype, dev), _flat(h, "h", s, x.dtype, dev),
+            _flat(y, "y", s, branch.dtype, dev), _flat(stats, "stats", rows, f, dev),
+            _flat(post_stats, "post_stats", rows, f, dev))
+
+
+def residual_norm_workspace(x, branch, scale=None, gate=None, post_gamma=None, ctx: Context | None = None) -> int:
+    """Bytes of the workspace that residual_norm_backward takes for these operands."""
+    dev = _device_of(x, ctx)
+    any_vector = x.data_ptr() or 16  # only whether a vector is there counts
+    g, t, c = x.shape
+    shape = _ResidualNormShape(_dtype_code(x, "x"), _dtype_code(branch, "branch"), g, t, c, 0.0, any_vector, any_vector,
+                               None if scale is None else any_vector, None if gate is None else any_vector,
+                               None if post_gamma is None else any_vector, None if post_gamma is None else any_vector)
+    need = _S()
+    _launch("vk_residual_norm_workspace", dev, ctx, ctypes.byref(shape), ctypes.byref(need))
+    return need.value
+
+
+def residual_norm_backward(d_h, d_y, h, branch, stats, gamma, d_x, d_branch, d_gamma, d_beta, scale=None, gate=None,
+                           post_gamma=None, post_beta=None, post_stats=None, d_scale=None, d_gate=None,
+                           d_post_gamma=None, d_post_beta=None, workspace=None, ctx: Context | None = None) -> None:
+    """vk_residual_norm_backward: the gradients of residual_norm_forward for d_h (of h by the residual stream; None:
+    none) and d_y, from h, branch and the statistics.
+
+    d_x may be d_h and d_branch may be d_y.  d_scale, d_gate, d_post_gamma and d_post_beta are given where their
+    vectors are.  workspace: a uint8 tensor of residual_norm_workspace(...) bytes; allocated on torch's current
+    stream where there is no ctx (with a ctx, whose stream may be another one, it is the caller's)."""
+    import torch
+
+    dev = _device_of(h, ctx)
+    f = torch.float32
+    shape = _residual_norm_shape(h, branch, gamma, gamma, 0.0, scale, gate, post_gamma, post_beta, dev)
+    s, rows, vec = h.shape, (*h.shape[:2], 2), (h.shape[2],)
+    if workspace is None:
+        if ctx is not None:
+            raise ValueError("with a ctx, the workspace is given by the caller")
+        need = residual_norm_workspace(h, branch, scale, gate, post_gamma)
+        workspace = torch.empty(need, dtype=torch.uint8, device=h.device)
+    grads = _ResidualNormGrads(_flat(d_x, "d_x", s, h.dtype, dev), _flat(d_branch, "d_branch", s, branch.dtype, dev),
+                               _flat(d_gamma, "d_gamma", vec, f, dev), _flat(d_beta, "d_beta", vec, f, dev),
+                               _flat(d_scale, "d_scale", vec, f, dev),
+                               _flat(d_gate, "d_gate", (s[0], s[2]), f, dev),
+                               _flat(d_post_gamma, "d_post_gamma", vec, f, dev),
+                               _flat(d_post_beta, "d_post_beta", vec, f, dev))
+    _launch("vk_residual_norm_backward", dev, ctx, ctypes.byref(shape), _flat(d_h, "d_h", s, h.dtype, dev),
+            _flat(d_y, "d_y", s, branch.dtype, dev), _flat(h, "h", s, h.dtype, dev),
+            _flat(branch, "branch", s, branch.dtype, dev), _flat(stats, "stats", rows, f, dev),
+            _flat(post_stats, "post_stats", rows, f, dev), ctypes.byref(grads), workspace.data_ptr(),
+            workspace.numel() * workspace.element_size())

@@ -156,6 +156,8 @@ extern "C" int vk_attention_forward(vk_ctx* ctx, const vk_attention_shape* shape
     VK_TRY(heads_view(name, "k", k, shape->dtype, B, H, a.nk, D, 16, &vk_));
     VK_TRY(heads_view(name, "v", v, shape->dtype, B, H, a.nk, D, 16, &vv));
     VK_TRY(apart(name, {vo.p, lse}, {vq.p, vk_.p, vv.p}));
+    if (bf16 && a.dim == 64)
+      return vk_cuda_status(attention_forward_tc(a, vq, vk_, vv, vo, lse, ctx->d_err, ctx->stream), name);
     return vk_cuda_status(attention_forward_simt(a, bf16, vq, vk_, vv, vo, lse, ctx->stream), name);
   });
 }
@@ -194,6 +196,8 @@ extern "C" int vk_attention_backward(vk_ctx* ctx, const vk_attention_shape* shap
     VK_TRY(heads_view(name, "d_out", d_out, shape->dtype, B, H, a.nq, D, 16, &vg));
     VK_TRY(floats_ok(name, "lse", lse));
     VK_TRY(apart(name, {vdq.p, vdk.p, vdv.p, delta}, {vq.p, vk_.p, vv.p, vo.p, vg.p, lse}));
+    if (bf16 && a.dim == 64)
+      return vk_cuda_status(attention_backward_tc(a, vq, vk_, vv, vo, lse, vg, vdq, vdk, vdv, delta, ctx->d_err, s), name);
     return vk_cuda_status(attention_backward_simt(a, bf16, vq, vk_, vv, vo, lse, vg, vdq, vdk, vdv, delta, s), name);
   });
 }

@@ -37,6 +37,12 @@ cudaError_t attention_forward_simt(const AttnShape& a, bool bf16, HeadsView q, H
 cudaError_t attention_backward_simt(const AttnShape& a, bool bf16, HeadsView q, HeadsView k, HeadsView v, HeadsView out,
                                     const float* lse, HeadsView d_out, HeadsView dq, HeadsView dk, HeadsView dv,
                                     float* delta, cudaStream_t s);
+// The same on the tensor cores, bf16, head_dim 64 (vk_attention_grad_tc.cu).
+cudaError_t attention_forward_tc(const AttnShape& a, HeadsView q, HeadsView k, HeadsView v, HeadsView out, float* lse,
+                                 int* err, cudaStream_t s);
+cudaError_t attention_backward_tc(const AttnShape& a, HeadsView q, HeadsView k, HeadsView v, HeadsView out,
+                                  const float* lse, HeadsView d_out, HeadsView dq, HeadsView dk, HeadsView dv,
+                                  float* delta, int* err, cudaStream_t s);
 // Zeros over [batch, heads, tokens, dim] / one value over n floats.
 cudaError_t zero_heads(HeadsView x, bool bf16, int batch, int heads, int tokens, int dim, cudaStream_t s);
 cudaError_t fill_f32(float* x, size_t n, float value, cudaStream_t s);

@@ -11,7 +11,8 @@
 //
 //   warp 0       TMA producer
 //   warp 1       TMEM owner; lane 0 issues the MMAs
-//   warps 2..17  the elementwise work on S (and dP) in TMEM, one row per
+//   warps 2, 3   idle: register shares go by groups of four warps
+//   warps 4..19  the elementwise work on S (and dP) in TMEM, one row per
 //                thread, the columns of a tile split between warps of the
 //                same lane quadrant
 //
@@ -30,7 +31,7 @@ namespace {
 constexpr int TR = 128;                 // rows of a tile, columns of a block
 constexpr int TILE_B = TR * 128;        // bytes of 128 rows of 64 bf16
 constexpr int ST = 4;                   // streamed blocks in flight
-constexpr int TC_THREADS = 18 * 32;
+constexpr int TC_THREADS = 20 * 32;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 __device__ __forceinline__ void tma_load_4d(void* dst, const void* desc, uint64_t* bar, int32_t y, int32_t z, int32_t w) {
@@ -61,19 +62,80 @@ __device__ __forceinline__ void zero_tail(uint8_t* a, uint8_t* b, int valid, int
   __syncwarp();
 }
 
+// Division of n < 2^31 by a constant: a few instructions where the general
+// one takes a hundred, at every item.
+struct FastDiv {
+  uint32_t mul, shift;
+  FastDiv(uint32_t d) : mul(0), shift(0) {
+    while ((uint64_t{1} << shift) < d) ++shift;
+    mul = static_cast<uint32_t>((((uint64_t{1} << shift) - d) << 32) / d + 1);
+  }
+  __device__ __forceinline__ int operator()(int n) const {
+    return static_cast<int>((__umulhi(static_cast<uint32_t>(n), mul) + static_cast<uint32_t>(n)) >> shift);
+  }
+};
+
+// The launch gives each of the 640 threads 96 registers; the elementwise warps
+// take 104 and the first four warps keep 64: 512 * 104 + 128 * 64 = 640 * 96.
+__device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 104;"); }
+__device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 64;"); }
+
+// True in one lane of a converged warp.  MMAs are issued under it: the compiler
+// knows that a single lane is active and keeps their operands in uniform
+// registers.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\tselp.u32 %0, 1, 0, e;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
+// After a wait ran out: the copies and products that are still under way must
+// not outlive the block's shared and tensor memory.  Waits for a phase whatever
+// the error word says, a tenth of a second at most.
+__device__ __forceinline__ void drain(uint64_t* bar, uint32_t parity) {
+  const uint64_t t0 = globaltimer();
+  while (!mbar_try_wait(smem_u32(bar), parity) && globaltimer() - t0 < 100000000ull) {
+  }
+}
+
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* err, int code) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, code));
 }
 
-__device__ __forceinline__ void store_bf16x16(__nv_bfloat16* p, const float* x, float f) {
-  uint4* d = reinterpret_cast<uint4*>(p);
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-    d[i] = make_uint4(pack_bf16x2(x[8 * i] * f, x[8 * i + 1] * f), pack_bf16x2(x[8 * i + 2] * f, x[8 * i + 3] * f),
-                      pack_bf16x2(x[8 * i + 4] * f, x[8 * i + 5] * f), pack_bf16x2(x[8 * i + 6] * f, x[8 * i + 7] * f));
+__device__ __forceinline__ void tma_store_4d(const void* desc, const void* src, int32_t x, int32_t y, int32_t z, int32_t w) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(desc)),
+               "r"(smem_u32(src)), "r"(x), "r"(y), "r"(z), "r"(w)
+               : "memory");
 }
-__device__ __forceinline__ void store_zero32(__nv_bfloat16* p) {  // 32 bytes
-  reinterpret_cast<uint4*>(p)[0] = reinterpret_cast<uint4*>(p)[1] = make_uint4(0, 0, 0, 0);
+
+// 16-byte piece c of row `lane` of a warp's 32 x 32 (64-byte rows) or 32 x 64
+// (128-byte rows) output staging, in the order of TMA's 64- and 128-byte
+// swizzles.  Rows leave through TMA because a thread's own stores, one row
+// each, would touch 32 lines per instruction: 2000 cycles of address work per
+// tile where an item has about 15000.
+__device__ __forceinline__ uint4* staged64(uint8_t* s, int lane, int c) {
+  return reinterpret_cast<uint4*>(s + lane * 64 + ((c ^ (lane >> 1)) & 3) * 16);
+}
+__device__ __forceinline__ uint4* staged128(uint8_t* s, int lane, int c) {
+  return reinterpret_cast<uint4*>(s + lane * 128 + ((c ^ lane) & 7) * 16);
+}
+__device__ __forceinline__ uint4 pack8(const float* x, float f) {
+  return make_uint4(pack_bf16x2(x[0] * f, x[1] * f), pack_bf16x2(x[2] * f, x[3] * f), pack_bf16x2(x[4] * f, x[5] * f),
+                    pack_bf16x2(x[6] * f, x[7] * f));
+}
+// The staged rows are on their way when this returns; the warp's lane 0 waits
+// for them (bulk_wait_read) before the staging is used again.
+__device__ __forceinline__ void send_rows(const void* desc, const uint8_t* s, int x, int y, int rows, int z, int w, int lane) {
+  fence_proxy_async();
+  __syncwarp();
+  if (lane == 0) {
+    if (y < rows) tma_store_4d(desc, s, x, y, z, w);
+    bulk_commit();
+  }
+}
+__device__ __forceinline__ void store_zeros(__nv_bfloat16* p, int n) {
+  for (int i = 0; i < n; i += 8) *reinterpret_cast<uint4*>(p + i) = make_uint4(0, 0, 0, 0);
 }
 
 // A reference to subtract from scores of which `top` is the largest so far.
@@ -101,8 +163,9 @@ constexpr size_t F_SMEM = 1024 + TILE_B * (4 + 2 * ST) + 4096 + 512;
 
 __global__ void __launch_bounds__(TC_THREADS, 1)
     k_attn_forward_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                      const __grid_constant__ CUtensorMap tmV, AttnShape a, HeadsView out, float* __restrict__ lse,
-                      int items, int per_head, int tpi, int* err) {
+                      const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO, AttnShape a,
+                      HeadsView out, float* __restrict__ lse, int items, int per_head, FastDiv by_head, FastDiv by_batch,
+                      int tpi, int* err) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;  // [item parity][tile]
@@ -111,14 +174,15 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   float2* sX = reinterpret_cast<float2*>(sV + ST * TILE_B);  // [tile][half][row] (reference, sum)
   uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(sX) + 4096);
   uint64_t* q_full = bars;           // [2] item parity
-  uint64_t* q_empty = q_full + 2;    // [2]
-  uint64_t* kv_full = q_empty + 2;   // [ST]
+  uint64_t* q_empty = q_full + 2;    // [2 parities][2 tiles]
+  uint64_t* kv_full = q_empty + 4;   // [ST]
   uint64_t* kv_empty = kv_full + ST; // [ST]
   uint64_t* s_full = kv_empty + ST;  // [2] tile: S(j) ready, every earlier product of the tile done
   uint64_t* p_full = s_full + 2;     // [2 tiles][2 halves]
   uint64_t* o_done = p_full + 4;     // [2] tile
   uint64_t* x_full = o_done + 2;     // [2] tile: references and sums of both halves written
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(x_full + 2);
+  uint64_t* stopped = x_full + 2;    // every product done, after an error
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(stopped + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   struct Item {
@@ -126,8 +190,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   };
   auto item_of = [&](int it) {
     Item r;
-    const int bh = it / per_head;
-    r.b = bh / a.heads;
+    const int bh = by_head(it);
+    r.b = by_batch(bh);
     r.h = bh - r.b * a.heads;
     r.q0 = (it - bh * per_head) * tpi * TR;
     r.nq = seq_len(a.q_lens, r.b, a.nq);
@@ -141,7 +205,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 1);
-      mbar_init(&q_empty[i], 1);
+      mbar_init(&q_empty[2 * i], 8);  // the tile's warps, once their output has left the buffer
+      mbar_init(&q_empty[2 * i + 1], 8);
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[2 * i], 4);
       mbar_init(&p_full[2 * i + 1], 4);
@@ -152,6 +217,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       mbar_init(&kv_full[i], 1);
       mbar_init(&kv_empty[i], 1);
     }
+    mbar_init(stopped, 1);
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -161,17 +227,27 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  constexpr uint32_t tmem = 0;  // all 512 columns are ours: they start at 0
 
+  if (warp < 4) regs_dec();
   if (warp == 0) {
     if (lane == 0) {
-      uint32_t g = 0;
+      uint32_t g = 0, c = 0;               // blocks, items with work
+      uint32_t used[2][2] = {{0, 0}, {0, 0}};  // [parity][tile]
       bool ok = true;
-      for (int it = blockIdx.x, c = 0; it < items && ok; it += gridDim.x) {
+      for (int it = blockIdx.x; it < items && ok; it += gridDim.x) {
         const Item I = item_of(it);
         if (I.tiles == 0) continue;
         const int qb = c & 1;
-        if (c >= 2 && !mbar_wait(&q_empty[qb], ((c >> 1) - 1) & 1, err, VK_DEV_TIMEOUT_PRODUCER)) break;
+        // a tile's buffer is handed back by the warps of that tile, for the items in which it had work
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          if (ok && t < I.tiles) {
+            uint32_t& u = qb ? used[1][t] : used[0][t];
+            if (u > 0) ok = mbar_wait(&q_empty[qb * 2 + t], (u - 1) & 1, err, VK_DEV_TIMEOUT_PRODUCER);
+            ++u;
+          }
+        if (!ok) break;
         ++c;
         mbar_arrive_expect_tx(&q_full[qb], I.tiles * TILE_B);
         for (int t = 0; t < I.tiles; ++t) tma_load_4d(sQ + (qb * 2 + t) * TILE_B, &tmQ, &q_full[qb], I.q0 + t * TR, I.h, I.b);
@@ -182,6 +258,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
           tma_load_4d(sK + st * TILE_B, &tmK, &kv_full[st], j * TR, I.h, I.b);
           tma_load_4d(sV + st * TILE_B, &tmV, &kv_full[st], j * TR, I.h, I.b);
         }
+      }
+      if (*reinterpret_cast<volatile int*>(err) != 0) {
+        for (uint32_t i = g > ST ? g - ST : 0; i < g; ++i) drain(&kv_full[i % ST], (i / ST) & 1);
+        for (uint32_t i = c > 2 ? c - 2 : 0; i < c; ++i) drain(&q_full[i & 1], (i >> 1) & 1);
       }
     }
   } else if (warp == 1) {
@@ -208,7 +288,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       if (!(ok = warp_wait(&q_full[qb], (c >> 1) & 1, err, VK_DEV_TIMEOUT_MMA) && block_ready(g, 0))) break;
       ++c;
       tc_fence_after();
-      if (lane == 0)
+      if (elect_one())
         for (int t = 0; t < I.tiles; ++t) issue_s(t, g % ST);
       for (int j = 0; j < I.nb && ok; ++j, ++g) {
         const bool more = j + 1 < I.nb;
@@ -224,7 +304,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
           for (int h = 0; h < 2; ++h) {
             if (h == 1 && j > 0 && !(ok = warp_wait(&p_full[2 * t + 1], par, err, VK_DEV_TIMEOUT_MMA))) break;
             tc_fence_after();
-            if (lane == 0) {
+            if (elect_one()) {
 #pragma unroll
               for (int k = 0; k < 4; ++k)
                 umma_f16_ts(tmem + t * 256 + 128 + h * 64, tmem + t * 256 + h * 64 + k * 8,
@@ -232,38 +312,50 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
             }
           }
           if (!ok) break;
-          if (lane == 0) {
+          if (elect_one()) {
             if (more)
               issue_s(t, (g + 1) % ST);  // after the products that read P, which it overwrites
             else
               umma_commit(&o_done[t]);
           }
         }
-        if (ok && lane == 0) umma_commit(&kv_empty[g % ST]);
+        if (ok && elect_one()) umma_commit(&kv_empty[g % ST]);
       }
-      if (ok && lane == 0) umma_commit(&q_empty[qb]);
     }
-  } else {
-    const int e = warp - 2, quad = warp & 3;
+    if (!ok) {
+      if (elect_one()) umma_commit(stopped);
+      drain(stopped, 0);
+    }
+  } else if (warp >= 4) {
+    regs_inc();
+    const int e = warp - 4, quad = warp & 3;
     const int t = e >> 3, h = (e >> 2) & 1;
     const uint32_t tb = tmem + t * 256 + (static_cast<uint32_t>(quad * 32) << 16);
     const uint32_t ts = tb + h * 64, to = tb + 128 + h * 64;
     const float sl2 = a.scale * LOG2E;
     const int trow = quad * 32 + lane;
-    uint32_t sp = 0, ct = 0;
+    uint32_t sp = 0, ct = 0, c = 0;  // blocks and items of this tile, items with work
+    int owed = -1;                   // the Q buffer whose staged output is still leaving
+    auto settle = [&]() {
+      if (owed >= 0 && lane == 0) {
+        bulk_wait_read<0>();
+        mbar_arrive(&q_empty[owed * 2 + t]);
+      }
+      owed = -1;
+    };
     bool ok = true;
-    for (int it = blockIdx.x; it < items && ok; it += gridDim.x) {
+    for (int it = blockIdx.x; it < items && ok && t < tpi; it += gridDim.x) {
       const Item I = item_of(it);
-      if (t >= tpi) break;
       const int row = I.q0 + t * TR + trow;
-      __nv_bfloat16* op = static_cast<__nv_bfloat16*>(out.p) + I.b * out.sb + I.h * out.sh + row * out.st + h * 32;
       float* lp = lse + (static_cast<size_t>(I.b) * a.heads + I.h) * a.nq + row;
+      const int qb = c & 1;
+      if (I.tiles > 0) ++c;
       if (t >= I.tiles) {  // no queries here, or no keys
         if (row < a.nq) {
-          store_zero32(op);
-          store_zero32(op + 16);
+          store_zeros(static_cast<__nv_bfloat16*>(out.p) + I.b * out.sb + I.h * out.sh + row * out.st + h * 32, 32);
           if (h == 0) *lp = -INFINITY;
         }
+        settle();
         continue;
       }
       float m_ref = -INFINITY, l_run = 0.0f;
@@ -289,49 +381,38 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
           return fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3])) * sl2;
         };
         uint32_t pk[32];
-        // p = 2^(s scale log2e - m), packed; returns the row's sum.  At the
-        // first block m is the maximum of these 64 keys.
-        auto exp_pass = [&](bool set_ref) {
-          uint32_t r[64];
-          tmem_ld32(ts, *reinterpret_cast<uint32_t(*)[32]>(&r[0]));
-          tmem_ld32(ts + 32, *reinterpret_cast<uint32_t(*)[32]>(&r[32]));
-          tmem_wait_ld();
-          if (set_ref) {
-            float pm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            if (full) {
-#pragma unroll
-              for (int i = 0; i < 64; i += 2)
-                pm[(i >> 1) & 3] = max3f(pm[(i >> 1) & 3], __uint_as_float(r[i]), __uint_as_float(r[i + 1]));
-            } else {
-#pragma unroll
-              for (int i = 0; i < 64; ++i)
-                if (i < valid) pm[i & 3] = fmaxf(pm[i & 3], __uint_as_float(r[i]));
-            }
-            m_ref = fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3])) * sl2;
-          }
+        // p = 2^(s scale log2e - m), packed; returns the row's sum
+        auto exp_pass = [&]() {
           // (where nothing but -inf came so far, the first finite score overflows the check below)
           const float m = finite_ref(m_ref);
           const float2 scale2 = make_float2(sl2, sl2), shift2 = make_float2(-m, -m);
           float2 ps[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            float2 p = exp2_pair<F_MASK>(
-                ffma2(make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), scale2, shift2), i);
-            if (!full) {
-              p.x = 2 * i < valid ? p.x : 0.0f;
-              p.y = 2 * i + 1 < valid ? p.y : 0.0f;
+          for (int c = 0; c < 2; ++c) {
+            uint32_t r[32];
+            tmem_ld32(ts + c * 32, r);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              float2 p = exp2_pair<F_MASK>(
+                  ffma2(make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), scale2, shift2), i);
+              if (!full) {
+                p.x = c * 32 + 2 * i < valid ? p.x : 0.0f;
+                p.y = c * 32 + 2 * i + 1 < valid ? p.y : 0.0f;
+              }
+              ps[i & 1] = fadd2(ps[i & 1], p);
+              pk[c * 16 + i] = pack_bf16x2(p.x, p.y);
             }
-            ps[i & 1] = fadd2(ps[i & 1], p);
-            pk[i] = pack_bf16x2(p.x, p.y);
           }
           return (ps[0].x + ps[0].y) + (ps[1].x + ps[1].y);
         };
+        if (j == 0) m_ref = half_max();
         // One pass against the running reference.  The final quotient does not
         // depend on it, so p may exceed 1; a row whose sum reaches 2^20 is done
         // again against the block's own maximum, with O and the sum rescaled
         // (the earlier products are complete: S(j) was issued after them, and
         // at the first block O is overwritten anyway).
-        float l_blk = exp_pass(j == 0);
+        float l_blk = exp_pass();
         if (__any_sync(0xffffffffu, !(l_blk < 1048576.0f))) {
           const float m_new = fmaxf(m_ref, half_max());
           const float f = ex2_approx(m_ref - finite_ref(m_new));
@@ -346,7 +427,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
           }
           l_run *= f;
           m_ref = m_new;
-          l_blk = exp_pass(false);
+          l_blk = exp_pass();
         }
         tmem_st32(ts, pk);
         tmem_wait_st();
@@ -354,6 +435,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[2 * t + h]);
         l_run += l_blk;
+        if (j == 0) settle();
       }
       if (!ok) break;
       sX[(t * 2 + h) * TR + trow] = make_float2(m_ref, l_run);
@@ -370,22 +452,28 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       const float top = finite_ref(fmaxf(x0.x, x1.x));
       const float f0 = ex2_approx(x0.x - top), f1 = ex2_approx(x1.x - top);
       const float sum = f0 * x0.y + f1 * x1.y;
-      uint32_t o0[32], o1[32];  // this warp's half of the 64 output columns
-      tmem_ld32(tb + 128 + h * 32, o0);
-      tmem_ld32(tb + 192 + h * 32, o1);
-      tmem_wait_ld();
-      tc_fence_before();
-      if (row < a.nq) {
-        const bool live = row < I.nq && sum != 0.0f;
-        const float inv = 1.0f / sum, g0 = f0 * inv, g1 = f1 * inv;
-        float o[32];
+      const bool live = row < I.nq && sum != 0.0f;
+      const float inv = 1.0f / sum, g0 = f0 * inv, g1 = f1 * inv;
+      // this warp's half of the output columns, staged over the tile's queries (every product is done with them)
+      uint8_t* stage = sQ + (qb * 2 + t) * TILE_B + (h * 4 + quad) * 2048;
 #pragma unroll
-        for (int d = 0; d < 32; ++d) o[d] = live ? fmaf(__uint_as_float(o0[d]), g0, __uint_as_float(o1[d]) * g1) : 0.0f;
-        store_bf16x16(op, o, 1.0f);
-        store_bf16x16(op + 16, o + 16, 1.0f);
-        if (h == 0) *lp = live ? fmaf(top, LN2, logf(sum)) : -INFINITY;
+      for (int d0 = 0; d0 < 32; d0 += 16) {
+        uint32_t o0[16], o1[16];
+        tmem_ld16(tb + 128 + h * 32 + d0, o0);
+        tmem_ld16(tb + 192 + h * 32 + d0, o1);
+        tmem_wait_ld();
+        float o[16];
+#pragma unroll
+        for (int d = 0; d < 16; ++d) o[d] = live ? fmaf(__uint_as_float(o0[d]), g0, __uint_as_float(o1[d]) * g1) : 0.0f;
+        *staged64(stage, lane, d0 / 8) = pack8(o, 1.0f);
+        *staged64(stage, lane, d0 / 8 + 1) = pack8(o + 8, 1.0f);
       }
+      tc_fence_before();
+      send_rows(&tmO, stage, h * 32, I.q0 + t * TR + quad * 32, a.nq, I.h, I.b, lane);
+      owed = qb;
+      if (h == 0 && row < a.nq) *lp = live ? fmaf(top, LN2, logf(sum)) : -INFINITY;
     }
+    if (lane == 0) bulk_wait<0>();
   }
   __syncthreads();
   if (warp == 1) {
@@ -398,27 +486,26 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
 // Both backward kernels run one pipeline.  A CTA walks its items (tiles of
 // 128 own rows) and the blocks of 128 streamed rows of each as one sequence of
 // blocks n = 0, 1, ...; TMEM holds S twice ([0, 128), [128, 256)), dP once
-// ([256, 384)) and the accumulators ([384, 512)).  Per block:
-//   MMA  S(n+2) = own1 . streamed1     after the products that read P/dS(n)
-//        dP(n+1) = own2 . streamed2    as soon as block n's dP has been read
-//   warps p = 2^(S scale log2e - lse log2e), then dS = p (dP - delta), written
-//        as bf16 over the columns of S they read
-// so the exponentials of a block start while its dP is still being computed,
-// and the products on P/dS(n) run under the elementwise work of n + 1.
-// Each of the 16 warps has 32 rows and 32 of the 128 columns.
+// ([256, 384)) and the accumulators ([384, 512)).  Two groups of 8 warps take
+// the even and the odd blocks.  For block n:
+//   group  p = 2^(S scale log2e - lse log2e), while dP(n) is computed; then
+//          dS = p (dP - delta); P and dS as bf16 over the columns of S
+//   MMA    dP(n+1) = own2 . streamed2   as soon as dP(n) has been read
+//          acc += P/dS(n) . streamed
+//          S(n+2) = own1 . streamed1    over the P/dS just used
+// so one group's exponentials (MUFU, 16 a clock) run beside the other's
+// products and TMEM traffic.  Each warp has 32 rows and 64 of the 128 columns.
+//
+// Between its two uses p waits as 2^15 p in f16 (32 registers instead of 64;
+// off by 2^-12 down to p = 2^-29): small next to the bf16 rounding of dS.  The
+// 2^15 goes into the exponent of 2^x, and out again with dP - delta and with
+// the result of dv.
 namespace {
 constexpr uint32_t B_MASK = 0x0u;
 constexpr uint32_t COL_DP = 256, COL_ACC = 384;
-constexpr size_t B_STATS = ST * 2 * TR * sizeof(float);  // dk/dv: (-lse log2e, delta) of the streamed rows; dq: delta's parts
-constexpr size_t B_SMEM = 1024 + TILE_B * (4 + 2 * ST) + B_STATS + 512;
-
-// One block of the walk.
-struct Blk {
-  int it, j, nb, c;  // item, block of the item and their number, ordinal of the item among those with work
-  int b, h, r0;      // sequence, head, first own row
-  int own, len;      // own and streamed rows of the sequence
-  bool ok;
-};
+constexpr float P_SHIFT = 15.0f, P_SCALE = 32768.0f;
+constexpr size_t B_STATS = ST * 2 * TR * sizeof(float);  // dk/dv: (shift, delta) of the streamed rows; dq: delta's parts
+constexpr size_t B_SMEM = 1024 + TILE_B * (4 + 2 * ST + 1) + B_STATS + 512;
 }  // namespace
 
 // DQ: own rows are queries (own1 = q, own2 = d_out), streamed ones keys
@@ -427,79 +514,73 @@ struct Blk {
 template <bool DQ>
 __global__ void __launch_bounds__(TC_THREADS, 1)
     k_attn_backward_tc(const __grid_constant__ CUtensorMap tmO1, const __grid_constant__ CUtensorMap tmO2,
-                       const __grid_constant__ CUtensorMap tmS1, const __grid_constant__ CUtensorMap tmS2, AttnShape a,
-                       HeadsView out, HeadsView d_out, const float* __restrict__ lse, float* delta, HeadsView g1,
-                       HeadsView g2, int items, int per_head, int* err) {
+                       const __grid_constant__ CUtensorMap tmS1, const __grid_constant__ CUtensorMap tmS2,
+                       const __grid_constant__ CUtensorMap tmOut, const __grid_constant__ CUtensorMap tmG1,
+                       const __grid_constant__ CUtensorMap tmG2, AttnShape a, const float* __restrict__ lse, float* delta,
+                       HeadsView g1, HeadsView g2, int items, int per_head, FastDiv by_head, FastDiv by_batch, int* err) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sOwn = smem;  // [item parity][own1, own2]
+  uint8_t* sOwn = smem;  // [item parity][own1, own2], then the item's output on its way out
   uint8_t* s1 = smem + 4 * TILE_B;
   uint8_t* s2 = s1 + ST * TILE_B;
-  float* sStat = reinterpret_cast<float*>(s2 + ST * TILE_B);
+  uint8_t* sOut = s2 + ST * TILE_B;  // dq: the item's tile of `out`, for delta
+  float* sStat = reinterpret_cast<float*>(sOut + TILE_B);
   uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(sStat) + B_STATS);
-  uint64_t* own_full = bars;           // [2]
-  uint64_t* own_empty = own_full + 2;  // [2]
-  uint64_t* st_full = own_empty + 2;   // [ST]
-  uint64_t* st_empty = st_full + ST;   // [ST]
-  uint64_t* s_full = st_empty + ST;    // [2]
-  uint64_t* dp_full = s_full + 2;
-  uint64_t* ds_full = dp_full + 1;     // P and dS of a block written, its dP read
-  uint64_t* acc_full = ds_full + 1;    // the item's last products done
-  uint64_t* part_full = acc_full + 1;  // dq: delta's parts written
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(part_full + 1);
+  uint64_t* own_full = bars;            // [2] item parity
+  uint64_t* own_empty = own_full + 2;   // [2]
+  uint64_t* st_full = own_empty + 2;    // [ST]
+  uint64_t* st_empty = st_full + ST;    // [ST]
+  uint64_t* s_full = st_empty + ST;     // [2] group
+  uint64_t* dp_full = s_full + 2;       // [2] group
+  uint64_t* ds_full = dp_full + 2;      // [2] group: P and dS of its block written, the block's dP read
+  uint64_t* acc_full = ds_full + 2;     // [2] item parity: the item's last products done
+  uint64_t* acc_free = acc_full + 2;    // the item's accumulators read
+  uint64_t* part_full = acc_free + 1;   // [2] item parity, dq: delta's parts written, the item's tile of `out` read
+  uint64_t* stopped = part_full + 2;    // every product done, after an error
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(stopped + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int total_own = DQ ? a.nq : a.nk, total_len = DQ ? a.nk : a.nq;
-  auto load_item = [&](Blk& k) {
-    const int bh = k.it / per_head;
-    k.b = bh / a.heads;
-    k.h = bh - k.b * a.heads;
-    k.r0 = (k.it - bh * per_head) * TR;
-    const int nq = seq_len(a.q_lens, k.b, a.nq), nk = seq_len(a.kv_lens, k.b, a.nk);
-    k.own = DQ ? nq : nk;
-    k.len = DQ ? nk : nq;
-    k.nb = k.r0 < k.own ? (k.len + TR - 1) / TR : 0;
+  // An item: 128 own rows of one (sequence, head), and what it streams.
+  struct Item {
+    int it, bh, r0, own, len, nb;  // own and streamed rows of the sequence, blocks
   };
-  // skipped(k) sees the items without work
-  auto seek = [&](Blk& k, auto skipped) {
-    k.j = 0;
-    while ((k.ok = k.it < items)) {
-      load_item(k);
-      if (k.nb > 0) break;
-      skipped(k);
-      k.it += gridDim.x;
+  // The first item from `it` on, in this CTA's steps, that has own rows and
+  // something to stream (it >= items: none); skipped(I) sees those before it.
+  auto seek = [&](int it, auto skipped) {
+    Item I{};
+    for (; it < items; it += gridDim.x) {
+      I.bh = by_head(it);
+      I.r0 = (it - I.bh * per_head) * TR;
+      const int b = by_batch(I.bh);
+      const int nq = seq_len(a.q_lens, b, a.nq), nk = seq_len(a.kv_lens, b, a.nk);
+      I.own = DQ ? nq : nk;
+      I.len = DQ ? nk : nq;
+      I.nb = I.r0 < I.own ? (I.len + TR - 1) / TR : 0;
+      if (I.nb > 0) break;
+      skipped(I);
     }
+    I.it = it;
+    return I;
   };
-  auto nothing = [](const Blk&) {};
-  auto first = [&](auto skipped) {
-    Blk k{};
-    k.it = blockIdx.x;
-    seek(k, skipped);
-    return k;
-  };
-  auto next = [&](Blk k, auto skipped) {
-    if (k.ok && ++k.j == k.nb) {
-      k.it += gridDim.x;
-      ++k.c;
-      seek(k, skipped);
-    }
-    return k;
-  };
+  auto nothing = [](const Item&) {};
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&own_full[i], 1);
-      mbar_init(&own_empty[i], 1);
+      mbar_init(&own_empty[i], 8);
       mbar_init(&s_full[i], 1);
+      mbar_init(&dp_full[i], 1);
+      mbar_init(&ds_full[i], 8);
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&part_full[i], 8);
     }
     for (int i = 0; i < ST; ++i) {
       mbar_init(&st_full[i], 1);
       mbar_init(&st_empty[i], 1);
     }
-    mbar_init(dp_full, 1);
-    mbar_init(ds_full, 16);
-    mbar_init(acc_full, 1);
-    mbar_init(part_full, 16);
+    mbar_init(acc_free, 8);
+    mbar_init(stopped, 1);
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -509,49 +590,75 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  constexpr uint32_t tmem = 0;  // all 512 columns are ours: they start at 0
 
+  if (warp < 4) regs_dec();
   if (warp == 0) {
-    uint32_t n = 0;
-    for (Blk k = first(nothing); k.ok; k = next(k, nothing), ++n) {
-      const int ob = k.c & 1;
-      if (k.j == 0) {
-        if (k.c >= 2 && !warp_wait(&own_empty[ob], ((k.c >> 1) - 1) & 1, err, VK_DEV_TIMEOUT_PRODUCER)) break;
-        if (lane == 0) {
-          mbar_arrive_expect_tx(&own_full[ob], 2 * TILE_B);
-          tma_load_4d(sOwn + (2 * ob) * TILE_B, &tmO1, &own_full[ob], k.r0, k.h, k.b);
-          tma_load_4d(sOwn + (2 * ob + 1) * TILE_B, &tmO2, &own_full[ob], k.r0, k.h, k.b);
-        }
-      }
-      const uint32_t st = n % ST;
-      if (!warp_wait(&st_empty[st], ((n / ST) & 1) ^ 1, err, VK_DEV_TIMEOUT_PRODUCER)) break;
-      if constexpr (!DQ) {
-        // the streamed rows' statistics; a row past the length gets -inf: its p is 2^-inf = 0
-        const size_t at = (static_cast<size_t>(k.b) * a.heads + k.h) * a.nq;
-        float l[4], d[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int row = k.j * TR + i * 32 + lane;
-          const bool in = row < k.len;
-          l[i] = in ? lse[at + row] : INFINITY;
-          d[i] = in ? delta[at + row] : 0.0f;
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          // lse = -inf: a row of scores of -inf only, whose p is 2^(-inf - 0) = 0
-          sStat[st * 2 * TR + i * 32 + lane] = l[i] == -INFINITY ? 0.0f : -l[i] * LOG2E;
-          sStat[st * 2 * TR + TR + i * 32 + lane] = d[i];
-        }
-        __syncwarp();
-      }
+    uint32_t n = 0, c = 0;        // blocks, items
+    uint32_t sent = 0, owns = 0;  // how many of them are loaded or on their way
+    bool ok = true;
+    for (Item I = seek(blockIdx.x, nothing); ok && I.it < items; I = seek(I.it + gridDim.x, nothing), ++c) {
+      const uint32_t ob = c & 1;
+      const int b = by_batch(I.bh), h = I.bh - b * a.heads;
+      if (c >= 2 && !(ok = warp_wait(&own_empty[ob], ((c >> 1) - 1) & 1, err, VK_DEV_TIMEOUT_PRODUCER))) break;
+      if (DQ && c >= 1 && !(ok = warp_wait(&part_full[(c - 1) & 1], ((c - 1) >> 1) & 1, err, VK_DEV_TIMEOUT_PRODUCER))) break;
       if (lane == 0) {
-        mbar_arrive_expect_tx(&st_full[st], 2 * TILE_B);
-        tma_load_4d(s1 + st * TILE_B, &tmS1, &st_full[st], k.j * TR, k.h, k.b);
-        tma_load_4d(s2 + st * TILE_B, &tmS2, &st_full[st], k.j * TR, k.h, k.b);
+        mbar_arrive_expect_tx(&own_full[ob], (DQ ? 3 : 2) * TILE_B);
+        tma_load_4d(sOwn + (2 * ob) * TILE_B, &tmO1, &own_full[ob], I.r0, h, b);
+        tma_load_4d(sOwn + (2 * ob + 1) * TILE_B, &tmO2, &own_full[ob], I.r0, h, b);
+        if constexpr (DQ) tma_load_4d(sOut, &tmOut, &own_full[ob], I.r0, h, b);
       }
+      owns = c + 1;
+      for (int j = 0; j < I.nb; ++j, ++n) {
+        const uint32_t st = n % ST;
+        float l[4], d[4];
+        if constexpr (!DQ) {  // the streamed rows' statistics; a row past the length gets p = 2^-inf = 0
+          const size_t at = static_cast<size_t>(I.bh) * a.nq;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int row = j * TR + i * 32 + lane;
+            l[i] = row < I.len ? lse[at + row] : INFINITY;
+            d[i] = row < I.len ? delta[at + row] : 0.0f;
+          }
+        }
+        if (!(ok = warp_wait(&st_empty[st], ((n / ST) & 1) ^ 1, err, VK_DEV_TIMEOUT_PRODUCER))) break;
+        if constexpr (!DQ) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            // lse = -inf: a row of scores of -inf only, whose p is 2^(-inf - 0) = 0
+            sStat[st * 2 * TR + i * 32 + lane] = l[i] == -INFINITY ? 0.0f : fmaf(l[i], -LOG2E, P_SHIFT);
+            sStat[st * 2 * TR + TR + i * 32 + lane] = d[i] * (-1.0f / P_SCALE);
+          }
+          __syncwarp();
+        }
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&st_full[st], 2 * TILE_B);
+          tma_load_4d(s1 + st * TILE_B, &tmS1, &st_full[st], j * TR, h, b);
+          tma_load_4d(s2 + st * TILE_B, &tmS2, &st_full[st], j * TR, h, b);
+        }
+        sent = n + 1;
+      }
+    }
+    if (*reinterpret_cast<volatile int*>(err) != 0) {
+      for (uint32_t i = sent > ST ? sent - ST : 0; i < sent; ++i) drain(&st_full[i % ST], (i / ST) & 1);
+      for (uint32_t i = owns > 2 ? owns - 2 : 0; i < owns; ++i) drain(&own_full[i & 1], (i >> 1) & 1);
     }
   } else if (warp == 1) {
     constexpr uint32_t idS = idesc_bf16(128, 128), idA = idesc_bf16_bmn(128, 64);
+    // One block of the walk: block j of nb of the c-th item with work.
+    struct Blk {
+      int it, j, nb, len;
+      uint32_t c;
+      bool ok;
+    };
+    auto load = [&](int it, uint32_t c) {
+      const Item I = seek(it, nothing);
+      return Blk{I.it, 0, I.nb, I.len, c, I.it < items};
+    };
+    auto next = [&](Blk k) {
+      if (k.ok && ++k.j == k.nb) k = load(k.it + gridDim.x, k.c + 1);
+      return k;
+    };
     // waits for a block's operands and clears what lies past the length
     auto ready = [&](const Blk& k, uint32_t n) {
       if (k.j == 0 && !warp_wait(&own_full[k.c & 1], (k.c >> 1) & 1, err, VK_DEV_TIMEOUT_MMA)) return false;
@@ -567,27 +674,26 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       for (int k = 0; k < 4; ++k) umma_f16(tmem + col, od + k * 2, sd + k * 2, idS, k > 0 ? 1u : 0u);
     };
     auto issue_s = [&](const Blk& k, uint32_t n) {
-      if (lane == 0) {
+      if (elect_one()) {
         product((n & 1) * TR, sOwn + (k.c & 1) * 2 * TILE_B, s1 + n % ST * TILE_B);
         umma_commit(&s_full[n & 1]);
       }
     };
     auto issue_dp = [&](const Blk& k, uint32_t n) {
-      if (lane == 0) {
+      if (elect_one()) {
         product(COL_DP, sOwn + ((k.c & 1) * 2 + 1) * TILE_B, s2 + n % ST * TILE_B);
-        umma_commit(dp_full);
-        if (k.j + 1 == k.nb) umma_commit(&own_empty[k.c & 1]);  // its S was issued before
+        umma_commit(&dp_full[n & 1]);
       }
     };
-    // acc += A . streamed, A = bf16 columns `col` + 32 (k / 2) + 8 (k % 2) of TMEM
+    // acc += A . streamed, A = bf16 columns `col` + 64 (k / 4) + 8 (k % 4) of TMEM
     auto sum = [&](uint32_t acc, uint32_t col, const uint8_t* streamed, bool fresh) {
       const uint64_t sd = smem_desc_mn_sw128(smem_u32(streamed));
 #pragma unroll
       for (int k = 0; k < 8; ++k)
-        umma_f16_ts(tmem + acc, tmem + col + (k >> 1) * 32 + (k & 1) * 8, sd + static_cast<uint64_t>(k * (2048 >> 4)), idA,
+        umma_f16_ts(tmem + acc, tmem + col + (k >> 2) * 64 + (k & 3) * 8, sd + static_cast<uint64_t>(k * (2048 >> 4)), idA,
                     fresh && k == 0 ? 0u : 1u);
     };
-    Blk b0 = first(nothing), b1 = next(b0, nothing), b2 = next(b1, nothing);
+    Blk b0 = load(blockIdx.x, 0), b1 = next(b0), b2 = next(b1);
     bool ok = true;
     if (b0.ok && (ok = ready(b0, 0))) {
       issue_s(b0, 0);
@@ -595,19 +701,23 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     }
     if (ok && b1.ok && (ok = ready(b1, 1))) issue_s(b1, 1);
     for (uint32_t n = 0; ok && b0.ok; ++n) {
-      if (!(ok = warp_wait(ds_full, n & 1, err, VK_DEV_TIMEOUT_MMA))) break;
+      if (!(ok = warp_wait(&ds_full[n & 1], (n >> 1) & 1, err, VK_DEV_TIMEOUT_MMA))) break;
       tc_fence_after();
       if (b1.ok) issue_dp(b1, n + 1);
-      if (lane == 0) {
+      if (b0.j == 0 && b0.c > 0) {  // the last item's accumulators have been read
+        if (!(ok = warp_wait(acc_free, (b0.c - 1) & 1, err, VK_DEV_TIMEOUT_MMA))) break;
+        tc_fence_after();
+      }
+      if (elect_one()) {
         const uint32_t col = (n & 1) * TR;
         if constexpr (DQ) {
           sum(COL_ACC, col, s1 + n % ST * TILE_B, b0.j == 0);  // dq += dS k
         } else {
           sum(COL_ACC, col, s2 + n % ST * TILE_B, b0.j == 0);            // dv += P^T d_out
-          sum(COL_ACC + 64, col + 16, s1 + n % ST * TILE_B, b0.j == 0);  // dk += dS^T q
+          sum(COL_ACC + 64, col + 32, s1 + n % ST * TILE_B, b0.j == 0);  // dk += dS^T q
         }
         umma_commit(&st_empty[n % ST]);
-        if (b0.j + 1 == b0.nb) umma_commit(acc_full);
+        if (b0.j + 1 == b0.nb) umma_commit(&acc_full[b0.c & 1]);
       }
       if (b2.ok) {
         if (!(ok = ready(b2, n + 2))) break;
@@ -615,186 +725,190 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       }
       b0 = b1;
       b1 = b2;
-      b2 = next(b2, nothing);
+      b2 = next(b2);
     }
-  } else {
-    const int quad = warp & 3, part = (warp - 2) >> 2;  // columns [32 part, 32 part + 32)
+    if (!ok) {
+      if (elect_one()) umma_commit(stopped);
+      drain(stopped, 0);
+    }
+  } else if (warp >= 4) {
+    regs_inc();
+    const int quad = warp & 3, grp = (warp - 4) >> 3, half = ((warp - 4) >> 2) & 1;  // columns [64 half, 64 half + 64)
     const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
+    const uint32_t ts = tmem + grp * TR + half * 64 + lanes, tp = tmem + COL_DP + half * 64 + lanes;
     const float sl2 = a.scale * LOG2E;
     const int trow = quad * 32 + lane;
-    // this thread's piece of its own row: dq columns [16 part, +16); dv (parts
-    // 0, 1) or dk (parts 2, 3) columns [32 (part & 1), +32)
-    auto piece = [&](const Blk& k) {
-      const HeadsView& v = DQ || part < 2 ? g1 : g2;
-      return static_cast<__nv_bfloat16*>(v.p) + k.b * v.sb + k.h * v.sh + static_cast<int64_t>(k.r0 + trow) * v.st +
-             (DQ ? part * 16 : (part & 1) * 32);
-    };
-    auto skipped = [&](const Blk& k) {  // no own rows, or nothing to stream
-      if (k.r0 + trow >= total_own) return;
-      __nv_bfloat16* p = piece(k);
-      store_zero32(p);
+    auto skipped = [&](const Item& I) {  // no own rows, or nothing to stream: zeros
+      const int row = I.r0 + trow;
+      if (grp != 0 || row >= total_own) return;
+      const HeadsView& v = DQ || half == 0 ? g1 : g2;
+      const int b = by_batch(I.bh), h = I.bh - b * a.heads;
+      __nv_bfloat16* p = static_cast<__nv_bfloat16*>(v.p) + b * v.sb + h * v.sh + row * v.st;
       if constexpr (DQ) {
-        if (part == 0) delta[(static_cast<size_t>(k.b) * a.heads + k.h) * a.nq + k.r0 + trow] = 0.0f;
+        store_zeros(p + half * 32, 32);
+        if (half == 0) delta[static_cast<size_t>(I.bh) * a.nq + row] = 0.0f;
       } else {
-        store_zero32(p + 16);
+        store_zeros(p, 64);
       }
     };
-    // own row statistics (dq): lse, and this thread's 16 of the 64 products of delta
-    float lse_next = 0.0f;
-    uint4 o_next[2], d_next[2];
-    auto fetch = [&](const Blk& k) {
-      const int row = k.r0 + trow;
-      lse_next = 0.0f;
-      o_next[0] = o_next[1] = d_next[0] = d_next[1] = make_uint4(0, 0, 0, 0);
-      if (!k.ok || row >= k.own) return;
-      lse_next = lse[(static_cast<size_t>(k.b) * a.heads + k.h) * a.nq + row];
-      const uint4* op = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(out.p) + k.b * out.sb +
-                                                       k.h * out.sh + row * out.st + part * 16);
-      const uint4* dp = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(d_out.p) + k.b * d_out.sb +
-                                                       k.h * d_out.sh + row * d_out.st + part * 16);
-      o_next[0] = op[0];
-      o_next[1] = op[1];
-      d_next[0] = dp[0];
-      d_next[1] = dp[1];
+    auto own_lse = [&](const Item& I) {
+      const int row = I.r0 + trow;
+      return I.it < items && row < I.own ? lse[static_cast<size_t>(I.bh) * a.nq + row] : 0.0f;
     };
-    auto partial_delta = [&]() {
-      const uint32_t* o = reinterpret_cast<const uint32_t*>(o_next);
-      const uint32_t* d = reinterpret_cast<const uint32_t*>(d_next);
-      float x = 0.0f, y = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        x = fmaf(__uint_as_float(o[i] << 16), __uint_as_float(d[i] << 16), x);
-        y = fmaf(__uint_as_float(o[i] & 0xffff0000u), __uint_as_float(d[i] & 0xffff0000u), y);
+    int owed = -1;  // the item whose staged output is still leaving its own tiles
+    auto settle = [&]() {
+      if (owed >= 0 && lane == 0) {
+        bulk_wait_read<0>();
+        mbar_arrive(&own_empty[owed & 1]);
       }
-      return x + y;
+      owed = -1;
     };
-    auto finish = [&](const Blk& k, uint32_t c) {  // the item's accumulators to memory
-      if (!warp_wait(acc_full, c & 1, err, VK_DEV_TIMEOUT_EPILOGUE)) return false;
+    // An item's accumulators to memory, staged over its own tiles (every
+    // product is done with them): dq columns [32 half, +32), or all of dv
+    // (half 0) or dk (half 1).
+    auto finish = [&](const Item& I, uint32_t c) {
+      if (!warp_wait(&acc_full[c & 1], (c >> 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE)) return false;
       tc_fence_after();
-      const int row = k.r0 + trow;
-      if constexpr (DQ) {
+      settle();
+      const bool live = I.r0 + trow < I.own;
+      const int b = by_batch(I.bh), h = I.bh - b * a.heads;
+      constexpr int W = DQ ? 32 : 64;
+      uint8_t* stage = sOwn + (c & 1) * 2 * TILE_B + (half * 4 + quad) * (W * 64);
+      const float f = !live ? 0.0f : DQ || half == 1 ? a.scale : 1.0f / P_SCALE;
+#pragma unroll
+      for (int d0 = 0; d0 < W; d0 += 16) {
         uint32_t r[16];
-        tmem_ld16(tmem + COL_ACC + lanes + part * 16, r);
+        tmem_ld16(tmem + COL_ACC + lanes + half * W + d0, r);
         tmem_wait_ld();
-        tc_fence_before();
-        if (row < k.own)
-          store_bf16x16(piece(k), reinterpret_cast<const float*>(r), a.scale);
-        else if (row < total_own)
-          store_zero32(piece(k));
-      } else {
-        uint32_t r[32];
-        tmem_ld32(tmem + COL_ACC + lanes + part * 32, r);
-        tmem_wait_ld();
-        tc_fence_before();
-        if (row < k.own) {
-          const float f = part < 2 ? 1.0f : a.scale;
-          store_bf16x16(piece(k), reinterpret_cast<const float*>(r), f);
-          store_bf16x16(piece(k) + 16, reinterpret_cast<const float*>(r) + 16, f);
-        } else if (row < total_own) {
-          store_zero32(piece(k));
-          store_zero32(piece(k) + 16);
+        float x[16];
+#pragma unroll
+        for (int d = 0; d < 16; ++d) x[d] = live ? __uint_as_float(r[d]) : 0.0f;
+        if constexpr (DQ) {
+          *staged64(stage, lane, d0 / 8) = pack8(x, f);
+          *staged64(stage, lane, d0 / 8 + 1) = pack8(x + 8, f);
+        } else {
+          *staged128(stage, lane, d0 / 8) = pack8(x, f);
+          *staged128(stage, lane, d0 / 8 + 1) = pack8(x + 8, f);
         }
       }
+      tc_fence_before();
+      send_rows(DQ || half == 0 ? &tmG1 : &tmG2, stage, DQ ? half * 32 : 0, I.r0 + quad * 32, total_own, h, b, lane);
+      owed = static_cast<int>(c);
+      if (lane == 0) mbar_arrive(acc_free);
       return true;
     };
-    Blk k = first(skipped), done{};
-    bool pending = false, ok = true;
-    float shift = 0.0f, dl = 0.0f;
-    if constexpr (DQ) fetch(k);
-    for (uint32_t n = 0; k.ok; ++n) {
-      const uint32_t st = n % ST, ts = tmem + (n & 1) * TR + part * 32 + lanes;
-      if (DQ && k.j == 0) shift = lse_next == -INFINITY ? 0.0f : -lse_next * LOG2E;
-      const int valid = DQ ? k.len - k.j * TR - part * 32 : 32;  // of this warp's columns (dk/dv: by the statistics)
-      if (!(ok = warp_wait(&s_full[n & 1], (n >> 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
-      tc_fence_after();
-      float p[32];
-      {
+    Item I = seek(blockIdx.x, skipped);
+    uint32_t n0 = 0, c = 0;  // blocks and items before this one
+    bool ok = true;
+    float lse_next = DQ ? own_lse(I) : 0.0f;
+    while (ok && I.it < items) {
+      const Item N = seek(I.it + gridDim.x, skipped);
+      float2 shift2, delta2 = make_float2(0.0f, 0.0f);
+      if constexpr (DQ) {
+        shift2.x = shift2.y = lse_next == -INFINITY ? 0.0f : fmaf(lse_next, -LOG2E, P_SHIFT);
+        lse_next = own_lse(N);
+      }
+      bool fresh = true;  // this group has had no block of the item yet
+      for (int j = (n0 ^ grp) & 1; j < I.nb; j += 2) {
+        const uint32_t n = n0 + j, st = n % ST;
+        const int valid = DQ ? I.len - j * TR - half * 64 : 64;  // of this warp's columns (dk/dv: by the statistics)
+        // (an item of one block has none of the other group: its tiles may be the ones still owed)
+        if (owed >= 0 && static_cast<int>(c) >= owed + 2) settle();
         if constexpr (!DQ) {  // the statistics came with the block
           if (!(ok = warp_wait(&st_full[st], (n / ST) & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
         }
-        uint32_t r[32];
-        tmem_ld32(ts, r);
-        tmem_wait_ld();
-        const float4* sl = reinterpret_cast<const float4*>(sStat + st * 2 * TR + part * 32);
+        if (!(ok = warp_wait(&s_full[grp], (n >> 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
+        tc_fence_after();
+        uint32_t ph[32];  // 2^15 p, f16
 #pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-          float2 h0 = make_float2(shift, shift), h1 = h0;
-          if constexpr (!DQ) {
-            const float4 v = sl[i / 2];
-            h0 = make_float2(v.x, v.y);
-            h1 = make_float2(v.z, v.w);
+        for (int q = 0; q < 2; ++q) {
+          uint32_t r[32], pk[16];
+          tmem_ld32(ts + q * 32, r);
+          tmem_wait_ld();
+          const float4* sl = reinterpret_cast<const float4*>(sStat + st * 2 * TR + half * 64 + q * 32);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            float2 sh = shift2;
+            if constexpr (!DQ) {
+              const float4 v = sl[i / 2];
+              sh = i & 1 ? make_float2(v.z, v.w) : make_float2(v.x, v.y);
+            }
+            float2 e = exp2_pair<B_MASK>(
+                ffma2(make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), make_float2(sl2, sl2), sh), i);
+            if (DQ && valid < 64) {
+              e.x = q * 32 + 2 * i < valid ? e.x : 0.0f;
+              e.y = q * 32 + 2 * i + 1 < valid ? e.y : 0.0f;
+            }
+            ph[q * 16 + i] = pack_f16x2(e.x, e.y);
+            if constexpr (!DQ) pk[i] = pack_bf16x2(e.x, e.y);
           }
-          const float2 e0 = exp2_pair<B_MASK>(
-              ffma2(make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), make_float2(sl2, sl2), h0), i);
-          const float2 e1 = exp2_pair<B_MASK>(
-              ffma2(make_float2(__uint_as_float(r[2 * i + 2]), __uint_as_float(r[2 * i + 3])), make_float2(sl2, sl2), h1), i + 1);
-          p[2 * i] = e0.x, p[2 * i + 1] = e0.y, p[2 * i + 2] = e1.x, p[2 * i + 3] = e1.y;
+          if constexpr (!DQ) tmem_st16(ts + q * 16, pk);  // over columns read above
         }
-        if (DQ && valid < 32) {
+        if (DQ && fresh) {
+          // delta, from the tiles of out and d_out, by the group that has the item's first block: 32 of a row's 64
+          // products per thread, which meet in shared memory
+          float* parts = sStat + (c & 1) * 2 * TR;
+          if (j == 0) {
+            if (!(ok = warp_wait(&own_full[c & 1], (c >> 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
+            const uint8_t* og = sOwn + ((c & 1) * 2 + 1) * TILE_B;
+            float x = 0.0f, y = 0.0f;
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (i >= valid) p[i] = 0.0f;
-        }
-      }
-      if constexpr (!DQ) {
-        uint32_t pk[16];
+            for (int i = 0; i < 4; ++i) {
+              const int at = trow * 128 + (((half * 4 + i) ^ trow) & 7) * 16;
+              const uint4 ov = *reinterpret_cast<const uint4*>(sOut + at), gv = *reinterpret_cast<const uint4*>(og + at);
+              const uint32_t o[4] = {ov.x, ov.y, ov.z, ov.w}, g[4] = {gv.x, gv.y, gv.z, gv.w};
 #pragma unroll
-        for (int i = 0; i < 16; ++i) pk[i] = pack_bf16x2(p[2 * i], p[2 * i + 1]);
-        tmem_st16(ts, pk);
-      }
-      if (k.j == 0) {
-        if (pending && !(ok = finish(done, done.c))) break;
-        pending = false;
-        if constexpr (DQ) {
-          float* mine = sStat + (k.c & 1) * 4 * TR;
-          mine[part * TR + trow] = partial_delta();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(part_full);
-          if (!(ok = warp_wait(part_full, k.c & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
-          dl = (mine[trow] + mine[TR + trow]) + (mine[2 * TR + trow] + mine[3 * TR + trow]);
-          if (part == 0 && k.r0 + trow < total_own)
-            delta[(static_cast<size_t>(k.b) * a.heads + k.h) * a.nq + k.r0 + trow] = dl;
-        }
-      }
-      const Blk after = next(k, skipped);
-      if constexpr (DQ) {
-        if (k.j + 1 == k.nb) fetch(after);
-      }
-      if (!(ok = warp_wait(dp_full, n & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
-      tc_fence_after();
-      {
-        uint32_t r[32], pk[16];
-        tmem_ld32(tmem + COL_DP + part * 32 + lanes, r);
-        tmem_wait_ld();
-        const float4* sd = reinterpret_cast<const float4*>(sStat + st * 2 * TR + TR + part * 32);
-#pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-          float2 h0 = make_float2(dl, dl), h1 = h0;
-          if constexpr (!DQ) {
-            const float4 v = sd[i / 2];
-            h0 = make_float2(v.x, v.y);
-            h1 = make_float2(v.z, v.w);
+              for (int u = 0; u < 4; ++u) {
+                x = fmaf(__uint_as_float(o[u] << 16), __uint_as_float(g[u] << 16), x);
+                y = fmaf(__uint_as_float(o[u] & 0xffff0000u), __uint_as_float(g[u] & 0xffff0000u), y);
+              }
+            }
+            parts[half * TR + trow] = x + y;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&part_full[c & 1]);
           }
-          const float2 d0 = fmul2(fsub2(make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), h0),
-                                  make_float2(p[2 * i], p[2 * i + 1]));
-          const float2 d1 = fmul2(fsub2(make_float2(__uint_as_float(r[2 * i + 2]), __uint_as_float(r[2 * i + 3])), h1),
-                                  make_float2(p[2 * i + 2], p[2 * i + 3]));
-          pk[i] = pack_bf16x2(d0.x, d0.y);
-          pk[i + 1] = pack_bf16x2(d1.x, d1.y);
+          if (!(ok = warp_wait(&part_full[c & 1], (c >> 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
+          const float dl = parts[trow] + parts[TR + trow];
+          delta2.x = delta2.y = dl * (-1.0f / P_SCALE);
+          const int row = I.r0 + trow;
+          if (j == 0 && half == 0 && row < total_own) delta[static_cast<size_t>(I.bh) * a.nq + row] = row < I.own ? dl : 0.0f;
         }
-        tmem_st16(DQ ? ts : ts + 16, pk);
+        fresh = false;
+        if (!(ok = warp_wait(&dp_full[grp], (n >> 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
+        tc_fence_after();
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          uint32_t r[32], pk[16];
+          tmem_ld32(tp + q * 32, r);
+          tmem_wait_ld();
+          const float4* sd = reinterpret_cast<const float4*>(sStat + st * 2 * TR + TR + half * 64 + q * 32);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            float2 dl = delta2;
+            if constexpr (!DQ) {
+              const float4 v = sd[i / 2];
+              dl = i & 1 ? make_float2(v.z, v.w) : make_float2(v.x, v.y);
+            }
+            const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&ph[q * 16 + i]));
+            const float2 ds = fmul2(ffma2(make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])),
+                                          make_float2(1.0f / P_SCALE, 1.0f / P_SCALE), dl),
+                                    p);
+            pk[i] = pack_bf16x2(ds.x, ds.y);
+          }
+          tmem_st16(ts + (DQ ? 0 : 32) + q * 16, pk);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ds_full[grp]);
+        settle();
+        if (j + 1 == I.nb && !(ok = finish(I, c))) break;
       }
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(ds_full);
-      if (k.j + 1 == k.nb) {
-        done = k;
-        pending = true;
-      }
-      k = after;
+      n0 += I.nb;
+      ++c;
+      I = N;
     }
-    if (ok && pending) finish(done, done.c);
+    if (lane == 0) bulk_wait<0>();
   }
   __syncthreads();
   if (warp == 1) {
@@ -805,19 +919,21 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
 
 // ------------------------------------------------------------------ launches
 namespace {
-bool heads_map(CUtensorMap* m, const HeadsView& v, int batch, int heads, int tokens) {
+// Boxes of `rows` rows and `cols` of the 64 columns.
+bool heads_map(CUtensorMap* m, const HeadsView& v, int batch, int heads, int tokens, uint32_t rows = TR, uint32_t cols = 64) {
   const uint64_t dims[4] = {64, static_cast<uint64_t>(tokens), static_cast<uint64_t>(heads), static_cast<uint64_t>(batch)};
   const uint64_t strides[3] = {static_cast<uint64_t>(v.st) * 2, static_cast<uint64_t>(v.sh) * 2, static_cast<uint64_t>(v.sb) * 2};
-  const uint32_t box[4] = {64, TR, 1, 1};
-  return make_tmap_nd(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, v.p, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  const uint32_t box[4] = {cols, rows, 1, 1};
+  return make_tmap_nd(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, v.p, 4, dims, strides, box,
+                      cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
 }
 }  // namespace
 
 cudaError_t attention_forward_tc(const AttnShape& a, HeadsView q, HeadsView k, HeadsView v, HeadsView out, float* lse,
                                  int* err, cudaStream_t s) {
-  CUtensorMap mq, mk, mv;
+  CUtensorMap mq, mk, mv, mo;
   if (!heads_map(&mq, q, a.batch, a.heads, a.nq) || !heads_map(&mk, k, a.batch, a.heads, a.nk) ||
-      !heads_map(&mv, v, a.batch, a.heads, a.nk))
+      !heads_map(&mv, v, a.batch, a.heads, a.nk) || !heads_map(&mo, out, a.batch, a.heads, a.nq, 32, 32))
     return cudaErrorInvalidValue;
   const void* fn = reinterpret_cast<const void*>(k_attn_forward_tc);
   const cudaError_t e = ensure_smem_limit(fn, static_cast<int>(F_SMEM));
@@ -827,28 +943,31 @@ cudaError_t attention_forward_tc(const AttnShape& a, HeadsView q, HeadsView k, H
   const int tpi = (nt + 1) / 2 * bh < num_sms() ? 1 : 2;
   const int per_head = (nt + tpi - 1) / tpi, items = per_head * bh;
   const int grid = items < num_sms() ? items : num_sms();
-  k_attn_forward_tc<<<grid, TC_THREADS, F_SMEM, s>>>(mq, mk, mv, a, out, lse, items, per_head, tpi, err);
+  k_attn_forward_tc<<<grid, TC_THREADS, F_SMEM, s>>>(mq, mk, mv, mo, a, out, lse, items, per_head, FastDiv(per_head),
+                                                     FastDiv(a.heads), tpi, err);
   return cudaGetLastError();
 }
 
 cudaError_t attention_backward_tc(const AttnShape& a, HeadsView q, HeadsView k, HeadsView v, HeadsView out,
                                   const float* lse, HeadsView d_out, HeadsView dq, HeadsView dk, HeadsView dv,
                                   float* delta, int* err, cudaStream_t s) {
-  CUtensorMap mq, mk, mv, mg;
+  CUtensorMap mq, mk, mv, mg, mo, mdq, mdk, mdv;
   if (!heads_map(&mq, q, a.batch, a.heads, a.nq) || !heads_map(&mk, k, a.batch, a.heads, a.nk) ||
-      !heads_map(&mv, v, a.batch, a.heads, a.nk) || !heads_map(&mg, d_out, a.batch, a.heads, a.nq))
+      !heads_map(&mv, v, a.batch, a.heads, a.nk) || !heads_map(&mg, d_out, a.batch, a.heads, a.nq) ||
+      !heads_map(&mo, out, a.batch, a.heads, a.nq) || !heads_map(&mdq, dq, a.batch, a.heads, a.nq, 32, 32) ||
+      !heads_map(&mdk, dk, a.batch, a.heads, a.nk, 32) || !heads_map(&mdv, dv, a.batch, a.heads, a.nk, 32))
     return cudaErrorInvalidValue;
   cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(k_attn_backward_tc<true>), static_cast<int>(B_SMEM));
   if (e == cudaSuccess) e = ensure_smem_limit(reinterpret_cast<const void*>(k_attn_backward_tc<false>), static_cast<int>(B_SMEM));
   if (e != cudaSuccess) return e;
   const int bh = a.batch * a.heads, sms = num_sms();
   const int qt = (a.nq + TR - 1) / TR, kt = (a.nk + TR - 1) / TR;
-  k_attn_backward_tc<true><<<qt * bh < sms ? qt * bh : sms, TC_THREADS, B_SMEM, s>>>(mq, mg, mk, mv, a, out, d_out, lse, delta,
-                                                                                    dq, dq, qt * bh, qt, err);
+  k_attn_backward_tc<true><<<qt * bh < sms ? qt * bh : sms, TC_THREADS, B_SMEM, s>>>(
+      mq, mg, mk, mv, mo, mdq, mdq, a, lse, delta, dq, dq, qt * bh, qt, FastDiv(qt), FastDiv(a.heads), err);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  k_attn_backward_tc<false><<<kt * bh < sms ? kt * bh : sms, TC_THREADS, B_SMEM, s>>>(mk, mv, mq, mg, a, out, d_out, lse, delta,
-                                                                                     dv, dk, kt * bh, kt, err);
+  k_attn_backward_tc<false><<<kt * bh < sms ? kt * bh : sms, TC_THREADS, B_SMEM, s>>>(
+      mk, mv, mq, mg, mo, mdv, mdk, a, lse, delta, dv, dk, kt * bh, kt, FastDiv(kt), FastDiv(a.heads), err);
   return cudaGetLastError();
 }
 

@@ -109,13 +109,13 @@ __device__ __forceinline__ void tma_store_4d(const void* desc, const void* src, 
                : "memory");
 }
 
-// 16-byte piece c of row `lane` of a warp's output staging, 32 rows of ROW (32
-// or 64) bytes in the order of TMA's swizzle of that width.  Rows leave through TMA because a thread's own stores, one row
+// 16-byte piece c of row `lane` of a warp's output staging, 32 rows of ROW (64
+// or 128) bytes in the order of TMA's swizzle of that width.  Rows leave through TMA because a thread's own stores, one row
 // each, would touch 32 lines per instruction: 2000 cycles of address work per
 // tile where an item has about 15000.
 template <int ROW>
 __device__ __forceinline__ uint4* staged(uint8_t* s, int lane, int c) {
-  if constexpr (ROW == 32) return reinterpret_cast<uint4*>(s + lane * 32 + ((c ^ (lane >> 2)) & 1) * 16);
+  if constexpr (ROW == 128) return reinterpret_cast<uint4*>(s + lane * 128 + ((c ^ lane) & 7) * 16);
   return reinterpret_cast<uint4*>(s + lane * 64 + ((c ^ (lane >> 1)) & 3) * 16);
 }
 __device__ __forceinline__ uint4 pack8(const float* x, float f) {
@@ -492,22 +492,27 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
 // Both backward kernels run one pipeline.  A CTA walks its items (tiles of
 // 128 own rows) and the blocks of 128 streamed rows of each as one sequence of
 // blocks n = 0, 1, ...  TMEM: S [0, 128), dP [128, 256), P and dS as bf16
-// [256, 384), accumulators [384, 512).  For block n each of the 16 warps, with
-// 32 rows and 32 of the 128 columns,
-//   reads S and hands it back   -> MMA: S(n+1) = own1 . streamed1
-//   p = 2^(S scale log2e - lse log2e)
-//   reads dP and hands it back  -> MMA: dP(n+1) = own2 . streamed2
-//   dS = p (dP - delta); writes P and dS
-//                               -> MMA: acc += P/dS(n) . streamed
-// S and dP are handed back as soon as they are in registers, so the next
-// block's are there before the warps are done with this one, and the warps,
-// which may be up to a block apart, keep MUFU (the exponentials, 16 a clock),
-// the FMA pipes and the tensor core busy side by side.  P and dS over the
-// columns of S (with S twice and dP once) tied S(n+2) to the products of
-// block n: 2600 and 3100 cycles a block.
+// [256, 384), accumulators [384, 512).  Two groups of 8 warps take the even
+// and the odd blocks; each warp has 32 rows and 64 of the 128 columns:
+//   reads S and hands it back   -> MMA: the next block's S = own1 . streamed1
+//   p = 2^(S scale log2e - lse log2e); dk/dv: writes P
+//                               -> MMA: dv += P^T . streamed2
+//   reads dP and hands it back  -> MMA: the next block's dP = own2 . streamed2
+//   dS = p (dP - delta); writes dS
+//                               -> MMA: dk (dq) += dS . streamed1
+// S and dP are handed back as soon as they are in registers, so the other
+// group's are there before it asks, and one group's exponentials (MUFU, 16 a
+// clock) run beside the other's products and TMEM traffic.  With all 16 warps
+// on one block the phases followed one another: 2500 and 3000 cycles a block.
+//
+// Between its two uses p waits as 2^15 p in f16 (32 registers instead of 64;
+// off by 2^-12 down to p = 2^-29): small next to the bf16 rounding of dS.  The
+// 2^15 goes into the exponent of 2^x, and out again with dP - delta and with
+// the result of dv.
 namespace {
 constexpr uint32_t B_MASK = 0x0u;
 constexpr uint32_t COL_DP = 128, COL_P = 256, COL_ACC = 384;
+constexpr float P_SHIFT = 15.0f, P_SCALE = 32768.0f;
 constexpr size_t B_STATS = ST * 2 * TR * sizeof(float);  // dk/dv: (shift, delta) of the streamed rows; dq: delta's parts
 constexpr size_t B_SMEM = 1024 + TILE_B * (4 + 2 * ST + 1) + B_STATS + 512;
 }  // namespace
@@ -534,15 +539,18 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   uint64_t* own_empty = own_full + 2;   // [2]
   uint64_t* st_full = own_empty + 2;    // [ST]
   uint64_t* st_empty = st_full + ST;    // [ST]
-  uint64_t* s_full = st_empty + ST;
-  uint64_t* s_free = s_full + 1;        // S read
-  uint64_t* dp_full = s_free + 1;
-  uint64_t* dp_free = dp_full + 1;      // dP read
-  uint64_t* ds_full = dp_free + 1;      // [2] block parity: P and dS written (a dq warp may be a block ahead here)
-  uint64_t* ds_free = ds_full + 2;      // [2] P and dS (dq: one of two dS) used
-  uint64_t* acc_full = ds_free + 2;     // [2] item parity: the item's last products done
+  uint64_t* s_full = st_empty + ST;     // [2] group
+  uint64_t* dp_full = s_full + 2;       // [2] group
+  uint64_t* ds_full = dp_full + 2;      // [2] group: dS written
+  uint64_t* acc_full = ds_full + 2;     // [2] item parity: the item's last products done
   uint64_t* part_full = acc_full + 2;   // [2] item parity, dq: delta's parts written, the item's tile of `out` read
-  uint64_t* stopped = part_full + 2;    // every product done, after an error
+  uint64_t* s_free = part_full + 2;     // S read
+  uint64_t* dp_free = s_free + 1;       // dP read
+  uint64_t* p_full = dp_free + 1;       // dk/dv: P written
+  uint64_t* p_free = p_full + 1;        // dk/dv: P used
+  uint64_t* ds_free = p_free + 1;       // dk/dv: dS used
+  uint64_t* acc_free = ds_free + 1;     // the item's accumulators read
+  uint64_t* stopped = acc_free + 1;     // every product done, after an error
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(stopped + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -574,16 +582,19 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&own_full[i], 1);
-      mbar_init(&own_empty[i], 16);
-      mbar_init(&ds_full[i], 16);
-      mbar_init(&ds_free[i], 1);
+      mbar_init(&own_empty[i], 8);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&dp_full[i], 1);
+      mbar_init(&ds_full[i], 8);
       mbar_init(&acc_full[i], 1);
-      mbar_init(&part_full[i], 16);
+      mbar_init(&part_full[i], 8);
     }
-    mbar_init(s_full, 1);
-    mbar_init(s_free, 16);
-    mbar_init(dp_full, 1);
-    mbar_init(dp_free, 16);
+    mbar_init(s_free, 8);
+    mbar_init(dp_free, 8);
+    mbar_init(p_full, 8);
+    mbar_init(p_free, 1);
+    mbar_init(ds_free, 1);
+    mbar_init(acc_free, 8);
     for (int i = 0; i < ST; ++i) {
       mbar_init(&st_full[i], 1);
       mbar_init(&st_empty[i], 1);
@@ -634,8 +645,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             // lse = -inf: a row of scores of -inf only, whose p is 2^(-inf - 0) = 0
-            sStat[st * 2 * TR + i * 32 + lane] = l[i] == -INFINITY ? 0.0f : -l[i] * LOG2E;
-            sStat[st * 2 * TR + TR + i * 32 + lane] = d[i];
+            sStat[st * 2 * TR + i * 32 + lane] = l[i] == -INFINITY ? 0.0f : fmaf(l[i], -LOG2E, P_SHIFT);
+            sStat[st * 2 * TR + TR + i * 32 + lane] = d[i] * (-1.0f / P_SCALE);
           }
           __syncwarp();
         }
@@ -684,13 +695,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     auto issue_s = [&](const Blk& k, uint32_t n) {
       if (elect_one()) {
         product(0, sOwn + (k.c & 1) * 2 * TILE_B, s1 + n % ST * TILE_B);
-        umma_commit(s_full);
+        umma_commit(&s_full[n & 1]);
       }
     };
     auto issue_dp = [&](const Blk& k, uint32_t n) {
       if (elect_one()) {
         product(COL_DP, sOwn + ((k.c & 1) * 2 + 1) * TILE_B, s2 + n % ST * TILE_B);
-        umma_commit(dp_full);
+        umma_commit(&dp_full[n & 1]);
       }
     };
     // acc += A . streamed, A = 64 columns of TMEM from `col` on
@@ -700,36 +711,57 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       for (int k = 0; k < 8; ++k)
         umma_f16_ts(tmem + acc, tmem + col + k * 8, sd + static_cast<uint64_t>(k * (2048 >> 4)), idA, fresh && k == 0 ? 0u : 1u);
     };
-    Blk b0 = load(blockIdx.x, 0), b1 = next(b0);
+    // the last item's accumulators have been read
+    auto acc_ready = [&](const Blk& k) {
+      return k.j > 0 || k.c == 0 || warp_wait(acc_free, (k.c - 1) & 1, err, VK_DEV_TIMEOUT_MMA);
+    };
+    Blk b0 = load(blockIdx.x, 0), b1 = next(b0), b2 = next(b1);
     bool ok = true;
+    auto next_s = [&](const Blk& k, uint32_t n) {  // S of block n, once block n - 1's has been read
+      if (!(ok = ready(k, n) && warp_wait(s_free, (n - 1) & 1, err, VK_DEV_TIMEOUT_MMA))) return;
+      tc_fence_after();
+      issue_s(k, n);
+    };
     if (b0.ok && (ok = ready(b0, 0))) {
       issue_s(b0, 0);
       issue_dp(b0, 0);
     }
+    if (ok && b1.ok) next_s(b1, 1);
     for (uint32_t n = 0; ok && b0.ok; ++n) {
-      if (b1.ok) {
-        if (!(ok = ready(b1, n + 1) && warp_wait(s_free, n & 1, err, VK_DEV_TIMEOUT_MMA))) break;
+      if constexpr (!DQ) {
+        if (!(ok = warp_wait(p_full, n & 1, err, VK_DEV_TIMEOUT_MMA) && acc_ready(b0))) break;
         tc_fence_after();
-        issue_s(b1, n + 1);
+        if (elect_one()) {
+          sum(COL_ACC, COL_P, s2 + n % ST * TILE_B, b0.j == 0);  // dv += P^T d_out
+          umma_commit(p_free);
+        }
+      }
+      // S(n+2) early -- unless its item takes over the tiles of block n's
+      const bool late = b2.c >= b0.c + 2;
+      if (b2.ok && !late) next_s(b2, n + 2);
+      if (!ok) break;
+      if (b1.ok) {
         if (!(ok = warp_wait(dp_free, n & 1, err, VK_DEV_TIMEOUT_MMA))) break;
         tc_fence_after();
         issue_dp(b1, n + 1);
       }
       if (!(ok = warp_wait(&ds_full[n & 1], (n >> 1) & 1, err, VK_DEV_TIMEOUT_MMA))) break;
+      if (DQ && !(ok = acc_ready(b0))) break;
       tc_fence_after();
       if (elect_one()) {
         if constexpr (DQ) {
           sum(COL_ACC, COL_P + (n & 1) * 64, s1 + n % ST * TILE_B, b0.j == 0);  // dq += dS k
         } else {
-          sum(COL_ACC, COL_P, s2 + n % ST * TILE_B, b0.j == 0);            // dv += P^T d_out
           sum(COL_ACC + 64, COL_P + 64, s1 + n % ST * TILE_B, b0.j == 0);  // dk += dS^T q
+          umma_commit(ds_free);
         }
         umma_commit(&st_empty[n % ST]);
-        umma_commit(&ds_free[DQ ? n & 1 : 0]);
         if (b0.j + 1 == b0.nb) umma_commit(&acc_full[b0.c & 1]);
       }
+      if (b2.ok && late) next_s(b2, n + 2);
       b0 = b1;
-      b1 = next(b1);
+      b1 = b2;
+      b2 = next(b2);
     }
     if (!ok) {
       if (elect_one()) umma_commit(stopped);
@@ -737,38 +769,48 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     }
   } else if (warp >= 4) {
     regs_inc();
-    const int quad = warp & 3, part = (warp - 4) >> 2;  // columns [32 part, 32 part + 32)
+    const int quad = warp & 3, grp = (warp - 4) >> 3, half = ((warp - 4) >> 2) & 1;  // columns [64 half, 64 half + 64)
     const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
-    const uint32_t ts = tmem + part * 32 + lanes, tp = tmem + COL_P + part * 16 + lanes;
+    const uint32_t ts = tmem + half * 64 + lanes;
+    // dk/dv: P at COL_P, dS 64 columns on; dq: a dS for each group
+    const uint32_t tp = tmem + COL_P + half * 32 + lanes, td = tp + (DQ ? grp * 64 : 64);
     const float sl2 = a.scale * LOG2E;
     const int trow = quad * 32 + lane;
-    constexpr int W = DQ ? 16 : 32;  // this warp's columns of the results: dq, or dv (parts 0, 1) and dk (parts 2, 3)
-    const int out_col = DQ ? part * 16 : (part & 1) * 32;
+    constexpr int W = DQ ? 32 : 64;  // this warp's columns of the results: half of dq, or all of dv (half 0) or dk (half 1)
     auto skipped = [&](const Item& I) {  // no own rows, or nothing to stream: zeros
       const int row = I.r0 + trow;
-      if (row >= total_own) return;
-      const HeadsView& v = DQ || part < 2 ? g1 : g2;
+      if (grp != 0 || row >= total_own) return;
+      const HeadsView& v = DQ || half == 0 ? g1 : g2;
       const int b = by_batch(I.bh), h = I.bh - b * a.heads;
-      store_zeros(static_cast<__nv_bfloat16*>(v.p) + b * v.sb + h * v.sh + row * v.st + out_col, W);
-      if (DQ && part == 0) delta[static_cast<size_t>(I.bh) * a.nq + row] = 0.0f;
+      store_zeros(static_cast<__nv_bfloat16*>(v.p) + b * v.sb + h * v.sh + row * v.st + (DQ ? half * 32 : 0), W);
+      if (DQ && half == 0) delta[static_cast<size_t>(I.bh) * a.nq + row] = 0.0f;
     };
     auto own_lse = [&](const Item& I) {
       const int row = I.r0 + trow;
       return I.it < items && row < I.own ? lse[static_cast<size_t>(I.bh) * a.nq + row] : 0.0f;
     };
-    // An item's accumulators to memory, staged over its own tiles (every
-    // product is done with them).
+    int owed = -1;  // the item whose staged output is still leaving its own tiles
+    auto settle = [&]() {
+      if (owed >= 0 && lane == 0) {
+        bulk_wait_read<0>();
+        mbar_arrive(&own_empty[owed & 1]);
+      }
+      owed = -1;
+    };
+    // An item's accumulators to memory, by the group that had its last block,
+    // staged over its own tiles (every product is done with them).
     auto finish = [&](const Item& I, uint32_t c) {
       if (!warp_wait(&acc_full[c & 1], (c >> 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE)) return false;
       tc_fence_after();
+      settle();
       const bool live = I.r0 + trow < I.own;
       const int b = by_batch(I.bh), h = I.bh - b * a.heads;
-      uint8_t* stage = sOwn + (c & 1) * 2 * TILE_B + (part * 4 + quad) * (W * 64);
-      const float f = DQ || part >= 2 ? a.scale : 1.0f;
+      uint8_t* stage = sOwn + (c & 1) * 2 * TILE_B + (half * 4 + quad) * (W * 64);
+      const float f = DQ || half == 1 ? a.scale : 1.0f / P_SCALE;
 #pragma unroll
       for (int d0 = 0; d0 < W; d0 += 16) {
         uint32_t r[16];
-        tmem_ld16(tmem + COL_ACC + lanes + part * W + d0, r);
+        tmem_ld16(tmem + COL_ACC + lanes + half * W + d0, r);
         tmem_wait_ld();
         float x[16];
 #pragma unroll
@@ -777,38 +819,48 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         *staged<W * 2>(stage, lane, d0 / 8 + 1) = pack8(x + 8, f);
       }
       tc_fence_before();
-      send_rows(DQ || part < 2 ? &tmG1 : &tmG2, stage, out_col, I.r0 + quad * 32, total_own, h, b, lane);
+      send_rows(DQ || half == 0 ? &tmG1 : &tmG2, stage, DQ ? half * 32 : 0, I.r0 + quad * 32, total_own, h, b, lane);
+      owed = static_cast<int>(c);
+      if (lane == 0) mbar_arrive(acc_free);
       return true;
     };
-    Item I = seek(blockIdx.x, skipped), last{};
-    uint32_t n = 0, c = 0;  // blocks, items
+    Item I = seek(blockIdx.x, skipped);
+    uint32_t n0 = 0, c = 0;  // blocks and items before this one
     bool ok = true;
     float lse_next = DQ ? own_lse(I) : 0.0f;
     while (ok && I.it < items) {
       const Item N = seek(I.it + gridDim.x, skipped);
       float2 shift2, delta2 = make_float2(0.0f, 0.0f);
       if constexpr (DQ) {
-        shift2.x = shift2.y = lse_next == -INFINITY ? 0.0f : -lse_next * LOG2E;
+        shift2.x = shift2.y = lse_next == -INFINITY ? 0.0f : fmaf(lse_next, -LOG2E, P_SHIFT);
         lse_next = own_lse(N);
       }
-      for (int j = 0; j < I.nb; ++j, ++n) {
-        const uint32_t st = n % ST;
-        const int valid = DQ ? I.len - j * TR - part * 32 : 32;  // of this warp's columns (dk/dv: by the statistics)
+      bool fresh = true;  // this group has had no block of the item yet
+      for (int j = (n0 ^ grp) & 1; j < I.nb; j += 2) {
+        const uint32_t n = n0 + j, st = n % ST;
+        // (after items of one block, this item's tiles may be the ones still owed)
+        if (owed >= 0 && static_cast<int>(c) >= owed + 2) settle();
         if constexpr (!DQ) {  // the statistics came with the block
           if (!(ok = warp_wait(&st_full[st], (n / ST) & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
         }
-        if (!(ok = warp_wait(s_full, n & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
+        if (!(ok = warp_wait(&s_full[grp], (n >> 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
         tc_fence_after();
-        float p[32];
-        {
+        uint32_t ph[32], pk[DQ ? 1 : 32];  // 2^15 p as f16, and as bf16 for dv
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
           uint32_t r[32];
-          tmem_ld32(ts, r);
+          tmem_ld32(ts + q * 32, r);
           tmem_wait_ld();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(s_free);
-          if (DQ && valid < 32) mask_columns(r, valid);
-          const float4* sl = reinterpret_cast<const float4*>(sStat + st * 2 * TR + part * 32);
+          if (q == 1) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(s_free);
+          }
+          if constexpr (DQ) {
+            const int valid = I.len - j * TR - half * 64 - q * 32;
+            if (valid < 32) mask_columns(r, valid);
+          }
+          const float4* sl = reinterpret_cast<const float4*>(sStat + st * 2 * TR + half * 64 + q * 32);
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             float2 sh = shift2;
@@ -818,19 +870,22 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
             }
             const float2 e = exp2_pair<B_MASK>(
                 ffma2(make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), make_float2(sl2, sl2), sh), i);
-            p[2 * i] = e.x, p[2 * i + 1] = e.y;
+            ph[q * 16 + i] = pack_f16x2(e.x, e.y);
+            if constexpr (!DQ) pk[q * 16 + i] = pack_bf16x2(e.x, e.y);
           }
         }
-        if (j == 0) {
-          if (c > 0 && !(ok = finish(last, c - 1))) break;
-          if constexpr (DQ) {
-            // delta, from the tiles of out and d_out: 16 of a row's 64 products per thread, which meet in shared memory
+        settle();
+        if (DQ && fresh) {
+          // delta, from the tiles of out and d_out, by the group that has the item's first block: 32 of a row's 64
+          // products per thread, which meet in shared memory
+          float* parts = sStat + (c & 1) * 2 * TR;
+          if (j == 0) {
             if (!(ok = warp_wait(&own_full[c & 1], (c >> 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
             const uint8_t* og = sOwn + ((c & 1) * 2 + 1) * TILE_B;
             float x = 0.0f, y = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const int at = trow * 128 + (((part * 2 + i) ^ trow) & 7) * 16;
+            for (int i = 0; i < 4; ++i) {
+              const int at = trow * 128 + (((half * 4 + i) ^ trow) & 7) * 16;
               const uint4 ov = *reinterpret_cast<const uint4*>(sOut + at), gv = *reinterpret_cast<const uint4*>(og + at);
               const uint32_t o[4] = {ov.x, ov.y, ov.z, ov.w}, g[4] = {gv.x, gv.y, gv.z, gv.w};
 #pragma unroll
@@ -839,35 +894,40 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
                 y = fmaf(__uint_as_float(o[u] & 0xffff0000u), __uint_as_float(g[u] & 0xffff0000u), y);
               }
             }
-            float* parts = sStat + (c & 1) * 4 * TR;
-            parts[part * TR + trow] = x + y;
+            parts[half * TR + trow] = x + y;
             __syncwarp();
             if (lane == 0) mbar_arrive(&part_full[c & 1]);
-            if (!(ok = warp_wait(&part_full[c & 1], (c >> 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
-            const float dl = (parts[trow] + parts[TR + trow]) + (parts[2 * TR + trow] + parts[3 * TR + trow]);
-            delta2.x = delta2.y = dl;
-            const int row = I.r0 + trow;
-            if (part == 0 && row < total_own) delta[static_cast<size_t>(I.bh) * a.nq + row] = row < I.own ? dl : 0.0f;
           }
+          if (!(ok = warp_wait(&part_full[c & 1], (c >> 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
+          const float dl = parts[trow] + parts[TR + trow];
+          delta2.x = delta2.y = dl * (-1.0f / P_SCALE);
+          const int row = I.r0 + trow;
+          if (j == 0 && half == 0 && row < total_own) delta[static_cast<size_t>(I.bh) * a.nq + row] = row < I.own ? dl : 0.0f;
         }
+        fresh = false;
         if constexpr (!DQ) {
-          uint32_t pk[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) pk[i] = pack_bf16x2(p[2 * i], p[2 * i + 1]);
-          if (n > 0 && !(ok = warp_wait(&ds_free[0], (n - 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
+          if (n > 0 && !(ok = warp_wait(p_free, (n - 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
           tc_fence_after();
-          tmem_st16(tp, pk);
-        }
-        if (!(ok = warp_wait(dp_full, n & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
-        tc_fence_after();
-        {
-          uint32_t r[32], pk[16];
-          tmem_ld32(ts + COL_DP, r);
-          tmem_wait_ld();
+          tmem_st32(tp, pk);
+          tmem_wait_st();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(dp_free);
-          const float4* sd = reinterpret_cast<const float4*>(sStat + st * 2 * TR + TR + part * 32);
+          if (lane == 0) mbar_arrive(p_full);
+        }
+        if (!(ok = warp_wait(&dp_full[grp], (n >> 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
+        tc_fence_after();
+        uint32_t dk[32];
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          uint32_t r[32];
+          tmem_ld32(ts + COL_DP + q * 32, r);
+          tmem_wait_ld();
+          if (q == 1) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(dp_free);
+          }
+          const float4* sd = reinterpret_cast<const float4*>(sStat + st * 2 * TR + TR + half * 64 + q * 32);
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             float2 dl = delta2;
@@ -875,34 +935,27 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
               const float4 v = sd[i / 2];
               dl = i & 1 ? make_float2(v.z, v.w) : make_float2(v.x, v.y);
             }
-            const float2 ds = fmul2(fsub2(make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), dl),
-                                    make_float2(p[2 * i], p[2 * i + 1]));
-            pk[i] = pack_bf16x2(ds.x, ds.y);
-          }
-          if constexpr (DQ) {
-            if (n > 1 && !(ok = warp_wait(&ds_free[n & 1], ((n >> 1) - 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
-            tc_fence_after();
-            tmem_st16(tp + (n & 1) * 64, pk);
-          } else {
-            tmem_st16(tp + 64, pk);
+            const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&ph[q * 16 + i]));
+            const float2 ds = fmul2(ffma2(make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])),
+                                          make_float2(1.0f / P_SCALE, 1.0f / P_SCALE), dl),
+                                    p);
+            dk[q * 16 + i] = pack_bf16x2(ds.x, ds.y);
           }
         }
+        // (dq: this group's last dS was used before dP(n) was computed)
+        if (!DQ && n > 0 && !(ok = warp_wait(ds_free, (n - 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
+        tc_fence_after();
+        tmem_st32(td, dk);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&ds_full[n & 1]);
-          if (j == 0 && c > 0) {  // the last item's rows have left its tiles
-            bulk_wait_read<0>();
-            mbar_arrive(&own_empty[(c - 1) & 1]);
-          }
-        }
+        if (lane == 0) mbar_arrive(&ds_full[grp]);
+        if (j + 1 == I.nb && !(ok = finish(I, c))) break;
       }
-      last = I;
-      I = N;
+      n0 += I.nb;
       ++c;
+      I = N;
     }
-    if (ok && c > 0) finish(last, c - 1);
     if (lane == 0) bulk_wait<0>();
   }
   __syncthreads();
@@ -920,9 +973,7 @@ bool heads_map(CUtensorMap* m, const HeadsView& v, int batch, int heads, int tok
   const uint64_t strides[3] = {static_cast<uint64_t>(v.st) * 2, static_cast<uint64_t>(v.sh) * 2, static_cast<uint64_t>(v.sb) * 2};
   const uint32_t box[4] = {cols, rows, 1, 1};
   return make_tmap_nd(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, v.p, 4, dims, strides, box,
-                      cols == 64   ? CU_TENSOR_MAP_SWIZZLE_128B
-                      : cols == 32 ? CU_TENSOR_MAP_SWIZZLE_64B
-                                   : CU_TENSOR_MAP_SWIZZLE_32B);
+                      cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
 }
 }  // namespace
 
@@ -951,8 +1002,8 @@ cudaError_t attention_backward_tc(const AttnShape& a, HeadsView q, HeadsView k, 
   CUtensorMap mq, mk, mv, mg, mo, mdq, mdk, mdv;
   if (!heads_map(&mq, q, a.batch, a.heads, a.nq) || !heads_map(&mk, k, a.batch, a.heads, a.nk) ||
       !heads_map(&mv, v, a.batch, a.heads, a.nk) || !heads_map(&mg, d_out, a.batch, a.heads, a.nq) ||
-      !heads_map(&mo, out, a.batch, a.heads, a.nq) || !heads_map(&mdq, dq, a.batch, a.heads, a.nq, 32, 16) ||
-      !heads_map(&mdk, dk, a.batch, a.heads, a.nk, 32, 32) || !heads_map(&mdv, dv, a.batch, a.heads, a.nk, 32, 32))
+      !heads_map(&mo, out, a.batch, a.heads, a.nq) || !heads_map(&mdq, dq, a.batch, a.heads, a.nq, 32, 32) ||
+      !heads_map(&mdk, dk, a.batch, a.heads, a.nk, 32) || !heads_map(&mdv, dv, a.batch, a.heads, a.nk, 32))
     return cudaErrorInvalidValue;
   cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(k_attn_backward_tc<true>), static_cast<int>(B_SMEM));
   if (e == cudaSuccess) e = ensure_smem_limit(reinterpret_cast<const void*>(k_attn_backward_tc<false>), static_cast<int>(B_SMEM));

@@ -10,8 +10,9 @@
 // instead of 5).
 //
 //   warp 0       TMA producer
-//   warp 1       TMEM owner; lane 0 issues the MMAs
-//   warps 2, 3   idle: register shares go by groups of four warps
+//   warp 1       TMEM owner; one thread issues the MMAs
+//   warp 2       with lengths: clears the tails of streamed tiles
+//   warp 3       idle: register shares go by groups of four warps
 //   warps 4..19  the elementwise work on S (and dP) in TMEM, one row per
 //                thread, the columns of a tile split between warps of the
 //                same lane quadrant
@@ -51,8 +52,8 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
       : "memory");
 }
 
-// Zeroes rows [valid, 128) of two tiles that TMA wrote; all lanes of a warp,
-// before its MMAs read them.  A swizzled row stays in its own 128 bytes.
+// Zeroes rows [valid, 128) of two tiles that TMA wrote, before MMAs read them;
+// all lanes of a warp.  A swizzled row stays in its own 128 bytes.
 __device__ __forceinline__ void zero_tail(uint8_t* a, uint8_t* b, int valid, int lane) {
   for (int i = valid * 8 + lane; i < TR * 8; i += 32) {
     reinterpret_cast<uint4*>(a)[i] = make_uint4(0, 0, 0, 0);
@@ -80,9 +81,10 @@ struct FastDiv {
 __device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 104;"); }
 __device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 64;"); }
 
-// True in one lane of a converged warp.  MMAs are issued under it: the compiler
-// knows that a single lane is active and keeps their operands in uniform
-// registers.
+// True in one lane of a converged warp.  The MMA loops run under it: the
+// compiler knows that a single thread is active and keeps the operands in
+// uniform registers (under `lane == 0` each MMA took 115 cycles to issue), and
+// that thread's waits need no vote of the warp.
 __device__ __forceinline__ bool elect_one() {
   uint32_t p;
   asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\tselp.u32 %0, 1, 0, e;\n\t}" : "=r"(p));
@@ -98,8 +100,25 @@ __device__ __forceinline__ void drain(uint64_t* bar, uint32_t parity) {
   }
 }
 
+// One thread's wait for a phase; false (and `code` in the error word) when it
+// ran out.  The clock and the error word are looked at every 1024 tries only.
+__device__ __forceinline__ bool thread_wait(uint64_t* bar, uint32_t parity, int* err, int code) {
+  const uint32_t a = smem_u32(bar);
+  uint64_t t0 = 0;
+  for (uint32_t it = 1; !mbar_try_wait(a, parity); ++it) {
+    if ((it & 1023u) != 0) continue;
+    const uint64_t t = globaltimer();
+    if (t0 == 0) t0 = t;
+    if (*reinterpret_cast<volatile int*>(err) != 0 || t - t0 > VK_WAIT_NS) {
+      record_error(err, code);
+      return false;
+    }
+  }
+  return true;
+}
+// The same for a warp: one outcome for all lanes.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* err, int code) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, code));
+  return __all_sync(0xffffffffu, thread_wait(bar, parity, err, code));
 }
 
 __device__ __forceinline__ void tma_store_4d(const void* desc, const void* src, int32_t x, int32_t y, int32_t z, int32_t w) {
@@ -185,7 +204,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   uint64_t* q_empty = q_full + 2;    // [2 parities][2 tiles]
   uint64_t* kv_full = q_empty + 4;   // [ST]
   uint64_t* kv_empty = kv_full + ST; // [ST]
-  uint64_t* s_full = kv_empty + ST;  // [2] tile: S(j) ready, every earlier product of the tile done
+  uint64_t* kv_clean = kv_empty + ST; // [ST] with lengths: what lies past them is zero
+  uint64_t* s_full = kv_clean + ST;  // [2] tile: S(j) ready, every earlier product of the tile done
   uint64_t* p_full = s_full + 2;     // [2 tiles][2 halves]
   uint64_t* o_done = p_full + 4;     // [2] tile
   uint64_t* x_full = o_done + 2;     // [2] tile: references and sums of both halves written
@@ -224,6 +244,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     for (int i = 0; i < ST; ++i) {
       mbar_init(&kv_full[i], 1);
       mbar_init(&kv_empty[i], 1);
+      mbar_init(&kv_clean[i], 1);
     }
     mbar_init(stopped, 1);
     fence_mbar_init();
@@ -273,66 +294,70 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       }
     }
   } else if (warp == 1) {
-    constexpr uint32_t idS = idesc_bf16(128, 128), idO = idesc_bf16_bmn(128, 64);
-    uint32_t g = 0, sp[2] = {0u, 0u};
-    bool ok = true;
-    for (int it = blockIdx.x, c = 0; it < items && ok; it += gridDim.x) {
-      const Item I = item_of(it);
-      if (I.tiles == 0) continue;
-      const int qb = c & 1;
-      auto block_ready = [&](uint32_t gg, int j) {
-        if (!warp_wait(&kv_full[gg % ST], (gg / ST) & 1, err, VK_DEV_TIMEOUT_MMA)) return false;
-        const int valid = I.nk - j * TR;
-        if (valid < TR && I.nk < a.nk) zero_tail(sK + gg % ST * TILE_B, sV + gg % ST * TILE_B, valid, lane);
-        return true;
-      };
-      auto issue_s = [&](int t, uint32_t st) {
-        const uint64_t qd = smem_desc_k_sw128(smem_u32(sQ + (qb * 2 + t) * TILE_B));
-        const uint64_t kd = smem_desc_k_sw128(smem_u32(sK + st * TILE_B));
+    if (elect_one()) {
+      constexpr uint32_t idS = idesc_bf16(128, 128), idO = idesc_bf16_bmn(128, 64);
+      uint64_t* kv_ready = a.kv_lens != nullptr ? kv_clean : kv_full;
+      uint32_t g = 0, c = 0, sp[2] = {0u, 0u};  // blocks, items with work; blocks of each tile
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, uint32_t parity) { return ok = ok && thread_wait(bar, parity & 1, err, VK_DEV_TIMEOUT_MMA); };
+      for (int it = blockIdx.x; it < items && ok; it += gridDim.x) {
+        const Item I = item_of(it);
+        if (I.tiles == 0) continue;
+        const uint32_t qb = c & 1;
+        auto issue_s = [&](int t, uint32_t st) {
+          const uint64_t qd = smem_desc_k_sw128(smem_u32(sQ + (qb * 2 + t) * TILE_B));
+          const uint64_t kd = smem_desc_k_sw128(smem_u32(sK + st * TILE_B));
 #pragma unroll
-        for (int k = 0; k < 4; ++k) umma_f16(tmem + t * 256, qd + k * 2, kd + k * 2, idS, k > 0 ? 1u : 0u);
-        umma_commit(&s_full[t]);
-      };
-      if (!(ok = warp_wait(&q_full[qb], (c >> 1) & 1, err, VK_DEV_TIMEOUT_MMA) && block_ready(g, 0))) break;
-      ++c;
-      tc_fence_after();
-      if (elect_one())
+          for (int k = 0; k < 4; ++k) umma_f16(tmem + t * 256, qd + k * 2, kd + k * 2, idS, k > 0 ? 1u : 0u);
+          umma_commit(&s_full[t]);
+        };
+        if (!wait(&q_full[qb], c >> 1) || !wait(&kv_ready[g % ST], g / ST)) break;
+        ++c;
+        tc_fence_after();
         for (int t = 0; t < I.tiles; ++t) issue_s(t, g % ST);
-      for (int j = 0; j < I.nb && ok; ++j, ++g) {
-        const bool more = j + 1 < I.nb;
-        if (more && !(ok = block_ready(g + 1, j + 1))) break;
-        for (int t = 0; t < I.tiles && ok; ++t) {
+        for (int j = 0; j < I.nb && ok; ++j, ++g) {
+          const bool more = j + 1 < I.nb;
+          if (more && !wait(&kv_ready[(g + 1) % ST], (g + 1) / ST)) break;
           const uint64_t vd = smem_desc_mn_sw128(smem_u32(sV + g % ST * TILE_B));
-          const uint32_t par = sp[t] & 1;
-          ++sp[t];
-          // O is overwritten at an item's first block: both halves' warps
-          // have read the last item's O of this tile once they hand over P
-          if (!(ok = warp_wait(&p_full[2 * t], par, err, VK_DEV_TIMEOUT_MMA))) break;
-          if (j == 0 && !(ok = warp_wait(&p_full[2 * t + 1], par, err, VK_DEV_TIMEOUT_MMA))) break;
-          for (int h = 0; h < 2; ++h) {
-            if (h == 1 && j > 0 && !(ok = warp_wait(&p_full[2 * t + 1], par, err, VK_DEV_TIMEOUT_MMA))) break;
-            tc_fence_after();
-            if (elect_one()) {
+          for (int t = 0; t < I.tiles && ok; ++t) {
+            const uint32_t par = t == 0 ? sp[0]++ : sp[1]++;
+            // O is overwritten at an item's first block: both halves' warps
+            // have read the last item's O of this tile once they hand over P
+            if (!wait(&p_full[2 * t], par) || (j == 0 && !wait(&p_full[2 * t + 1], par))) break;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              if (h == 1 && j > 0 && !wait(&p_full[2 * t + 1], par)) break;
+              tc_fence_after();
 #pragma unroll
               for (int k = 0; k < 4; ++k)
                 umma_f16_ts(tmem + t * 256 + 128 + h * 64, tmem + t * 256 + h * 64 + k * 8,
                             vd + static_cast<uint64_t>((h * 4 + k) * (2048 >> 4)), idO, (j | k) > 0 ? 1u : 0u);
             }
-          }
-          if (!ok) break;
-          if (elect_one()) {
+            if (!ok) break;
             if (more)
               issue_s(t, (g + 1) % ST);  // after the products that read P, which it overwrites
             else
               umma_commit(&o_done[t]);
           }
+          umma_commit(&kv_empty[g % ST]);
         }
-        if (ok && elect_one()) umma_commit(&kv_empty[g % ST]);
+      }
+      if (!ok) {
+        umma_commit(stopped);
+        drain(stopped, 0);
       }
     }
-    if (!ok) {
-      if (elect_one()) umma_commit(stopped);
-      drain(stopped, 0);
+  } else if (warp == 2 && a.kv_lens != nullptr) {
+    uint32_t g = 0;
+    bool ok = true;
+    for (int it = blockIdx.x; it < items && ok; it += gridDim.x) {
+      const Item I = item_of(it);
+      if (I.tiles == 0) continue;
+      for (int j = 0; j < I.nb; ++j, ++g) {
+        if (!(ok = warp_wait(&kv_full[g % ST], (g / ST) & 1, err, VK_DEV_TIMEOUT_OTHER))) break;
+        if (I.nk - j * TR < TR) zero_tail(sK + g % ST * TILE_B, sV + g % ST * TILE_B, I.nk - j * TR, lane);
+        if (lane == 0) mbar_arrive(&kv_clean[g % ST]);
+      }
     }
   } else if (warp >= 4) {
     regs_inc();
@@ -539,7 +564,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   uint64_t* own_empty = own_full + 2;   // [2]
   uint64_t* st_full = own_empty + 2;    // [ST]
   uint64_t* st_empty = st_full + ST;    // [ST]
-  uint64_t* s_full = st_empty + ST;     // [2] group
+  uint64_t* st_clean = st_empty + ST;   // [ST] with lengths: what lies past them is zero
+  uint64_t* s_full = st_clean + ST;     // [2] group
   uint64_t* dp_full = s_full + 2;       // [2] group
   uint64_t* ds_full = dp_full + 2;      // [2] group: dS written
   uint64_t* acc_full = ds_full + 2;     // [2] item parity: the item's last products done
@@ -554,7 +580,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(stopped + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int total_own = DQ ? a.nq : a.nk, total_len = DQ ? a.nk : a.nq;
+  const int total_own = DQ ? a.nq : a.nk;
   // An item: 128 own rows of one (sequence, head), and what it streams.
   struct Item {
     int it, bh, r0, own, len, nb;  // own and streamed rows of the sequence, blocks
@@ -598,6 +624,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     for (int i = 0; i < ST; ++i) {
       mbar_init(&st_full[i], 1);
       mbar_init(&st_empty[i], 1);
+      mbar_init(&st_clean[i], 1);
     }
     mbar_init(stopped, 1);
     fence_mbar_init();
@@ -663,92 +690,75 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       for (uint32_t i = owns > 2 ? owns - 2 : 0; i < owns; ++i) drain(&own_full[i & 1], (i >> 1) & 1);
     }
   } else if (warp == 1) {
-    constexpr uint32_t idS = idesc_bf16(128, 128), idA = idesc_bf16_bmn(128, 64);
-    // One block of the walk: block j of nb of the c-th item with work.
-    struct Blk {
-      int it, j, nb, len;
-      uint32_t c;
-      bool ok;
-    };
-    auto load = [&](int it, uint32_t c) {
-      const Item I = seek(it, nothing);
-      return Blk{I.it, 0, I.nb, I.len, c, I.it < items};
-    };
-    auto next = [&](Blk k) {
-      if (k.ok && ++k.j == k.nb) k = load(k.it + gridDim.x, k.c + 1);
-      return k;
-    };
-    // waits for a block's operands and clears what lies past the length
-    auto ready = [&](const Blk& k, uint32_t n) {
-      if (k.j == 0 && !warp_wait(&own_full[k.c & 1], (k.c >> 1) & 1, err, VK_DEV_TIMEOUT_MMA)) return false;
-      if (!warp_wait(&st_full[n % ST], (n / ST) & 1, err, VK_DEV_TIMEOUT_MMA)) return false;
-      const int valid = k.len - k.j * TR;
-      if (valid < TR && k.len < total_len) zero_tail(s1 + n % ST * TILE_B, s2 + n % ST * TILE_B, valid, lane);
-      tc_fence_after();
-      return true;
-    };
-    auto product = [&](uint32_t col, const uint8_t* own, const uint8_t* streamed) {
-      const uint64_t od = smem_desc_k_sw128(smem_u32(own)), sd = smem_desc_k_sw128(smem_u32(streamed));
+    if (elect_one()) {
+      constexpr uint32_t idS = idesc_bf16(128, 128), idA = idesc_bf16_bmn(128, 64);
+      uint64_t* st_ready = (DQ ? a.kv_lens : a.q_lens) != nullptr ? st_clean : st_full;
+      // One block of the walk: block j of nb of the c-th item with work.
+      struct Blk {
+        int it, j, nb;
+        uint32_t c;
+        bool ok;
+      };
+      auto load = [&](int it, uint32_t c) {
+        const Item I = seek(it, nothing);
+        return Blk{I.it, 0, I.nb, c, I.it < items};
+      };
+      auto next = [&](Blk k) {
+        if (k.ok && ++k.j == k.nb) k = load(k.it + gridDim.x, k.c + 1);
+        return k;
+      };
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, uint32_t parity) { return ok = ok && thread_wait(bar, parity & 1, err, VK_DEV_TIMEOUT_MMA); };
+      auto ready = [&](const Blk& k, uint32_t n) {  // a block's operands are there
+        if (k.j == 0) wait(&own_full[k.c & 1], k.c >> 1);
+        return wait(&st_ready[n % ST], n / ST);
+      };
+      auto product = [&](uint32_t col, const uint8_t* own, const uint8_t* streamed) {
+        const uint64_t od = smem_desc_k_sw128(smem_u32(own)), sd = smem_desc_k_sw128(smem_u32(streamed));
 #pragma unroll
-      for (int k = 0; k < 4; ++k) umma_f16(tmem + col, od + k * 2, sd + k * 2, idS, k > 0 ? 1u : 0u);
-    };
-    auto issue_s = [&](const Blk& k, uint32_t n) {
-      if (elect_one()) {
+        for (int k = 0; k < 4; ++k) umma_f16(tmem + col, od + k * 2, sd + k * 2, idS, k > 0 ? 1u : 0u);
+      };
+      auto issue_s = [&](const Blk& k, uint32_t n) {
+        tc_fence_after();
         product(0, sOwn + (k.c & 1) * 2 * TILE_B, s1 + n % ST * TILE_B);
         umma_commit(&s_full[n & 1]);
-      }
-    };
-    auto issue_dp = [&](const Blk& k, uint32_t n) {
-      if (elect_one()) {
+      };
+      auto issue_dp = [&](const Blk& k, uint32_t n) {
+        tc_fence_after();
         product(COL_DP, sOwn + ((k.c & 1) * 2 + 1) * TILE_B, s2 + n % ST * TILE_B);
         umma_commit(&dp_full[n & 1]);
-      }
-    };
-    // acc += A . streamed, A = 64 columns of TMEM from `col` on
-    auto sum = [&](uint32_t acc, uint32_t col, const uint8_t* streamed, bool fresh) {
-      const uint64_t sd = smem_desc_mn_sw128(smem_u32(streamed));
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        umma_f16_ts(tmem + acc, tmem + col + k * 8, sd + static_cast<uint64_t>(k * (2048 >> 4)), idA, fresh && k == 0 ? 0u : 1u);
-    };
-    // the last item's accumulators have been read
-    auto acc_ready = [&](const Blk& k) {
-      return k.j > 0 || k.c == 0 || warp_wait(acc_free, (k.c - 1) & 1, err, VK_DEV_TIMEOUT_MMA);
-    };
-    Blk b0 = load(blockIdx.x, 0), b1 = next(b0), b2 = next(b1);
-    bool ok = true;
-    auto next_s = [&](const Blk& k, uint32_t n) {  // S of block n, once block n - 1's has been read
-      if (!(ok = ready(k, n) && warp_wait(s_free, (n - 1) & 1, err, VK_DEV_TIMEOUT_MMA))) return;
-      tc_fence_after();
-      issue_s(k, n);
-    };
-    if (b0.ok && (ok = ready(b0, 0))) {
-      issue_s(b0, 0);
-      issue_dp(b0, 0);
-    }
-    if (ok && b1.ok) next_s(b1, 1);
-    for (uint32_t n = 0; ok && b0.ok; ++n) {
-      if constexpr (!DQ) {
-        if (!(ok = warp_wait(p_full, n & 1, err, VK_DEV_TIMEOUT_MMA) && acc_ready(b0))) break;
+      };
+      // acc += A . streamed, A = 64 columns of TMEM from `col` on
+      auto sum = [&](uint32_t acc, uint32_t col, const uint8_t* streamed, bool fresh) {
         tc_fence_after();
-        if (elect_one()) {
+        const uint64_t sd = smem_desc_mn_sw128(smem_u32(streamed));
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          umma_f16_ts(tmem + acc, tmem + col + k * 8, sd + static_cast<uint64_t>(k * (2048 >> 4)), idA, fresh && k == 0 ? 0u : 1u);
+      };
+      auto acc_ready = [&](const Blk& k) {  // the last item's accumulators have been read
+        return k.j > 0 || k.c == 0 || wait(acc_free, k.c - 1);
+      };
+      auto next_s = [&](const Blk& k, uint32_t n) {  // S of block n, once block n - 1's has been read
+        if (ready(k, n) && wait(s_free, n - 1)) issue_s(k, n);
+      };
+      Blk b0 = load(blockIdx.x, 0), b1 = next(b0), b2 = next(b1);
+      if (b0.ok && ready(b0, 0)) {
+        issue_s(b0, 0);
+        issue_dp(b0, 0);
+      }
+      if (ok && b1.ok) next_s(b1, 1);
+      for (uint32_t n = 0; ok && b0.ok; ++n) {
+        if constexpr (!DQ) {
+          if (!wait(p_full, n) || !acc_ready(b0)) break;
           sum(COL_ACC, COL_P, s2 + n % ST * TILE_B, b0.j == 0);  // dv += P^T d_out
           umma_commit(p_free);
         }
-      }
-      // S(n+2) early -- unless its item takes over the tiles of block n's
-      const bool late = b2.c >= b0.c + 2;
-      if (b2.ok && !late) next_s(b2, n + 2);
-      if (!ok) break;
-      if (b1.ok) {
-        if (!(ok = warp_wait(dp_free, n & 1, err, VK_DEV_TIMEOUT_MMA))) break;
-        tc_fence_after();
-        issue_dp(b1, n + 1);
-      }
-      if (!(ok = warp_wait(&ds_full[n & 1], (n >> 1) & 1, err, VK_DEV_TIMEOUT_MMA))) break;
-      if (DQ && !(ok = acc_ready(b0))) break;
-      tc_fence_after();
-      if (elect_one()) {
+        // S(n+2) early -- unless its item takes over the tiles of block n's
+        const bool late = b2.c >= b0.c + 2;
+        if (b2.ok && !late) next_s(b2, n + 2);
+        if (b1.ok && wait(dp_free, n)) issue_dp(b1, n + 1);
+        if (!wait(&ds_full[n & 1], n >> 1) || (DQ && !acc_ready(b0))) break;
         if constexpr (DQ) {
           sum(COL_ACC, COL_P + (n & 1) * 64, s1 + n % ST * TILE_B, b0.j == 0);  // dq += dS k
         } else {
@@ -757,16 +767,25 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         }
         umma_commit(&st_empty[n % ST]);
         if (b0.j + 1 == b0.nb) umma_commit(&acc_full[b0.c & 1]);
+        if (b2.ok && late) next_s(b2, n + 2);
+        b0 = b1;
+        b1 = b2;
+        b2 = next(b2);
       }
-      if (b2.ok && late) next_s(b2, n + 2);
-      b0 = b1;
-      b1 = b2;
-      b2 = next(b2);
+      if (!ok) {
+        umma_commit(stopped);
+        drain(stopped, 0);
+      }
     }
-    if (!ok) {
-      if (elect_one()) umma_commit(stopped);
-      drain(stopped, 0);
-    }
+  } else if (warp == 2 && (DQ ? a.kv_lens : a.q_lens) != nullptr) {
+    uint32_t n = 0;
+    bool ok = true;
+    for (Item I = seek(blockIdx.x, nothing); ok && I.it < items; I = seek(I.it + gridDim.x, nothing))
+      for (int j = 0; j < I.nb; ++j, ++n) {
+        if (!(ok = warp_wait(&st_full[n % ST], (n / ST) & 1, err, VK_DEV_TIMEOUT_OTHER))) break;
+        if (I.len - j * TR < TR) zero_tail(s1 + n % ST * TILE_B, s2 + n % ST * TILE_B, I.len - j * TR, lane);
+        if (lane == 0) mbar_arrive(&st_clean[n % ST]);
+      }
   } else if (warp >= 4) {
     regs_inc();
     const int quad = warp & 3, grp = (warp - 4) >> 3, half = ((warp - 4) >> 2) & 1;  // columns [64 half, 64 half + 64)

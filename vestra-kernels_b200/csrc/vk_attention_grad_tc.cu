@@ -13,9 +13,10 @@
 //   warp 1       TMEM owner; one thread issues the MMAs
 //   warp 2       with lengths: clears the tails of streamed tiles
 //   warp 3       idle: register shares go by groups of four warps
-//   warps 4..19  the elementwise work on S (and dP) in TMEM, one row per
-//                thread, the columns of a tile split between warps of the
-//                same lane quadrant
+//   warps 4..11  the elementwise work on S (and dP) in TMEM: two groups of four
+//                warps, a row of 128 columns per thread.  (16 warps with 64
+//                or 32 columns each spent half of their instructions on
+//                waits and hand-overs, and most of their time in step.)
 //
 // S and dP are bf16 products in f32.  P and dS are rounded to bf16 for the
 // second products (one rounding of 2^-8 at most, next to the one of the
@@ -32,7 +33,7 @@ namespace {
 constexpr int TR = 128;                 // rows of a tile, columns of a block
 constexpr int TILE_B = TR * 128;        // bytes of 128 rows of 64 bf16
 constexpr int ST = 4;                   // streamed blocks in flight
-constexpr int TC_THREADS = 20 * 32;
+constexpr int TC_THREADS = 12 * 32;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 __device__ __forceinline__ void tma_load_4d(void* dst, const void* desc, uint64_t* bar, int32_t y, int32_t z, int32_t w) {
@@ -76,10 +77,10 @@ struct FastDiv {
   }
 };
 
-// The launch gives each of the 640 threads 96 registers; the elementwise warps
-// take 104 and the first four warps keep 64: 512 * 104 + 128 * 64 = 640 * 96.
-__device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 104;"); }
-__device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 64;"); }
+// The launch gives each of the 384 threads 168 registers; the elementwise warps
+// take 208 and the first four warps keep 88: 256 * 208 + 128 * 88 = 384 * 168.
+__device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 208;"); }
+__device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 88;"); }
 
 // True in one lane of a converged warp.  The MMA loops run under it: the
 // compiler knows that a single thread is active and keeps the operands in
@@ -121,21 +122,19 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* e
   return __all_sync(0xffffffffu, thread_wait(bar, parity, err, code));
 }
 
-__device__ __forceinline__ void tma_store_4d(const void* desc, const void* src, int32_t x, int32_t y, int32_t z, int32_t w) {
+__device__ __forceinline__ void tma_store_4d(const void* desc, const void* src, int32_t y, int32_t z, int32_t w) {
   asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(
                    reinterpret_cast<uint64_t>(desc)),
-               "r"(smem_u32(src)), "r"(x), "r"(y), "r"(z), "r"(w)
+               "r"(smem_u32(src)), "r"(0), "r"(y), "r"(z), "r"(w)
                : "memory");
 }
 
-// 16-byte piece c of row `lane` of a warp's output staging, 32 rows of ROW (64
-// or 128) bytes in the order of TMA's swizzle of that width.  Rows leave through TMA because a thread's own stores, one row
+// 16-byte piece c of row `lane` of a warp's output staging, 32 rows of 64 bf16
+// in the order of TMA's 128-byte swizzle.  Rows leave through TMA because a thread's own stores, one row
 // each, would touch 32 lines per instruction: 2000 cycles of address work per
 // tile where an item has about 15000.
-template <int ROW>
 __device__ __forceinline__ uint4* staged(uint8_t* s, int lane, int c) {
-  if constexpr (ROW == 128) return reinterpret_cast<uint4*>(s + lane * 128 + ((c ^ lane) & 7) * 16);
-  return reinterpret_cast<uint4*>(s + lane * 64 + ((c ^ (lane >> 1)) & 3) * 16);
+  return reinterpret_cast<uint4*>(s + lane * 128 + ((c ^ lane) & 7) * 16);
 }
 __device__ __forceinline__ uint4 pack8(const float* x, float f) {
   return make_uint4(pack_bf16x2(x[0] * f, x[1] * f), pack_bf16x2(x[2] * f, x[3] * f), pack_bf16x2(x[4] * f, x[5] * f),
@@ -143,16 +142,36 @@ __device__ __forceinline__ uint4 pack8(const float* x, float f) {
 }
 // The staged rows are on their way when this returns; the warp's lane 0 waits
 // for them (bulk_wait_read) before the staging is used again.
-__device__ __forceinline__ void send_rows(const void* desc, const uint8_t* s, int x, int y, int rows, int z, int w, int lane) {
+__device__ __forceinline__ void send_rows(const void* desc, const uint8_t* s, int y, int rows, int z, int w, int lane) {
   fence_proxy_async();
   __syncwarp();
   if (lane == 0) {
-    if (y < rows) tma_store_4d(desc, s, x, y, z, w);
+    if (y < rows) tma_store_4d(desc, s, y, z, w);
     bulk_commit();
   }
 }
-__device__ __forceinline__ void store_zeros(__nv_bfloat16* p, int n) {
-  for (int i = 0; i < n; i += 8) *reinterpret_cast<uint4*>(p + i) = make_uint4(0, 0, 0, 0);
+__device__ __forceinline__ void store_zeros(__nv_bfloat16* p) {  // a row
+  for (int i = 0; i < 64; i += 8) *reinterpret_cast<uint4*>(p + i) = make_uint4(0, 0, 0, 0);
+}
+// A row of 64 accumulator columns, times f, into the staging (zeros if not live).
+__device__ __forceinline__ void stage_row(uint8_t* s, int lane, uint32_t taddr, float f, bool live) {
+#pragma unroll
+  for (int d0 = 0; d0 < 64; d0 += 32) {
+    uint32_t r[32];
+    tmem_ld32(taddr + d0, r);
+    tmem_wait_ld();
+    float x[32];
+#pragma unroll
+    for (int d = 0; d < 32; ++d) x[d] = live ? __uint_as_float(r[d]) : 0.0f;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) *staged(s, lane, d0 / 8 + c) = pack8(x + 8 * c, f);
+  }
+}
+// 128 columns of a row.
+__device__ __forceinline__ void tmem_ld128(uint32_t taddr, uint32_t (&r)[128]) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c) tmem_ld32(taddr + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&r[c * 32]));
+  tmem_wait_ld();
 }
 
 // A reference to subtract from scores of which `top` is the largest so far.
@@ -162,10 +181,10 @@ __device__ __forceinline__ float finite_ref(float top) { return top == -INFINITY
 // Scores of columns from `valid` on become -inf.  The empty statement keeps
 // this a branch of the rare last block: as selects it would cost every block
 // two instructions a column.
-__device__ __forceinline__ void mask_columns(uint32_t (&r)[32], int valid) {
+__device__ __forceinline__ void mask_columns(uint32_t (&r)[128], int valid) {
   asm volatile("" ::: "memory");
 #pragma unroll
-  for (int i = 0; i < 32; ++i)
+  for (int i = 0; i < 128; ++i)
     if (i >= valid) r[i] = 0xff800000u;
 }
 
@@ -178,15 +197,16 @@ __device__ __forceinline__ float2 exp2_pair(float2 x, int i) {
 }  // namespace
 
 // ------------------------------------------------------------------ forward
-// TMEM per tile (256 columns): S, and P over it, at [0, 128), and two O
-// accumulators at [128, 192) and [192, 256): one for the first 64 keys of
-// every block and one for the last 64.  The warps of a key half keep their own
-// running reference and sum, so the two halves of a row meet only at the end:
-// out = (f0 O0 + f1 O1) / (f0 l0 + f1 l1) with f = 2^(m - max m).
+// An item is two query tiles of a head (one where pairs would leave SMs idle),
+// each with its own group of four warps.  TMEM: S of the tiles [0, 128) and
+// [128, 256), P as bf16 [256, 320) and [320, 384), O [384, 448) and [448, 512).
+// S is handed back as soon as it is in registers, so that the next block's is
+// there when the warps ask for it: they are bound by their exponentials.
 namespace {
 constexpr uint32_t F_MASK = 0x0u;
-constexpr size_t F_SMEM = 1024 + TILE_B * (4 + 2 * ST) + 4096 + 512;
-}
+constexpr uint32_t F_P = 256, F_O = 384;
+constexpr size_t F_SMEM = 1024 + TILE_B * (4 + 2 * ST) + 512;
+}  // namespace
 
 __global__ void __launch_bounds__(TC_THREADS, 1)
     k_attn_forward_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
@@ -195,21 +215,20 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
                       int tpi, int* err) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sQ = smem;  // [item parity][tile]
+  uint8_t* sQ = smem;  // [item parity][tile], then the tile's output on its way out
   uint8_t* sK = smem + 4 * TILE_B;
   uint8_t* sV = sK + ST * TILE_B;
-  float2* sX = reinterpret_cast<float2*>(sV + ST * TILE_B);  // [tile][half][row] (reference, sum)
-  uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(sX) + 4096);
-  uint64_t* q_full = bars;           // [2] item parity
-  uint64_t* q_empty = q_full + 2;    // [2 parities][2 tiles]
-  uint64_t* kv_full = q_empty + 4;   // [ST]
-  uint64_t* kv_empty = kv_full + ST; // [ST]
-  uint64_t* kv_clean = kv_empty + ST; // [ST] with lengths: what lies past them is zero
-  uint64_t* s_full = kv_clean + ST;  // [2] tile: S(j) ready, every earlier product of the tile done
-  uint64_t* p_full = s_full + 2;     // [2 tiles][2 halves]
-  uint64_t* o_done = p_full + 4;     // [2] tile
-  uint64_t* x_full = o_done + 2;     // [2] tile: references and sums of both halves written
-  uint64_t* stopped = x_full + 2;    // every product done, after an error
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sV + ST * TILE_B);
+  uint64_t* q_full = bars;             // [2] item parity
+  uint64_t* q_empty = q_full + 2;      // [2 parities][2 tiles]
+  uint64_t* kv_full = q_empty + 4;     // [ST]
+  uint64_t* kv_empty = kv_full + ST;   // [ST]
+  uint64_t* kv_clean = kv_empty + ST;  // [ST] with lengths: what lies past them is zero
+  uint64_t* s_full = kv_clean + ST;    // [2] tile
+  uint64_t* s_free = s_full + 2;       // [2] tile: S read
+  uint64_t* p_full = s_free + 2;       // [2] tile: P written
+  uint64_t* p_free = p_full + 2;       // [2] tile: P used, O complete up to its block
+  uint64_t* stopped = p_free + 2;      // every product done, after an error
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(stopped + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -233,13 +252,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 1);
-      mbar_init(&q_empty[2 * i], 8);  // the tile's warps, once their output has left the buffer
-      mbar_init(&q_empty[2 * i + 1], 8);
+      mbar_init(&q_empty[2 * i], 4);  // the tile's warps, once their output has left the buffer
+      mbar_init(&q_empty[2 * i + 1], 4);
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[2 * i], 4);
-      mbar_init(&p_full[2 * i + 1], 4);
-      mbar_init(&o_done[i], 1);
-      mbar_init(&x_full[i], 8);
+      mbar_init(&s_free[i], 4);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&p_free[i], 1);
     }
     for (int i = 0; i < ST; ++i) {
       mbar_init(&kv_full[i], 1);
@@ -260,8 +278,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
 
   if (warp < 4) regs_dec();
   if (warp == 0) {
-    if (lane == 0) {
-      uint32_t g = 0, c = 0;               // blocks, items with work
+    if (elect_one()) {
+      uint32_t g = 0, c = 0;                   // blocks, items with work
       uint32_t used[2][2] = {{0, 0}, {0, 0}};  // [parity][tile]
       bool ok = true;
       for (int it = blockIdx.x; it < items && ok; it += gridDim.x) {
@@ -273,7 +291,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         for (int t = 0; t < 2; ++t)
           if (ok && t < I.tiles) {
             uint32_t& u = qb ? used[1][t] : used[0][t];
-            if (u > 0) ok = mbar_wait(&q_empty[qb * 2 + t], (u - 1) & 1, err, VK_DEV_TIMEOUT_PRODUCER);
+            if (u > 0) ok = thread_wait(&q_empty[qb * 2 + t], (u - 1) & 1, err, VK_DEV_TIMEOUT_PRODUCER);
             ++u;
           }
         if (!ok) break;
@@ -282,7 +300,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         for (int t = 0; t < I.tiles; ++t) tma_load_4d(sQ + (qb * 2 + t) * TILE_B, &tmQ, &q_full[qb], I.q0 + t * TR, I.h, I.b);
         for (int j = 0; j < I.nb; ++j, ++g) {
           const uint32_t st = g % ST;
-          if (!(ok = mbar_wait(&kv_empty[st], ((g / ST) & 1) ^ 1, err, VK_DEV_TIMEOUT_PRODUCER))) break;
+          if (!(ok = thread_wait(&kv_empty[st], ((g / ST) & 1) ^ 1, err, VK_DEV_TIMEOUT_PRODUCER))) break;
           mbar_arrive_expect_tx(&kv_full[st], 2 * TILE_B);
           tma_load_4d(sK + st * TILE_B, &tmK, &kv_full[st], j * TR, I.h, I.b);
           tma_load_4d(sV + st * TILE_B, &tmV, &kv_full[st], j * TR, I.h, I.b);
@@ -297,48 +315,47 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     if (elect_one()) {
       constexpr uint32_t idS = idesc_bf16(128, 128), idO = idesc_bf16_bmn(128, 64);
       uint64_t* kv_ready = a.kv_lens != nullptr ? kv_clean : kv_full;
-      uint32_t g = 0, c = 0, sp[2] = {0u, 0u};  // blocks, items with work; blocks of each tile
+      uint32_t g = 0, c = 0;  // blocks, items with work
+      uint32_t n0 = 0, n1 = 0;  // blocks of each tile
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity) { return ok = ok && thread_wait(bar, parity & 1, err, VK_DEV_TIMEOUT_MMA); };
       for (int it = blockIdx.x; it < items && ok; it += gridDim.x) {
         const Item I = item_of(it);
         if (I.tiles == 0) continue;
         const uint32_t qb = c & 1;
-        auto issue_s = [&](int t, uint32_t st) {
+        // S of tile t, block n of that tile, once its last S has been read
+        auto issue_s = [&](int t, uint32_t n, uint32_t st) {
+          if (n > 0 && !wait(&s_free[t], n - 1)) return;
+          tc_fence_after();
           const uint64_t qd = smem_desc_k_sw128(smem_u32(sQ + (qb * 2 + t) * TILE_B));
           const uint64_t kd = smem_desc_k_sw128(smem_u32(sK + st * TILE_B));
 #pragma unroll
-          for (int k = 0; k < 4; ++k) umma_f16(tmem + t * 256, qd + k * 2, kd + k * 2, idS, k > 0 ? 1u : 0u);
+          for (int k = 0; k < 4; ++k) umma_f16(tmem + t * TR, qd + k * 2, kd + k * 2, idS, k > 0 ? 1u : 0u);
           umma_commit(&s_full[t]);
+        };
+        auto issue_o = [&](int t, uint32_t n, uint32_t st, bool first) {
+          if (!wait(&p_full[t], n)) return;
+          tc_fence_after();
+          const uint64_t vd = smem_desc_mn_sw128(smem_u32(sV + st * TILE_B));
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            umma_f16_ts(tmem + F_O + t * 64, tmem + F_P + t * 64 + k * 8, vd + static_cast<uint64_t>(k * (2048 >> 4)), idO,
+                        first && k == 0 ? 0u : 1u);
+          umma_commit(&p_free[t]);
         };
         if (!wait(&q_full[qb], c >> 1) || !wait(&kv_ready[g % ST], g / ST)) break;
         ++c;
-        tc_fence_after();
-        for (int t = 0; t < I.tiles; ++t) issue_s(t, g % ST);
-        for (int j = 0; j < I.nb && ok; ++j, ++g) {
-          const bool more = j + 1 < I.nb;
-          if (more && !wait(&kv_ready[(g + 1) % ST], (g + 1) / ST)) break;
-          const uint64_t vd = smem_desc_mn_sw128(smem_u32(sV + g % ST * TILE_B));
-          for (int t = 0; t < I.tiles && ok; ++t) {
-            const uint32_t par = t == 0 ? sp[0]++ : sp[1]++;
-            // O is overwritten at an item's first block: both halves' warps
-            // have read the last item's O of this tile once they hand over P
-            if (!wait(&p_full[2 * t], par) || (j == 0 && !wait(&p_full[2 * t + 1], par))) break;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              if (h == 1 && j > 0 && !wait(&p_full[2 * t + 1], par)) break;
-              tc_fence_after();
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                umma_f16_ts(tmem + t * 256 + 128 + h * 64, tmem + t * 256 + h * 64 + k * 8,
-                            vd + static_cast<uint64_t>((h * 4 + k) * (2048 >> 4)), idO, (j | k) > 0 ? 1u : 0u);
-            }
-            if (!ok) break;
-            if (more)
-              issue_s(t, (g + 1) % ST);  // after the products that read P, which it overwrites
-            else
-              umma_commit(&o_done[t]);
+        issue_s(0, n0, g % ST);
+        if (I.tiles > 1) issue_s(1, n1, g % ST);
+        for (int j = 0; j < I.nb && ok; ++j, ++g, ++n0, n1 += I.tiles - 1) {
+          if (j + 1 < I.nb) {
+            if (!wait(&kv_ready[(g + 1) % ST], (g + 1) / ST)) break;
+            issue_s(0, n0 + 1, (g + 1) % ST);
+            if (I.tiles > 1) issue_s(1, n1 + 1, (g + 1) % ST);
           }
+          // (an item's first product overwrites O: its warps read the last item's before they hand over P)
+          issue_o(0, n0, g % ST, j == 0);
+          if (I.tiles > 1) issue_o(1, n1, g % ST, j == 0);
           umma_commit(&kv_empty[g % ST]);
         }
       }
@@ -361,14 +378,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     }
   } else if (warp >= 4) {
     regs_inc();
-    const int e = warp - 4, quad = warp & 3;
-    const int t = e >> 3, h = (e >> 2) & 1;
-    const uint32_t tb = tmem + t * 256 + (static_cast<uint32_t>(quad * 32) << 16);
-    const uint32_t ts = tb + h * 64, to = tb + 128 + h * 64;
+    const int t = (warp - 4) >> 2, quad = warp & 3;
+    const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
+    const uint32_t ts = tmem + t * TR + lanes, tp = tmem + F_P + t * 64 + lanes, to = tmem + F_O + t * 64 + lanes;
     const float sl2 = a.scale * LOG2E;
     const int trow = quad * 32 + lane;
-    uint32_t sp = 0, ct = 0, c = 0;  // blocks and items of this tile, items with work
-    int owed = -1;                   // the Q buffer whose staged output is still leaving
+    uint32_t n = 0, c = 0;  // blocks of this tile, items with work
+    int owed = -1;          // the Q buffer whose staged output is still leaving
     auto settle = [&]() {
       if (owed >= 0 && lane == 0) {
         bulk_wait_read<0>();
@@ -385,124 +401,79 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       if (I.tiles > 0) ++c;
       if (t >= I.tiles) {  // no queries here, or no keys
         if (row < a.nq) {
-          store_zeros(static_cast<__nv_bfloat16*>(out.p) + I.b * out.sb + I.h * out.sh + row * out.st + h * 32, 32);
-          if (h == 0) *lp = -INFINITY;
+          store_zeros(static_cast<__nv_bfloat16*>(out.p) + I.b * out.sb + I.h * out.sh + row * out.st);
+          *lp = -INFINITY;
         }
         settle();
         continue;
       }
-      float m_ref = -INFINITY, l_run = 0.0f;
-      for (int j = 0; j < I.nb; ++j, ++sp) {
-        if (!warp_wait(&s_full[t], sp & 1, err, VK_DEV_TIMEOUT_EPILOGUE)) {
-          ok = false;
-          break;
-        }
+      float m_ref = 0.0f, l_run = 0.0f;
+      for (int j = 0; j < I.nb; ++j, ++n) {
+        if (!(ok = warp_wait(&s_full[t], n & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
         tc_fence_after();
-        const int valid = I.nk - j * TR - h * 64;  // of this half's 64 keys
-        const bool full = valid >= 64;
-        auto half_max = [&]() {
-          float pm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        uint32_t r[128];
+        tmem_ld128(ts, r);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_free[t]);
+        if (I.nk - j * TR < TR) mask_columns(r, I.nk - j * TR);
+        float pm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            uint32_t r[32];
-            tmem_ld32(ts + c * 32, r);
-            tmem_wait_ld();
-            if (!full) mask_columns(r, valid - c * 32);
+        for (int i = 0; i < 128; i += 2)
+          pm[(i >> 1) & 3] = max3f(pm[(i >> 1) & 3], __uint_as_float(r[i]), __uint_as_float(r[i + 1]));
+        const float top = fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3])) * sl2;
+        if (j == 0) m_ref = finite_ref(top);
+        // p = 2^(s scale log2e - m) against a reference that stays while no
+        // score is more than 2^20 over it: the quotient O / l does not depend
+        // on it.  Then O (complete once P(n-1) is used) and l are rescaled.
+        if (__any_sync(0xffffffffu, top > m_ref + 20.0f)) {
+          if (j > 0) {
+            if (!(ok = warp_wait(&p_free[t], (n - 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
+            tc_fence_after();
+            const float m_new = fmaxf(m_ref, top), f = ex2_approx(m_ref - m_new);
 #pragma unroll
-            for (int i = 0; i < 32; i += 2)
-              pm[(i >> 1) & 3] = max3f(pm[(i >> 1) & 3], __uint_as_float(r[i]), __uint_as_float(r[i + 1]));
-          }
-          return fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3])) * sl2;
-        };
-        uint32_t pk[32];
-        // p = 2^(s scale log2e - m), packed; returns the row's sum
-        auto exp_pass = [&]() {
-          // (where nothing but -inf came so far, the first finite score overflows the check below)
-          const float m = finite_ref(m_ref);
-          const float2 scale2 = make_float2(sl2, sl2), shift2 = make_float2(-m, -m);
-          float2 ps[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+            for (int d0 = 0; d0 < 64; d0 += 16) {
+              uint32_t o[16];
+              tmem_ld16(to + d0, o);
+              tmem_wait_ld();
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            uint32_t r[32];
-            tmem_ld32(ts + c * 32, r);
-            tmem_wait_ld();
-            if (!full) mask_columns(r, valid - c * 32);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float2 p = exp2_pair<F_MASK>(
-                  ffma2(make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), scale2, shift2), i);
-              ps[i & 1] = fadd2(ps[i & 1], p);
-              pk[c * 16 + i] = pack_bf16x2(p.x, p.y);
+              for (int d = 0; d < 16; ++d) o[d] = __float_as_uint(__uint_as_float(o[d]) * f);
+              tmem_st16(to + d0, o);
             }
+            l_run *= f;
+            m_ref = m_new;
           }
-          return (ps[0].x + ps[0].y) + (ps[1].x + ps[1].y);
-        };
-        if (j == 0) m_ref = half_max();
-        // One pass against the running reference.  The final quotient does not
-        // depend on it, so p may exceed 1; a row whose sum reaches 2^20 is done
-        // again against the block's own maximum, with O and the sum rescaled
-        // (the earlier products are complete: S(j) was issued after them, and
-        // at the first block O is overwritten anyway).
-        float l_blk = exp_pass();
-        if (__any_sync(0xffffffffu, !(l_blk < 1048576.0f))) {
-          const float m_new = fmaxf(m_ref, half_max());
-          const float f = ex2_approx(m_ref - finite_ref(m_new));
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            uint32_t o[32];
-            tmem_ld32(to + c * 32, o);
-            tmem_wait_ld();
-#pragma unroll
-            for (int d = 0; d < 32; ++d) o[d] = __float_as_uint(__uint_as_float(o[d]) * f);
-            tmem_st32(to + c * 32, o);
-          }
-          l_run *= f;
-          m_ref = m_new;
-          l_blk = exp_pass();
         }
-        tmem_st32(ts, pk);
+        const float2 scale2 = make_float2(sl2, sl2), shift2 = make_float2(-m_ref, -m_ref);
+        float2 ps[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll
+        for (int i = 0; i < 64; ++i) {
+          const float2 p = exp2_pair<F_MASK>(
+              ffma2(make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), scale2, shift2), i);
+          ps[i & 1] = fadd2(ps[i & 1], p);
+          r[i] = pack_bf16x2(p.x, p.y);  // (over scores that are done with)
+        }
+        l_run += (ps[0].x + ps[0].y) + (ps[1].x + ps[1].y);
+        if (n > 0 && !(ok = warp_wait(&p_free[t], (n - 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
+        tc_fence_after();
+        tmem_st32(tp, *reinterpret_cast<uint32_t(*)[32]>(&r[0]));
+        tmem_st32(tp + 32, *reinterpret_cast<uint32_t(*)[32]>(&r[32]));
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[2 * t + h]);
-        l_run += l_blk;
+        if (lane == 0) mbar_arrive(&p_full[t]);
         if (j == 0) settle();
       }
-      if (!ok) break;
-      sX[(t * 2 + h) * TR + trow] = make_float2(m_ref, l_run);
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&x_full[t]);
-      if (!warp_wait(&x_full[t], ct & 1, err, VK_DEV_TIMEOUT_EPILOGUE) ||
-          !warp_wait(&o_done[t], ct & 1, err, VK_DEV_TIMEOUT_EPILOGUE)) {
-        ok = false;
-        break;
-      }
-      ++ct;
+      if (!ok || !(ok = warp_wait(&p_free[t], (n - 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
       tc_fence_after();
-      const float2 x0 = sX[t * 2 * TR + trow], x1 = sX[(t * 2 + 1) * TR + trow];
-      const float top = finite_ref(fmaxf(x0.x, x1.x));
-      const float f0 = ex2_approx(x0.x - top), f1 = ex2_approx(x1.x - top);
-      const float sum = f0 * x0.y + f1 * x1.y;
-      const bool live = row < I.nq && sum != 0.0f;
-      const float inv = 1.0f / sum, g0 = f0 * inv, g1 = f1 * inv;
-      // this warp's half of the output columns, staged over the tile's queries (every product is done with them)
-      uint8_t* stage = sQ + (qb * 2 + t) * TILE_B + (h * 4 + quad) * 2048;
-#pragma unroll
-      for (int d0 = 0; d0 < 32; d0 += 16) {
-        uint32_t o0[16], o1[16];
-        tmem_ld16(tb + 128 + h * 32 + d0, o0);
-        tmem_ld16(tb + 192 + h * 32 + d0, o1);
-        tmem_wait_ld();
-        float o[16];
-#pragma unroll
-        for (int d = 0; d < 16; ++d) o[d] = live ? fmaf(__uint_as_float(o0[d]), g0, __uint_as_float(o1[d]) * g1) : 0.0f;
-        *staged<64>(stage, lane, d0 / 8) = pack8(o, 1.0f);
-        *staged<64>(stage, lane, d0 / 8 + 1) = pack8(o + 8, 1.0f);
-      }
+      // staged over the tile's queries (every product is done with them)
+      const bool live = row < I.nq && l_run != 0.0f;
+      uint8_t* stage = sQ + (qb * 2 + t) * TILE_B + quad * 4096;
+      stage_row(stage, lane, to, live ? 1.0f / l_run : 0.0f, live);
       tc_fence_before();
-      send_rows(&tmO, stage, h * 32, I.q0 + t * TR + quad * 32, a.nq, I.h, I.b, lane);
+      send_rows(&tmO, stage, I.q0 + t * TR + quad * 32, a.nq, I.h, I.b, lane);
       owed = qb;
-      if (h == 0 && row < a.nq) *lp = live ? fmaf(top, LN2, logf(sum)) : -INFINITY;
+      if (row < a.nq) *lp = live ? fmaf(m_ref, LN2, logf(l_run)) : -INFINITY;
     }
     if (lane == 0) bulk_wait<0>();
   }
@@ -517,8 +488,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
 // Both backward kernels run one pipeline.  A CTA walks its items (tiles of
 // 128 own rows) and the blocks of 128 streamed rows of each as one sequence of
 // blocks n = 0, 1, ...  TMEM: S [0, 128), dP [128, 256), P and dS as bf16
-// [256, 384), accumulators [384, 512).  Two groups of 8 warps take the even
-// and the odd blocks; each warp has 32 rows and 64 of the 128 columns:
+// [256, 384), accumulators [384, 512).  The two groups of warps take the even
+// and the odd blocks; for each a warp
 //   reads S and hands it back   -> MMA: the next block's S = own1 . streamed1
 //   p = 2^(S scale log2e - lse log2e); dk/dv: writes P
 //                               -> MMA: dv += P^T . streamed2
@@ -527,18 +498,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
 //                               -> MMA: dk (dq) += dS . streamed1
 // S and dP are handed back as soon as they are in registers, so the other
 // group's are there before it asks, and one group's exponentials (MUFU, 16 a
-// clock) run beside the other's products and TMEM traffic.  With all 16 warps
-// on one block the phases followed one another: 2500 and 3000 cycles a block.
-//
-// Between its two uses p waits as 2^15 p in f16 (32 registers instead of 64;
-// off by 2^-12 down to p = 2^-29): small next to the bf16 rounding of dS.  The
-// 2^15 goes into the exponent of 2^x, and out again with dP - delta and with
-// the result of dv.
+// clock) run beside the other's products and TMEM traffic.
 namespace {
 constexpr uint32_t B_MASK = 0x0u;
 constexpr uint32_t COL_DP = 128, COL_P = 256, COL_ACC = 384;
-constexpr float P_SHIFT = 15.0f, P_SCALE = 32768.0f;
-constexpr size_t B_STATS = ST * 2 * TR * sizeof(float);  // dk/dv: (shift, delta) of the streamed rows; dq: delta's parts
+constexpr size_t B_STATS = ST * 2 * TR * sizeof(float);  // dk/dv: (-lse log2e, delta) of the streamed rows; dq: delta
 constexpr size_t B_SMEM = 1024 + TILE_B * (4 + 2 * ST + 1) + B_STATS + 512;
 }  // namespace
 
@@ -569,7 +533,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   uint64_t* dp_full = s_full + 2;       // [2] group
   uint64_t* ds_full = dp_full + 2;      // [2] group: dS written
   uint64_t* acc_full = ds_full + 2;     // [2] item parity: the item's last products done
-  uint64_t* part_full = acc_full + 2;   // [2] item parity, dq: delta's parts written, the item's tile of `out` read
+  uint64_t* part_full = acc_full + 2;   // [2] item parity, dq: delta written, the item's tile of `out` read
   uint64_t* s_free = part_full + 2;     // S read
   uint64_t* dp_free = s_free + 1;       // dP read
   uint64_t* p_full = dp_free + 1;       // dk/dv: P written
@@ -608,19 +572,19 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&own_full[i], 1);
-      mbar_init(&own_empty[i], 8);
+      mbar_init(&own_empty[i], 4);
       mbar_init(&s_full[i], 1);
       mbar_init(&dp_full[i], 1);
-      mbar_init(&ds_full[i], 8);
+      mbar_init(&ds_full[i], 4);
       mbar_init(&acc_full[i], 1);
-      mbar_init(&part_full[i], 8);
+      mbar_init(&part_full[i], 4);
     }
-    mbar_init(s_free, 8);
-    mbar_init(dp_free, 8);
-    mbar_init(p_full, 8);
+    mbar_init(s_free, 4);
+    mbar_init(dp_free, 4);
+    mbar_init(p_full, 4);
     mbar_init(p_free, 1);
     mbar_init(ds_free, 1);
-    mbar_init(acc_free, 8);
+    mbar_init(acc_free, 4);
     for (int i = 0; i < ST; ++i) {
       mbar_init(&st_full[i], 1);
       mbar_init(&st_empty[i], 1);
@@ -672,8 +636,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             // lse = -inf: a row of scores of -inf only, whose p is 2^(-inf - 0) = 0
-            sStat[st * 2 * TR + i * 32 + lane] = l[i] == -INFINITY ? 0.0f : fmaf(l[i], -LOG2E, P_SHIFT);
-            sStat[st * 2 * TR + TR + i * 32 + lane] = d[i] * (-1.0f / P_SCALE);
+            sStat[st * 2 * TR + i * 32 + lane] = l[i] == -INFINITY ? 0.0f : -l[i] * LOG2E;
+            sStat[st * 2 * TR + TR + i * 32 + lane] = d[i];
           }
           __syncwarp();
         }
@@ -788,21 +752,22 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       }
   } else if (warp >= 4) {
     regs_inc();
-    const int quad = warp & 3, grp = (warp - 4) >> 3, half = ((warp - 4) >> 2) & 1;  // columns [64 half, 64 half + 64)
+    const int quad = warp & 3, grp = (warp - 4) >> 2;
     const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
-    const uint32_t ts = tmem + half * 64 + lanes;
+    const uint32_t ts = tmem + lanes;
     // dk/dv: P at COL_P, dS 64 columns on; dq: a dS for each group
-    const uint32_t tp = tmem + COL_P + half * 32 + lanes, td = tp + (DQ ? grp * 64 : 64);
+    const uint32_t tp = tmem + COL_P + lanes, td = tp + (DQ ? grp * 64 : 64);
     const float sl2 = a.scale * LOG2E;
     const int trow = quad * 32 + lane;
-    constexpr int W = DQ ? 32 : 64;  // this warp's columns of the results: half of dq, or all of dv (half 0) or dk (half 1)
     auto skipped = [&](const Item& I) {  // no own rows, or nothing to stream: zeros
       const int row = I.r0 + trow;
       if (grp != 0 || row >= total_own) return;
-      const HeadsView& v = DQ || half == 0 ? g1 : g2;
       const int b = by_batch(I.bh), h = I.bh - b * a.heads;
-      store_zeros(static_cast<__nv_bfloat16*>(v.p) + b * v.sb + h * v.sh + row * v.st + (DQ ? half * 32 : 0), W);
-      if (DQ && half == 0) delta[static_cast<size_t>(I.bh) * a.nq + row] = 0.0f;
+      store_zeros(static_cast<__nv_bfloat16*>(g1.p) + b * g1.sb + h * g1.sh + row * g1.st);
+      if constexpr (DQ)
+        delta[static_cast<size_t>(I.bh) * a.nq + row] = 0.0f;
+      else
+        store_zeros(static_cast<__nv_bfloat16*>(g2.p) + b * g2.sb + h * g2.sh + row * g2.st);
     };
     auto own_lse = [&](const Item& I) {
       const int row = I.r0 + trow;
@@ -823,22 +788,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       tc_fence_after();
       settle();
       const bool live = I.r0 + trow < I.own;
-      const int b = by_batch(I.bh), h = I.bh - b * a.heads;
-      uint8_t* stage = sOwn + (c & 1) * 2 * TILE_B + (half * 4 + quad) * (W * 64);
-      const float f = DQ || half == 1 ? a.scale : 1.0f / P_SCALE;
-#pragma unroll
-      for (int d0 = 0; d0 < W; d0 += 16) {
-        uint32_t r[16];
-        tmem_ld16(tmem + COL_ACC + lanes + half * W + d0, r);
-        tmem_wait_ld();
-        float x[16];
-#pragma unroll
-        for (int d = 0; d < 16; ++d) x[d] = live ? __uint_as_float(r[d]) : 0.0f;
-        *staged<W * 2>(stage, lane, d0 / 8) = pack8(x, f);
-        *staged<W * 2>(stage, lane, d0 / 8 + 1) = pack8(x + 8, f);
-      }
+      const int b = by_batch(I.bh), h = I.bh - b * a.heads, y = I.r0 + quad * 32;
+      uint8_t* stage = sOwn + (c & 1) * 2 * TILE_B + quad * 4096;
+      stage_row(stage, lane, tmem + COL_ACC + lanes, DQ ? a.scale : 1.0f, live);
+      if constexpr (!DQ) stage_row(stage + TILE_B, lane, tmem + COL_ACC + 64 + lanes, a.scale, live);
       tc_fence_before();
-      send_rows(DQ || half == 0 ? &tmG1 : &tmG2, stage, DQ ? half * 32 : 0, I.r0 + quad * 32, total_own, h, b, lane);
+      send_rows(&tmG1, stage, y, total_own, h, b, lane);
+      if constexpr (!DQ) send_rows(&tmG2, stage + TILE_B, y, total_own, h, b, lane);
       owed = static_cast<int>(c);
       if (lane == 0) mbar_arrive(acc_free);
       return true;
@@ -851,7 +807,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       const Item N = seek(I.it + gridDim.x, skipped);
       float2 shift2, delta2 = make_float2(0.0f, 0.0f);
       if constexpr (DQ) {
-        shift2.x = shift2.y = lse_next == -INFINITY ? 0.0f : fmaf(lse_next, -LOG2E, P_SHIFT);
+        shift2.x = shift2.y = lse_next == -INFINITY ? 0.0f : -lse_next * LOG2E;
         lse_next = own_lse(N);
       }
       bool fresh = true;  // this group has had no block of the item yet
@@ -864,24 +820,19 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         }
         if (!(ok = warp_wait(&s_full[grp], (n >> 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
         tc_fence_after();
-        uint32_t ph[32], pk[DQ ? 1 : 32];  // 2^15 p as f16, and as bf16 for dv
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          uint32_t r[32];
-          tmem_ld32(ts + q * 32, r);
-          tmem_wait_ld();
-          if (q == 1) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(s_free);
-          }
+        float p[128];
+        {
+          uint32_t r[128];
+          tmem_ld128(ts, r);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(s_free);
           if constexpr (DQ) {
-            const int valid = I.len - j * TR - half * 64 - q * 32;
-            if (valid < 32) mask_columns(r, valid);
+            if (I.len - j * TR < TR) mask_columns(r, I.len - j * TR);
           }
-          const float4* sl = reinterpret_cast<const float4*>(sStat + st * 2 * TR + half * 64 + q * 32);
+          const float4* sl = reinterpret_cast<const float4*>(sStat + st * 2 * TR);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
+          for (int i = 0; i < 64; ++i) {
             float2 sh = shift2;
             if constexpr (!DQ) {
               const float4 v = sl[i / 2];
@@ -889,22 +840,20 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
             }
             const float2 e = exp2_pair<B_MASK>(
                 ffma2(make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), make_float2(sl2, sl2), sh), i);
-            ph[q * 16 + i] = pack_f16x2(e.x, e.y);
-            if constexpr (!DQ) pk[q * 16 + i] = pack_bf16x2(e.x, e.y);
+            p[2 * i] = e.x, p[2 * i + 1] = e.y;
           }
         }
         settle();
         if (DQ && fresh) {
-          // delta, from the tiles of out and d_out, by the group that has the item's first block: 32 of a row's 64
-          // products per thread, which meet in shared memory
-          float* parts = sStat + (c & 1) * 2 * TR;
+          // delta, from the tiles of out and d_out, by the group that has the item's first block
+          float* row_delta = sStat + (c & 1) * TR;
           if (j == 0) {
             if (!(ok = warp_wait(&own_full[c & 1], (c >> 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
             const uint8_t* og = sOwn + ((c & 1) * 2 + 1) * TILE_B;
             float x = 0.0f, y = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int at = trow * 128 + (((half * 4 + i) ^ trow) & 7) * 16;
+            for (int i = 0; i < 8; ++i) {
+              const int at = trow * 128 + ((i ^ trow) & 7) * 16;
               const uint4 ov = *reinterpret_cast<const uint4*>(sOut + at), gv = *reinterpret_cast<const uint4*>(og + at);
               const uint32_t o[4] = {ov.x, ov.y, ov.z, ov.w}, g[4] = {gv.x, gv.y, gv.z, gv.w};
 #pragma unroll
@@ -913,40 +862,49 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
                 y = fmaf(__uint_as_float(o[u] & 0xffff0000u), __uint_as_float(g[u] & 0xffff0000u), y);
               }
             }
-            parts[half * TR + trow] = x + y;
+            delta2.x = x + y;
+            row_delta[trow] = delta2.x;
             __syncwarp();
             if (lane == 0) mbar_arrive(&part_full[c & 1]);
+            const int row = I.r0 + trow;
+            if (row < total_own) delta[static_cast<size_t>(I.bh) * a.nq + row] = row < I.own ? delta2.x : 0.0f;
+          } else {
+            if (!(ok = warp_wait(&part_full[c & 1], (c >> 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
+            delta2.x = row_delta[trow];
           }
-          if (!(ok = warp_wait(&part_full[c & 1], (c >> 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
-          const float dl = parts[trow] + parts[TR + trow];
-          delta2.x = delta2.y = dl * (-1.0f / P_SCALE);
-          const int row = I.r0 + trow;
-          if (j == 0 && half == 0 && row < total_own) delta[static_cast<size_t>(I.bh) * a.nq + row] = row < I.own ? dl : 0.0f;
+          delta2.y = delta2.x;
         }
         fresh = false;
         if constexpr (!DQ) {
           if (n > 0 && !(ok = warp_wait(p_free, (n - 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
           tc_fence_after();
-          tmem_st32(tp, pk);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) pk[i] = pack_bf16x2(p[q * 32 + 2 * i], p[q * 32 + 2 * i + 1]);
+            tmem_st16(tp + q * 16, pk);
+          }
           tmem_wait_st();
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(p_full);
         }
         if (!(ok = warp_wait(&dp_full[grp], (n >> 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
+        // (dq: this group's last dS was used before dP(n) was computed)
+        if (!DQ && n > 0 && !(ok = warp_wait(ds_free, (n - 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
         tc_fence_after();
-        uint32_t dk[32];
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          uint32_t r[32];
+        for (int q = 0; q < 4; ++q) {
+          uint32_t r[32], pk[16];
           tmem_ld32(ts + COL_DP + q * 32, r);
           tmem_wait_ld();
-          if (q == 1) {
+          if (q == 3) {
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(dp_free);
           }
-          const float4* sd = reinterpret_cast<const float4*>(sStat + st * 2 * TR + TR + half * 64 + q * 32);
+          const float4* sd = reinterpret_cast<const float4*>(sStat + st * 2 * TR + TR + q * 32);
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             float2 dl = delta2;
@@ -954,17 +912,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
               const float4 v = sd[i / 2];
               dl = i & 1 ? make_float2(v.z, v.w) : make_float2(v.x, v.y);
             }
-            const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&ph[q * 16 + i]));
-            const float2 ds = fmul2(ffma2(make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])),
-                                          make_float2(1.0f / P_SCALE, 1.0f / P_SCALE), dl),
-                                    p);
-            dk[q * 16 + i] = pack_bf16x2(ds.x, ds.y);
+            const float2 ds = fmul2(fsub2(make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), dl),
+                                    make_float2(p[q * 32 + 2 * i], p[q * 32 + 2 * i + 1]));
+            pk[i] = pack_bf16x2(ds.x, ds.y);
           }
+          tmem_st16(td + q * 16, pk);
         }
-        // (dq: this group's last dS was used before dP(n) was computed)
-        if (!DQ && n > 0 && !(ok = warp_wait(ds_free, (n - 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
-        tc_fence_after();
-        tmem_st32(td, dk);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -986,13 +939,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
 
 // ------------------------------------------------------------------ launches
 namespace {
-// Boxes of `rows` rows and `cols` of the 64 columns.
-bool heads_map(CUtensorMap* m, const HeadsView& v, int batch, int heads, int tokens, uint32_t rows = TR, uint32_t cols = 64) {
+bool heads_map(CUtensorMap* m, const HeadsView& v, int batch, int heads, int tokens, uint32_t rows = TR) {
   const uint64_t dims[4] = {64, static_cast<uint64_t>(tokens), static_cast<uint64_t>(heads), static_cast<uint64_t>(batch)};
   const uint64_t strides[3] = {static_cast<uint64_t>(v.st) * 2, static_cast<uint64_t>(v.sh) * 2, static_cast<uint64_t>(v.sb) * 2};
-  const uint32_t box[4] = {cols, rows, 1, 1};
-  return make_tmap_nd(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, v.p, 4, dims, strides, box,
-                      cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+  const uint32_t box[4] = {64, rows, 1, 1};
+  return make_tmap_nd(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, v.p, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 }  // namespace
 
@@ -1000,7 +951,7 @@ cudaError_t attention_forward_tc(const AttnShape& a, HeadsView q, HeadsView k, H
                                  int* err, cudaStream_t s) {
   CUtensorMap mq, mk, mv, mo;
   if (!heads_map(&mq, q, a.batch, a.heads, a.nq) || !heads_map(&mk, k, a.batch, a.heads, a.nk) ||
-      !heads_map(&mv, v, a.batch, a.heads, a.nk) || !heads_map(&mo, out, a.batch, a.heads, a.nq, 32, 32))
+      !heads_map(&mv, v, a.batch, a.heads, a.nk) || !heads_map(&mo, out, a.batch, a.heads, a.nq, 32))
     return cudaErrorInvalidValue;
   const void* fn = reinterpret_cast<const void*>(k_attn_forward_tc);
   const cudaError_t e = ensure_smem_limit(fn, static_cast<int>(F_SMEM));
@@ -1021,7 +972,7 @@ cudaError_t attention_backward_tc(const AttnShape& a, HeadsView q, HeadsView k, 
   CUtensorMap mq, mk, mv, mg, mo, mdq, mdk, mdv;
   if (!heads_map(&mq, q, a.batch, a.heads, a.nq) || !heads_map(&mk, k, a.batch, a.heads, a.nk) ||
       !heads_map(&mv, v, a.batch, a.heads, a.nk) || !heads_map(&mg, d_out, a.batch, a.heads, a.nq) ||
-      !heads_map(&mo, out, a.batch, a.heads, a.nq) || !heads_map(&mdq, dq, a.batch, a.heads, a.nq, 32, 32) ||
+      !heads_map(&mo, out, a.batch, a.heads, a.nq) || !heads_map(&mdq, dq, a.batch, a.heads, a.nq, 32) ||
       !heads_map(&mdk, dk, a.batch, a.heads, a.nk, 32) || !heads_map(&mdv, dv, a.batch, a.heads, a.nk, 32))
     return cudaErrorInvalidValue;
   cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(k_attn_backward_tc<true>), static_cast<int>(B_SMEM));

@@ -10,9 +10,9 @@
 // instead of 5).
 //
 //   warp 0       TMA producer
-//   warp 1       TMEM owner; one thread issues the MMAs
+//   warp 1       TMEM owner; one thread issues MMAs
 //   warp 2       with lengths: clears the tails of streamed tiles
-//   warp 3       idle: register shares go by groups of four warps
+//   warp 3       one thread issues MMAs
 //   warps 4..11  the elementwise work on S (and dP) in TMEM: two groups of four
 //                warps, a row of 128 columns per thread.  (16 warps with 64
 //                or 32 columns each spent half of their instructions on
@@ -228,8 +228,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   uint64_t* s_free = s_full + 2;       // [2] tile: S read
   uint64_t* p_full = s_free + 2;       // [2] tile: P written
   uint64_t* p_free = p_full + 2;       // [2] tile: P used, O complete up to its block
-  uint64_t* stopped = p_free + 2;      // every product done, after an error
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(stopped + 1);
+  uint64_t* started = p_free + 2;      // tile 0 has read its first S
+  uint64_t* stopped = started + 1;     // [2] every product of the tile done, after an error
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(stopped + 2);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   struct Item {
@@ -261,10 +262,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     }
     for (int i = 0; i < ST; ++i) {
       mbar_init(&kv_full[i], 1);
-      mbar_init(&kv_empty[i], 1);
+      mbar_init(&kv_empty[i], tpi);
       mbar_init(&kv_clean[i], 1);
     }
-    mbar_init(stopped, 1);
+    mbar_init(started, 4);
+    mbar_init(&stopped[0], 1);
+    mbar_init(&stopped[1], 1);
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -311,57 +314,81 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         for (uint32_t i = c > 2 ? c - 2 : 0; i < c; ++i) drain(&q_full[i & 1], (i >> 1) & 1);
       }
     }
-  } else if (warp == 1) {
+  } else if (warp == 1 || (warp == 3 && tpi > 1)) {
+    // Each tile's MMAs come from a thread of their own, S a block ahead of P V:
+    // one thread for both would have to wait for their hand-overs in a fixed
+    // order.
     if (elect_one()) {
       constexpr uint32_t idS = idesc_bf16(128, 128), idO = idesc_bf16_bmn(128, 64);
+      const int t = warp == 1 ? 0 : 1;
       uint64_t* kv_ready = a.kv_lens != nullptr ? kv_clean : kv_full;
-      uint32_t g = 0, c = 0;  // blocks, items with work
-      uint32_t n0 = 0, n1 = 0;  // blocks of each tile
+      // One block of the walk: block j of nb of the c-th item with work.
+      struct Blk {
+        int it, tiles, j, nb;
+        uint32_t c;
+      };
+      auto load = [&](Blk k) {
+        for (; k.it < items; k.it += gridDim.x) {
+          const Item I = item_of(k.it);
+          k.tiles = I.tiles;
+          k.nb = I.nb;
+          if (I.tiles > 0) break;
+        }
+        k.j = 0;
+        return k;
+      };
+      auto next = [&](Blk k) {
+        if (++k.j < k.nb) return k;
+        k.it += gridDim.x;
+        ++k.c;
+        return load(k);
+      };
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity) { return ok = ok && thread_wait(bar, parity & 1, err, VK_DEV_TIMEOUT_MMA); };
-      for (int it = blockIdx.x; it < items && ok; it += gridDim.x) {
-        const Item I = item_of(it);
-        if (I.tiles == 0) continue;
-        const uint32_t qb = c & 1;
-        // S of tile t, block n of that tile, once its last S has been read
-        auto issue_s = [&](int t, uint32_t n, uint32_t st) {
-          if (n > 0 && !wait(&s_free[t], n - 1)) return;
-          tc_fence_after();
-          const uint64_t qd = smem_desc_k_sw128(smem_u32(sQ + (qb * 2 + t) * TILE_B));
-          const uint64_t kd = smem_desc_k_sw128(smem_u32(sK + st * TILE_B));
+      // S of block g, the n-th of this tile, once its last S has been read.
+      // (Every block is waited for, also where tile 1 has no work, so that no
+      // phase is missed; an item's queries come before its keys.)
+      auto issue_s = [&](const Blk& k, uint32_t n, uint32_t g) {
+        if (k.it >= items || !wait(&kv_ready[g % ST], g / ST) || t >= k.tiles) return;
+        if (k.j == 0) wait(&q_full[k.c & 1], k.c >> 1);
+        if (n > 0) wait(&s_free[t], n - 1);
+        if (!ok) return;
+        tc_fence_after();
+        const uint64_t qd = smem_desc_k_sw128(smem_u32(sQ + ((k.c & 1) * 2 + t) * TILE_B));
+        const uint64_t kd = smem_desc_k_sw128(smem_u32(sK + g % ST * TILE_B));
 #pragma unroll
-          for (int k = 0; k < 4; ++k) umma_f16(tmem + t * TR, qd + k * 2, kd + k * 2, idS, k > 0 ? 1u : 0u);
-          umma_commit(&s_full[t]);
-        };
-        auto issue_o = [&](int t, uint32_t n, uint32_t st, bool first) {
-          if (!wait(&p_full[t], n)) return;
+        for (int i = 0; i < 4; ++i) umma_f16(tmem + t * TR, qd + i * 2, kd + i * 2, idS, i > 0 ? 1u : 0u);
+        umma_commit(&s_full[t]);
+      };
+      uint32_t n = 0;  // blocks of this tile
+      Blk k = load(Blk{static_cast<int>(blockIdx.x), 0, 0, 0, 0});
+      // Tile 1 starts when tile 0 is about to take its exponentials: half a
+      // block apart, the two share MUFU in turn (in step they took 3600 cycles
+      // for a block of both, 2048 of them MUFU's).
+      if (t == 1 && k.it < items) wait(started, 0);
+      issue_s(k, 0, 0);
+      for (uint32_t g = 0; ok && k.it < items; ++g) {
+        const Blk b = next(k);
+        const bool mine = t < k.tiles;
+        issue_s(b, n + mine, g + 1);
+        if (mine) {
+          if (!wait(&p_full[t], n)) break;
           tc_fence_after();
-          const uint64_t vd = smem_desc_mn_sw128(smem_u32(sV + st * TILE_B));
-#pragma unroll
-          for (int k = 0; k < 8; ++k)
-            umma_f16_ts(tmem + F_O + t * 64, tmem + F_P + t * 64 + k * 8, vd + static_cast<uint64_t>(k * (2048 >> 4)), idO,
-                        first && k == 0 ? 0u : 1u);
-          umma_commit(&p_free[t]);
-        };
-        if (!wait(&q_full[qb], c >> 1) || !wait(&kv_ready[g % ST], g / ST)) break;
-        ++c;
-        issue_s(0, n0, g % ST);
-        if (I.tiles > 1) issue_s(1, n1, g % ST);
-        for (int j = 0; j < I.nb && ok; ++j, ++g, ++n0, n1 += I.tiles - 1) {
-          if (j + 1 < I.nb) {
-            if (!wait(&kv_ready[(g + 1) % ST], (g + 1) / ST)) break;
-            issue_s(0, n0 + 1, (g + 1) % ST);
-            if (I.tiles > 1) issue_s(1, n1 + 1, (g + 1) % ST);
-          }
+          const uint64_t vd = smem_desc_mn_sw128(smem_u32(sV + g % ST * TILE_B));
           // (an item's first product overwrites O: its warps read the last item's before they hand over P)
-          issue_o(0, n0, g % ST, j == 0);
-          if (I.tiles > 1) issue_o(1, n1, g % ST, j == 0);
-          umma_commit(&kv_empty[g % ST]);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            umma_f16_ts(tmem + F_O + t * 64, tmem + F_P + t * 64 + i * 8, vd + static_cast<uint64_t>(i * (2048 >> 4)), idO,
+                        k.j == 0 && i == 0 ? 0u : 1u);
+          umma_commit(&p_free[t]);
+          ++n;
         }
+        umma_commit(&kv_empty[g % ST]);
+        k = b;
       }
       if (!ok) {
-        umma_commit(stopped);
-        drain(stopped, 0);
+        umma_commit(&stopped[t]);
+        drain(&stopped[t], 0);
       }
     }
   } else if (warp == 2 && a.kv_lens != nullptr) {
@@ -414,8 +441,6 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         uint32_t r[128];
         tmem_ld128(ts, r);
         tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&s_free[t]);
         if (I.nk - j * TR < TR) mask_columns(r, I.nk - j * TR);
         float pm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -443,6 +468,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
             l_run *= f;
             m_ref = m_new;
           }
+        }
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&s_free[t]);
+          if (t == 0 && n == 0) mbar_arrive(started);
         }
         const float2 scale2 = make_float2(sl2, sl2), shift2 = make_float2(-m_ref, -m_ref);
         float2 ps[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};

@@ -197,13 +197,18 @@ __device__ __forceinline__ float2 exp2_pair(float2 x, int i) {
 }  // namespace
 
 // ------------------------------------------------------------------ forward
-// An item is two query tiles of a head (one where pairs would leave SMs idle),
-// each with its own group of four warps.  TMEM: S of the tiles [0, 128) and
+// An item is two query tiles, each with its own group of four warps, that
+// share the K / V blocks of their head (one tile where pairs would leave SMs
+// idle).  Without lengths, the last tiles of heads with an odd number of tiles
+// pair up across heads; such an item streams two K / V sequences in turn.
+// (865 tokens are 7 tiles: 19 items a CTA instead of 21 at 64 images.)  TMEM: S of the tiles [0, 128) and
 // [128, 256), P as bf16 [256, 320) and [320, 384), O [384, 448) and [448, 512).
 // S is handed back as soon as it is in registers, so that the next block's is
 // there when the warps ask for it: they are bound by their exponentials.
 namespace {
-constexpr uint32_t F_MASK = 0x0u;
+// Pairs of columns (of each 16) whose exponentials go to the FMA pipe:
+// measured at 64 images, 298 us for none, 293 for 4, 309 for 6.
+constexpr uint32_t F_MASK = 0x1111u;
 constexpr uint32_t F_P = 256, F_O = 384;
 constexpr size_t F_SMEM = 1024 + TILE_B * (4 + 2 * ST) + 512;
 }  // namespace
@@ -211,8 +216,8 @@ constexpr size_t F_SMEM = 1024 + TILE_B * (4 + 2 * ST) + 512;
 __global__ void __launch_bounds__(TC_THREADS, 1)
     k_attn_forward_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                       const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO, AttnShape a,
-                      HeadsView out, float* __restrict__ lse, int items, int per_head, FastDiv by_head, FastDiv by_batch,
-                      int tpi, int* err) {
+                      HeadsView out, float* __restrict__ lse, int items, int per_head, int mixed_from, FastDiv by_head,
+                      FastDiv by_batch, int tpi, int* err) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;  // [item parity][tile], then the tile's output on its way out
@@ -234,19 +239,32 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   struct Item {
-    int b, h, q0, tiles, nb, nq, nk;  // tiles: how many of its tiles have queries and keys
+    int bh[2], q0[2];  // (sequence, head) and first query of its tiles
+    int tiles;         // how many of its tiles have queries and keys
+    int kvs;           // K / V sequences that it streams
+    int nb, nq, nk;    // blocks of a sequence, its queries and keys
   };
   auto item_of = [&](int it) {
     Item r;
-    const int bh = by_head(it);
-    r.b = by_batch(bh);
-    r.h = bh - r.b * a.heads;
-    r.q0 = (it - bh * per_head) * tpi * TR;
-    r.nq = seq_len(a.q_lens, r.b, a.nq);
-    r.nk = seq_len(a.kv_lens, r.b, a.nk);
+    r.kvs = 1;
+    if (it < mixed_from) {
+      r.bh[0] = r.bh[1] = by_head(it);
+      r.q0[0] = (it - r.bh[0] * per_head) * tpi * TR;
+      r.q0[1] = r.q0[0] + TR;
+    } else {
+      r.bh[0] = 2 * (it - mixed_from);
+      r.bh[1] = r.bh[0] + 1;
+      r.q0[0] = r.q0[1] = (a.nq - 1) / TR * TR;
+      if (r.bh[1] < a.batch * a.heads)
+        r.kvs = 2;
+      else
+        r.q0[1] = a.nq;  // the last head of an odd number
+    }
+    const int b = by_batch(r.bh[0]);  // (one length for all where two sequences meet)
+    r.nq = seq_len(a.q_lens, b, a.nq);
+    r.nk = seq_len(a.kv_lens, b, a.nk);
     r.nb = (r.nk + TR - 1) / TR;
-    r.tiles = r.nb == 0 ? 0 : min(tpi, (r.nq - r.q0 + TR - 1) / TR);
-    if (r.tiles < 0) r.tiles = 0;
+    r.tiles = r.nb == 0 || r.q0[0] >= r.nq ? 0 : tpi == 2 && r.q0[1] < r.nq ? 2 : 1;
     return r;
   };
 
@@ -300,13 +318,17 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         if (!ok) break;
         ++c;
         mbar_arrive_expect_tx(&q_full[qb], I.tiles * TILE_B);
-        for (int t = 0; t < I.tiles; ++t) tma_load_4d(sQ + (qb * 2 + t) * TILE_B, &tmQ, &q_full[qb], I.q0 + t * TR, I.h, I.b);
-        for (int j = 0; j < I.nb; ++j, ++g) {
+        const int b0 = by_batch(I.bh[0]), h0 = I.bh[0] - b0 * a.heads, b1 = by_batch(I.bh[1]), h1 = I.bh[1] - b1 * a.heads;
+        tma_load_4d(sQ + qb * 2 * TILE_B, &tmQ, &q_full[qb], I.q0[0], h0, b0);
+        if (I.tiles > 1) tma_load_4d(sQ + (qb * 2 + 1) * TILE_B, &tmQ, &q_full[qb], I.q0[1], h1, b1);
+        for (int j = 0; j < I.nb * I.kvs; ++j, ++g) {
           const uint32_t st = g % ST;
           if (!(ok = thread_wait(&kv_empty[st], ((g / ST) & 1) ^ 1, err, VK_DEV_TIMEOUT_PRODUCER))) break;
+          const bool second = I.kvs == 2 && (j & 1);
+          const int y = (I.kvs == 2 ? j >> 1 : j) * TR, h = second ? h1 : h0, b = second ? b1 : b0;
           mbar_arrive_expect_tx(&kv_full[st], 2 * TILE_B);
-          tma_load_4d(sK + st * TILE_B, &tmK, &kv_full[st], j * TR, I.h, I.b);
-          tma_load_4d(sV + st * TILE_B, &tmV, &kv_full[st], j * TR, I.h, I.b);
+          tma_load_4d(sK + st * TILE_B, &tmK, &kv_full[st], y, h, b);
+          tma_load_4d(sV + st * TILE_B, &tmV, &kv_full[st], y, h, b);
         }
       }
       if (*reinterpret_cast<volatile int*>(err) != 0) {
@@ -322,68 +344,87 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       constexpr uint32_t idS = idesc_bf16(128, 128), idO = idesc_bf16_bmn(128, 64);
       const int t = warp == 1 ? 0 : 1;
       uint64_t* kv_ready = a.kv_lens != nullptr ? kv_clean : kv_full;
-      // One block of the walk: block j of nb of the c-th item with work.
-      struct Blk {
-        int it, tiles, j, nb;
-        uint32_t c;
+      // One slot of the K / V ring: slot j of the c-th item with work, `mine` if
+      // this tile uses it.
+      struct Slot {
+        int it, tiles, kvs, j, nb;
+        uint32_t c, g;  // ordinals of the item and of the slot
+        bool mine;
       };
-      auto load = [&](Blk k) {
+      auto load = [&](Slot k) {
         for (; k.it < items; k.it += gridDim.x) {
           const Item I = item_of(k.it);
           k.tiles = I.tiles;
-          k.nb = I.nb;
+          k.kvs = I.kvs;
+          k.nb = I.nb * I.kvs;
           if (I.tiles > 0) break;
         }
         k.j = 0;
+        k.mine = k.kvs == 2 ? t == 0 : t < k.tiles;
         return k;
       };
-      auto next = [&](Blk k) {
-        if (++k.j < k.nb) return k;
+      auto next = [&](Slot k) {
+        ++k.g;
+        if (++k.j < k.nb) {
+          if (k.kvs == 2) k.mine = !k.mine;
+          return k;
+        }
         k.it += gridDim.x;
         ++k.c;
         return load(k);
       };
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity) { return ok = ok && thread_wait(bar, parity & 1, err, VK_DEV_TIMEOUT_MMA); };
-      // S of block g, the n-th of this tile, once its last S has been read.
-      // (Every block is waited for, also where tile 1 has no work, so that no
-      // phase is missed; an item's queries come before its keys.)
-      auto issue_s = [&](const Blk& k, uint32_t n, uint32_t g) {
-        if (k.it >= items || !wait(&kv_ready[g % ST], g / ST) || t >= k.tiles) return;
-        if (k.j == 0) wait(&q_full[k.c & 1], k.c >> 1);
+      // Lets slots of the other tile go (each is waited for, so that no phase is missed).
+      auto skip = [&](Slot& k) {
+        while (k.it < items && !k.mine && wait(&kv_ready[k.g % ST], k.g / ST)) {
+          umma_commit(&kv_empty[k.g % ST]);
+          k = next(k);
+        }
+      };
+      // S of this tile's n-th block, once its last S has been read (an item's queries come before its keys)
+      auto issue_s = [&](const Slot& k, uint32_t n) {
+        if (k.it >= items || !wait(&kv_ready[k.g % ST], k.g / ST)) return;
+        if (k.j < k.kvs) wait(&q_full[k.c & 1], k.c >> 1);
         if (n > 0) wait(&s_free[t], n - 1);
         if (!ok) return;
         tc_fence_after();
         const uint64_t qd = smem_desc_k_sw128(smem_u32(sQ + ((k.c & 1) * 2 + t) * TILE_B));
-        const uint64_t kd = smem_desc_k_sw128(smem_u32(sK + g % ST * TILE_B));
+        const uint64_t kd = smem_desc_k_sw128(smem_u32(sK + k.g % ST * TILE_B));
 #pragma unroll
         for (int i = 0; i < 4; ++i) umma_f16(tmem + t * TR, qd + i * 2, kd + i * 2, idS, i > 0 ? 1u : 0u);
         umma_commit(&s_full[t]);
       };
-      uint32_t n = 0;  // blocks of this tile
-      Blk k = load(Blk{static_cast<int>(blockIdx.x), 0, 0, 0, 0});
+      Slot k = load(Slot{static_cast<int>(blockIdx.x), 0, 1, 0, 0, 0, 0, false});
       // Tile 1 starts when tile 0 is about to take its exponentials: half a
       // block apart, the two share MUFU in turn (in step they took 3600 cycles
       // for a block of both, 2048 of them MUFU's).
       if (t == 1 && k.it < items) wait(started, 0);
-      issue_s(k, 0, 0);
-      for (uint32_t g = 0; ok && k.it < items; ++g) {
-        const Blk b = next(k);
-        const bool mine = t < k.tiles;
-        issue_s(b, n + mine, g + 1);
-        if (mine) {
-          if (!wait(&p_full[t], n)) break;
-          tc_fence_after();
-          const uint64_t vd = smem_desc_mn_sw128(smem_u32(sV + g % ST * TILE_B));
-          // (an item's first product overwrites O: its warps read the last item's before they hand over P)
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            umma_f16_ts(tmem + F_O + t * 64, tmem + F_P + t * 64 + i * 8, vd + static_cast<uint64_t>(i * (2048 >> 4)), idO,
-                        k.j == 0 && i == 0 ? 0u : 1u);
-          umma_commit(&p_free[t]);
-          ++n;
+      skip(k);
+      issue_s(k, 0);
+      for (uint32_t n = 0; ok && k.it < items; ++n) {
+        // The next S goes first where it needs at most the slot after the next:
+        // further on, the ring would wait for this block's.
+        Slot b = next(k);
+        const bool near = b.it < items && (b.mine || b.kvs == 2);
+        if (near) {
+          skip(b);
+          issue_s(b, n + 1);
         }
-        umma_commit(&kv_empty[g % ST]);
+        if (!wait(&p_full[t], n)) break;
+        tc_fence_after();
+        const uint64_t vd = smem_desc_mn_sw128(smem_u32(sV + k.g % ST * TILE_B));
+        // (an item's first product overwrites O: its warps read the last item's before they hand over P)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          umma_f16_ts(tmem + F_O + t * 64, tmem + F_P + t * 64 + i * 8, vd + static_cast<uint64_t>(i * (2048 >> 4)), idO,
+                      k.j < k.kvs && i == 0 ? 0u : 1u);
+        umma_commit(&p_free[t]);
+        umma_commit(&kv_empty[k.g % ST]);
+        if (!near) {
+          skip(b);
+          issue_s(b, n + 1);
+        }
         k = b;
       }
       if (!ok) {
@@ -397,7 +438,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     for (int it = blockIdx.x; it < items && ok; it += gridDim.x) {
       const Item I = item_of(it);
       if (I.tiles == 0) continue;
-      for (int j = 0; j < I.nb; ++j, ++g) {
+      for (int j = 0; j < I.nb; ++j, ++g) {  // (with lengths, an item streams one sequence)
         if (!(ok = warp_wait(&kv_full[g % ST], (g / ST) & 1, err, VK_DEV_TIMEOUT_OTHER))) break;
         if (I.nk - j * TR < TR) zero_tail(sK + g % ST * TILE_B, sV + g % ST * TILE_B, I.nk - j * TR, lane);
         if (lane == 0) mbar_arrive(&kv_clean[g % ST]);
@@ -422,13 +463,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
     bool ok = true;
     for (int it = blockIdx.x; it < items && ok && t < tpi; it += gridDim.x) {
       const Item I = item_of(it);
-      const int row = I.q0 + t * TR + trow;
-      float* lp = lse + (static_cast<size_t>(I.b) * a.heads + I.h) * a.nq + row;
+      const int bh = t ? I.bh[1] : I.bh[0], q0 = t ? I.q0[1] : I.q0[0], row = q0 + trow;
+      const int b = by_batch(bh), h = bh - b * a.heads;
+      float* lp = lse + static_cast<size_t>(bh) * a.nq + row;
       const int qb = c & 1;
       if (I.tiles > 0) ++c;
       if (t >= I.tiles) {  // no queries here, or no keys
         if (row < a.nq) {
-          store_zeros(static_cast<__nv_bfloat16*>(out.p) + I.b * out.sb + I.h * out.sh + row * out.st);
+          store_zeros(static_cast<__nv_bfloat16*>(out.p) + b * out.sb + h * out.sh + row * out.st);
           *lp = -INFINITY;
         }
         settle();
@@ -501,7 +543,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       uint8_t* stage = sQ + (qb * 2 + t) * TILE_B + quad * 4096;
       stage_row(stage, lane, to, live ? 1.0f / l_run : 0.0f, live);
       tc_fence_before();
-      send_rows(&tmO, stage, I.q0 + t * TR + quad * 32, a.nq, I.h, I.b, lane);
+      send_rows(&tmO, stage, q0 + quad * 32, a.nq, h, b, lane);
       owed = qb;
       if (row < a.nq) *lp = live ? fmaf(m_ref, LN2, logf(l_run)) : -INFINITY;
     }
@@ -989,10 +1031,15 @@ cudaError_t attention_forward_tc(const AttnShape& a, HeadsView q, HeadsView k, H
   // Two query tiles share each K / V block; one where pairs would leave SMs idle.
   const int nt = (a.nq + TR - 1) / TR, bh = a.batch * a.heads;
   const int tpi = (nt + 1) / 2 * bh < num_sms() ? 1 : 2;
-  const int per_head = (nt + tpi - 1) / tpi, items = per_head * bh;
+  int per_head = (nt + tpi - 1) / tpi, items = per_head * bh, mixed_from = items;
+  if (tpi == 2 && nt % 2 == 1 && a.q_lens == nullptr && a.kv_lens == nullptr) {
+    per_head = nt / 2;
+    mixed_from = per_head * bh;
+    items = mixed_from + (bh + 1) / 2;
+  }
   const int grid = items < num_sms() ? items : num_sms();
-  k_attn_forward_tc<<<grid, TC_THREADS, F_SMEM, s>>>(mq, mk, mv, mo, a, out, lse, items, per_head, FastDiv(per_head),
-                                                     FastDiv(a.heads), tpi, err);
+  k_attn_forward_tc<<<grid, TC_THREADS, F_SMEM, s>>>(mq, mk, mv, mo, a, out, lse, items, per_head, mixed_from,
+                                                     FastDiv(per_head > 0 ? per_head : 1), FastDiv(a.heads), tpi, err);
   return cudaGetLastError();
 }
 

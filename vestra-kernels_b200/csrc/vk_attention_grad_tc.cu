@@ -13,7 +13,8 @@
 //   warp 1       TMEM owner; one thread issues MMAs
 //   warp 2       with lengths: clears the tails of streamed tiles
 //   warp 3       one thread issues MMAs
-//   warps 4..11  the elementwise work on S (and dP) in TMEM: two groups of four
+//   warps 4..7   backward: delta, and the results on their way to memory
+//   the others   the elementwise work on S (and dP) in TMEM: two groups of four
 //                warps, a row of 128 columns per thread.  (16 warps with 64
 //                or 32 columns each spent half of their instructions on
 //                waits and hand-overs, and most of their time in step.)
@@ -33,7 +34,7 @@ namespace {
 constexpr int TR = 128;                 // rows of a tile, columns of a block
 constexpr int TILE_B = TR * 128;        // bytes of 128 rows of 64 bf16
 constexpr int ST = 4;                   // streamed blocks in flight
-constexpr int TC_THREADS = 12 * 32;
+constexpr int F_THREADS = 12 * 32, B_THREADS = 16 * 32;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 __device__ __forceinline__ void tma_load_4d(void* dst, const void* desc, uint64_t* bar, int32_t y, int32_t z, int32_t w) {
@@ -51,6 +52,12 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
         "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr)
       : "memory");
+}
+
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
 }
 
 // Zeroes rows [valid, 128) of two tiles that TMA wrote, before MMAs read them;
@@ -77,10 +84,31 @@ struct FastDiv {
   }
 };
 
-// The launch gives each of the 384 threads 168 registers; the elementwise warps
-// take 208 and the first four warps keep 88: 256 * 208 + 128 * 88 = 384 * 168.
-__device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 208;"); }
-__device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 88;"); }
+// Register shares of the warps with the elementwise work and of the others.
+// Forward: 256 * 208 + 128 * 88 = 384 * 168, the launch's.  Backward:
+// 256 * 184 + 256 * 72 = 512 * 128.
+template <int N>
+__device__ __forceinline__ void regs_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+// K-major operand of 16 columns without swizzle: 8 x 16-byte pieces of 128
+// bytes, the two of a row 128 bytes apart, the next 8 rows 256.
+__device__ __forceinline__ uint64_t smem_desc_k16(uint32_t saddr) {
+  return static_cast<uint64_t>((saddr >> 4) & 0x3FFFu) | static_cast<uint64_t>(128u >> 4) << 16 |
+         static_cast<uint64_t>(256u >> 4) << 32 | static_cast<uint64_t>(1u) << 46;
+}
+// x = hi + mid + lo in bf16, 24 bits of it; not finite: hi alone.
+__device__ __forceinline__ void split3(float x, float& hi, float& mid, float& lo) {
+  hi = __bfloat162float(__float2bfloat16_rn(x));
+  const float rest = isfinite(x) ? x - hi : 0.0f;
+  mid = __bfloat162float(__float2bfloat16_rn(rest));
+  lo = rest - mid;
+}
 
 // True in one lane of a converged warp.  The MMA loops run under it: the
 // compiler knows that a single thread is active and keeps the operands in
@@ -213,7 +241,7 @@ constexpr uint32_t F_P = 256, F_O = 384;
 constexpr size_t F_SMEM = 1024 + TILE_B * (4 + 2 * ST) + 512;
 }  // namespace
 
-__global__ void __launch_bounds__(TC_THREADS, 1)
+__global__ void __launch_bounds__(F_THREADS, 1)
     k_attn_forward_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                       const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO, AttnShape a,
                       HeadsView out, float* __restrict__ lse, int items, int per_head, int mixed_from, FastDiv by_head,
@@ -224,8 +252,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   uint8_t* sK = smem + 4 * TILE_B;
   uint8_t* sV = sK + ST * TILE_B;
   uint64_t* bars = reinterpret_cast<uint64_t*>(sV + ST * TILE_B);
-  uint64_t* q_full = bars;             // [2] item parity
-  uint64_t* q_empty = q_full + 2;      // [2 parities][2 tiles]
+  uint64_t* q_full = bars;             // [2 item parities][2 tiles]
+  uint64_t* q_empty = q_full + 4;      // [2 item parities][2 tiles]
   uint64_t* kv_full = q_empty + 4;     // [ST]
   uint64_t* kv_empty = kv_full + ST;   // [ST]
   uint64_t* kv_clean = kv_empty + ST;  // [ST] with lengths: what lies past them is zero
@@ -270,7 +298,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&q_full[i], 1);
+      mbar_init(&q_full[2 * i], 1);
+      mbar_init(&q_full[2 * i + 1], 1);
       mbar_init(&q_empty[2 * i], 4);  // the tile's warps, once their output has left the buffer
       mbar_init(&q_empty[2 * i + 1], 4);
       mbar_init(&s_full[i], 1);
@@ -297,7 +326,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   tc_fence_after();
   constexpr uint32_t tmem = 0;  // all 512 columns are ours: they start at 0
 
-  if (warp < 4) regs_dec();
+  if (warp < 4) regs_dec<88>();
   if (warp == 0) {
     if (elect_one()) {
       uint32_t g = 0, c = 0;                   // blocks, items with work
@@ -317,10 +346,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
           }
         if (!ok) break;
         ++c;
-        mbar_arrive_expect_tx(&q_full[qb], I.tiles * TILE_B);
         const int b0 = by_batch(I.bh[0]), h0 = I.bh[0] - b0 * a.heads, b1 = by_batch(I.bh[1]), h1 = I.bh[1] - b1 * a.heads;
-        tma_load_4d(sQ + qb * 2 * TILE_B, &tmQ, &q_full[qb], I.q0[0], h0, b0);
-        if (I.tiles > 1) tma_load_4d(sQ + (qb * 2 + 1) * TILE_B, &tmQ, &q_full[qb], I.q0[1], h1, b1);
+        mbar_arrive_expect_tx(&q_full[qb * 2], TILE_B);
+        tma_load_4d(sQ + qb * 2 * TILE_B, &tmQ, &q_full[qb * 2], I.q0[0], h0, b0);
+        if (I.tiles > 1) {
+          mbar_arrive_expect_tx(&q_full[qb * 2 + 1], TILE_B);
+          tma_load_4d(sQ + (qb * 2 + 1) * TILE_B, &tmQ, &q_full[qb * 2 + 1], I.q0[1], h1, b1);
+        }
         for (int j = 0; j < I.nb * I.kvs; ++j, ++g) {
           const uint32_t st = g % ST;
           if (!(ok = thread_wait(&kv_empty[st], ((g / ST) & 1) ^ 1, err, VK_DEV_TIMEOUT_PRODUCER))) break;
@@ -333,7 +365,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       }
       if (*reinterpret_cast<volatile int*>(err) != 0) {
         for (uint32_t i = g > ST ? g - ST : 0; i < g; ++i) drain(&kv_full[i % ST], (i / ST) & 1);
-        for (uint32_t i = c > 2 ? c - 2 : 0; i < c; ++i) drain(&q_full[i & 1], (i >> 1) & 1);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (used[i >> 1][i & 1] > 0) drain(&q_full[i], (used[i >> 1][i & 1] - 1) & 1);
       }
     }
   } else if (warp == 1 || (warp == 3 && tpi > 1)) {
@@ -382,10 +416,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
           k = next(k);
         }
       };
-      // S of this tile's n-th block, once its last S has been read (an item's queries come before its keys)
+      // S of this tile's n-th block, once its last S has been read
+      uint32_t uses[2] = {0, 0};  // of the tile's two query buffers
       auto issue_s = [&](const Slot& k, uint32_t n) {
         if (k.it >= items || !wait(&kv_ready[k.g % ST], k.g / ST)) return;
-        if (k.j < k.kvs) wait(&q_full[k.c & 1], k.c >> 1);
+        if (k.j < k.kvs) wait(&q_full[(k.c & 1) * 2 + t], k.c & 1 ? uses[1]++ : uses[0]++);
         if (n > 0) wait(&s_free[t], n - 1);
         if (!ok) return;
         tc_fence_after();
@@ -445,7 +480,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       }
     }
   } else if (warp >= 4) {
-    regs_inc();
+    regs_inc<208>();
     const int t = (warp - 4) >> 2, quad = warp & 3;
     const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
     const uint32_t ts = tmem + t * TR + lanes, tp = tmem + F_P + t * 64 + lanes, to = tmem + F_O + t * 64 + lanes;
@@ -571,18 +606,24 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
 // S and dP are handed back as soon as they are in registers, so the other
 // group's are there before it asks, and one group's exponentials (MUFU, 16 a
 // clock) run beside the other's products and TMEM traffic.
+// dk/dv: the streamed rows' lse and delta belong to columns there, and reading
+// them back from shared memory for every row would take more of its bandwidth
+// than the operands do.  They enter the products instead, as three more
+// columns each (bf16 hi + mid + lo, 24 bits) against ones: S becomes
+// S - lse / scale and dP becomes dP - delta for two more MMAs a block.
 namespace {
 constexpr uint32_t B_MASK = 0x0u;
 constexpr uint32_t COL_DP = 128, COL_P = 256, COL_ACC = 384;
-constexpr size_t B_STATS = ST * 2 * TR * sizeof(float);  // dk/dv: (-lse log2e, delta) of the streamed rows; dq: delta
-constexpr size_t B_SMEM = 1024 + TILE_B * (4 + 2 * ST + 1) + B_STATS + 512;
+constexpr int EXT_B = TR * 32;                // 128 rows of 16 bf16
+constexpr int B_EXTRA = (ST + 2) * EXT_B;     // dk/dv: lse and delta of the streamed blocks, ones; dq: the tile of `out`, delta
+constexpr size_t B_SMEM = 1024 + TILE_B * (4 + 2 * ST) + B_EXTRA + 512;
 }  // namespace
 
 // DQ: own rows are queries (own1 = q, own2 = d_out), streamed ones keys
 // (k, v), acc = dq.  Otherwise own rows are keys (k, v), streamed ones queries
 // (q, d_out), acc = dv, dk.
 template <bool DQ>
-__global__ void __launch_bounds__(TC_THREADS, 1)
+__global__ void __launch_bounds__(B_THREADS, 1)
     k_attn_backward_tc(const __grid_constant__ CUtensorMap tmO1, const __grid_constant__ CUtensorMap tmO2,
                        const __grid_constant__ CUtensorMap tmS1, const __grid_constant__ CUtensorMap tmS2,
                        const __grid_constant__ CUtensorMap tmOut, const __grid_constant__ CUtensorMap tmG1,
@@ -593,9 +634,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   uint8_t* sOwn = smem;  // [item parity][own1, own2], then the item's output on its way out
   uint8_t* s1 = smem + 4 * TILE_B;
   uint8_t* s2 = s1 + ST * TILE_B;
-  uint8_t* sOut = s2 + ST * TILE_B;  // dq: the item's tile of `out`, for delta
-  float* sStat = reinterpret_cast<float*>(sOut + TILE_B);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(sStat) + B_STATS);
+  uint8_t* sExt = s2 + ST * TILE_B;                             // dk/dv: [ST] lse and delta, then the ones of S and of dP
+  uint8_t* sOut = sExt;                                         // dq: the item's tile of `out`, for delta
+  float* sDelta = reinterpret_cast<float*>(sOut + TILE_B);      // dq: [item parity][row]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sExt + B_EXTRA);
   uint64_t* own_full = bars;            // [2] item parity
   uint64_t* own_empty = own_full + 2;   // [2]
   uint64_t* st_full = own_empty + 2;    // [ST]
@@ -604,16 +646,16 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   uint64_t* s_full = st_clean + ST;     // [2] group
   uint64_t* dp_full = s_full + 2;       // [2] group
   uint64_t* ds_full = dp_full + 2;      // [2] group: dS written
-  uint64_t* acc_full = ds_full + 2;     // [2] item parity: the item's last products done
+  uint64_t* p_free = ds_full + 2;       // [2] group, dk/dv: its P used
+  uint64_t* ds_free = p_free + 2;       // [2] group: its dS used
+  uint64_t* acc_full = ds_free + 2;     // [2] item parity: the item's last products done
   uint64_t* part_full = acc_full + 2;   // [2] item parity, dq: delta written, the item's tile of `out` read
   uint64_t* s_free = part_full + 2;     // S read
   uint64_t* dp_free = s_free + 1;       // dP read
   uint64_t* p_full = dp_free + 1;       // dk/dv: P written
-  uint64_t* p_free = p_full + 1;        // dk/dv: P used
-  uint64_t* ds_free = p_free + 1;       // dk/dv: dS used
-  uint64_t* acc_free = ds_free + 1;     // the item's accumulators read
-  uint64_t* stopped = acc_free + 1;     // every product done, after an error
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(stopped + 1);
+  uint64_t* acc_free = p_full + 1;      // the item's accumulators read
+  uint64_t* stopped = acc_free + 1;     // [2] every product of a thread done, after an error
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(stopped + 2);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int total_own = DQ ? a.nq : a.nk;
@@ -648,22 +690,33 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       mbar_init(&s_full[i], 1);
       mbar_init(&dp_full[i], 1);
       mbar_init(&ds_full[i], 4);
+      mbar_init(&p_free[i], 1);
+      mbar_init(&ds_free[i], 1);
       mbar_init(&acc_full[i], 1);
       mbar_init(&part_full[i], 4);
+      mbar_init(&stopped[i], 1);
     }
     mbar_init(s_free, 4);
     mbar_init(dp_free, 4);
     mbar_init(p_full, 4);
-    mbar_init(p_free, 1);
-    mbar_init(ds_free, 1);
     mbar_init(acc_free, 4);
     for (int i = 0; i < ST; ++i) {
       mbar_init(&st_full[i], 1);
       mbar_init(&st_empty[i], 1);
       mbar_init(&st_clean[i], 1);
     }
-    mbar_init(stopped, 1);
     fence_mbar_init();
+  }
+  if constexpr (!DQ) {
+    // 16-byte piece of row r: the first holds the columns that count, the second stays zero
+    for (int i = threadIdx.x; i < (ST + 2) * TR * 2; i += B_THREADS) {
+      const int tile = i / (TR * 2), r = i / 2 % TR, k = i & 1;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (k == 0 && tile == ST) v = make_uint4(0x3f803f80u, 0x00003f80u, 0, 0);          // 1 1 1 0 0 0 0 0
+      if (k == 0 && tile == ST + 1) v = make_uint4(0, 0x3f800000u, 0x3f803f80u, 0);      // 0 0 0 1 1 1 0 0
+      *reinterpret_cast<uint4*>(sExt + tile * EXT_B + (r >> 3) * 256 + k * 128 + (r & 7) * 16) = v;
+    }
+    fence_proxy_async();
   }
   if (warp == 1) {
     tmem_alloc(tmem_slot, 512);
@@ -674,11 +727,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
   tc_fence_after();
   constexpr uint32_t tmem = 0;  // all 512 columns are ours: they start at 0
 
-  if (warp < 4) regs_dec();
+  if (warp < 8) regs_dec<72>();
   if (warp == 0) {
     uint32_t n = 0, c = 0;        // blocks, items
     uint32_t sent = 0, owns = 0;  // how many of them are loaded or on their way
     bool ok = true;
+    const float inv_scale = 1.0f / a.scale;
     for (Item I = seek(blockIdx.x, nothing); ok && I.it < items; I = seek(I.it + gridDim.x, nothing), ++c) {
       const uint32_t ob = c & 1;
       const int b = by_batch(I.bh), h = I.bh - b * a.heads;
@@ -694,23 +748,31 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       for (int j = 0; j < I.nb; ++j, ++n) {
         const uint32_t st = n % ST;
         float l[4], d[4];
-        if constexpr (!DQ) {  // the streamed rows' statistics; a row past the length gets p = 2^-inf = 0
+        if constexpr (!DQ) {
+          // the streamed rows' -lse / scale and -delta.  Rows past the length
+          // are zeros in q and d_out, so their p counts nothing; lse = -inf is
+          // a row of scores of -inf only, whose p is 2^-inf without it too.
           const size_t at = static_cast<size_t>(I.bh) * a.nq;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int row = j * TR + i * 32 + lane;
-            l[i] = row < I.len ? lse[at + row] : INFINITY;
-            d[i] = row < I.len ? delta[at + row] : 0.0f;
+            l[i] = row < I.len ? lse[at + row] : 0.0f;
+            d[i] = row < I.len ? -delta[at + row] : 0.0f;
+            l[i] = l[i] == -INFINITY ? 0.0f : -l[i] * inv_scale;
           }
         }
         if (!(ok = warp_wait(&st_empty[st], ((n / ST) & 1) ^ 1, err, VK_DEV_TIMEOUT_PRODUCER))) break;
         if constexpr (!DQ) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            // lse = -inf: a row of scores of -inf only, whose p is 2^(-inf - 0) = 0
-            sStat[st * 2 * TR + i * 32 + lane] = l[i] == -INFINITY ? 0.0f : -l[i] * LOG2E;
-            sStat[st * 2 * TR + TR + i * 32 + lane] = d[i];
+            const int r = i * 32 + lane;
+            float x[6];
+            split3(l[i], x[0], x[1], x[2]);
+            split3(d[i], x[3], x[4], x[5]);
+            *reinterpret_cast<uint4*>(sExt + st * EXT_B + (r >> 3) * 256 + (r & 7) * 16) =
+                make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), 0u);
           }
+          fence_proxy_async();
           __syncwarp();
         }
         if (lane == 0) {
@@ -725,7 +787,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       for (uint32_t i = sent > ST ? sent - ST : 0; i < sent; ++i) drain(&st_full[i % ST], (i / ST) & 1);
       for (uint32_t i = owns > 2 ? owns - 2 : 0; i < owns; ++i) drain(&own_full[i & 1], (i >> 1) & 1);
     }
-  } else if (warp == 1) {
+  } else if (warp == 1 || warp == 3) {
+    // Two threads issue the MMAs, one S and dP, one the sums: their hand-overs
+    // come in no fixed order.
     if (elect_one()) {
       constexpr uint32_t idS = idesc_bf16(128, 128), idA = idesc_bf16_bmn(128, 64);
       uint64_t* st_ready = (DQ ? a.kv_lens : a.q_lens) != nullptr ? st_clean : st_full;
@@ -745,72 +809,77 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       };
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity) { return ok = ok && thread_wait(bar, parity & 1, err, VK_DEV_TIMEOUT_MMA); };
-      auto ready = [&](const Blk& k, uint32_t n) {  // a block's operands are there
-        if (k.j == 0) wait(&own_full[k.c & 1], k.c >> 1);
-        return wait(&st_ready[n % ST], n / ST);
-      };
-      auto product = [&](uint32_t col, const uint8_t* own, const uint8_t* streamed) {
-        const uint64_t od = smem_desc_k_sw128(smem_u32(own)), sd = smem_desc_k_sw128(smem_u32(streamed));
+      Blk b0 = load(blockIdx.x, 0);
+      if (warp == 1) {
+        auto product = [&](uint32_t col, const uint8_t* own, const uint8_t* streamed, uint32_t st, int ones) {
+          tc_fence_after();
+          const uint64_t od = smem_desc_k_sw128(smem_u32(own)), sd = smem_desc_k_sw128(smem_u32(streamed));
 #pragma unroll
-        for (int k = 0; k < 4; ++k) umma_f16(tmem + col, od + k * 2, sd + k * 2, idS, k > 0 ? 1u : 0u);
-      };
-      auto issue_s = [&](const Blk& k, uint32_t n) {
-        tc_fence_after();
-        product(0, sOwn + (k.c & 1) * 2 * TILE_B, s1 + n % ST * TILE_B);
-        umma_commit(&s_full[n & 1]);
-      };
-      auto issue_dp = [&](const Blk& k, uint32_t n) {
-        tc_fence_after();
-        product(COL_DP, sOwn + ((k.c & 1) * 2 + 1) * TILE_B, s2 + n % ST * TILE_B);
-        umma_commit(&dp_full[n & 1]);
-      };
-      // acc += A . streamed, A = 64 columns of TMEM from `col` on
-      auto sum = [&](uint32_t acc, uint32_t col, const uint8_t* streamed, bool fresh) {
-        tc_fence_after();
-        const uint64_t sd = smem_desc_mn_sw128(smem_u32(streamed));
+          for (int k = 0; k < 4; ++k) umma_f16(tmem + col, od + k * 2, sd + k * 2, idS, k > 0 ? 1u : 0u);
+          if constexpr (!DQ)
+            umma_f16(tmem + col, smem_desc_k16(smem_u32(sExt + (ST + ones) * EXT_B)), smem_desc_k16(smem_u32(sExt + st * EXT_B)),
+                     idS, 1u);
+        };
+        // S of block n, once block n - 1's has been read
+        auto issue_s = [&](const Blk& k, uint32_t n) {
+          if (k.j == 0) wait(&own_full[k.c & 1], k.c >> 1);
+          if (!wait(&st_ready[n % ST], n / ST) || (n > 0 && !wait(s_free, n - 1))) return;
+          product(0, sOwn + (k.c & 1) * 2 * TILE_B, s1 + n % ST * TILE_B, n % ST, 0);
+          umma_commit(&s_full[n & 1]);
+        };
+        auto issue_dp = [&](const Blk& k, uint32_t n) {
+          if (n > 0 && !wait(dp_free, n - 1)) return;
+          product(COL_DP, sOwn + ((k.c & 1) * 2 + 1) * TILE_B, s2 + n % ST * TILE_B, n % ST, 1);
+          umma_commit(&dp_full[n & 1]);
+        };
+        Blk b1 = next(b0), b2 = next(b1);
+        if (b0.ok) {
+          issue_s(b0, 0);
+          if (ok) issue_dp(b0, 0);
+        }
+        if (ok && b1.ok) issue_s(b1, 1);
+        for (uint32_t n = 0; ok && b1.ok; ++n) {
+          // S(n+2) early -- unless its item takes over the tiles of block n's
+          const bool late = b2.c >= b0.c + 2;
+          if (b2.ok && !late) issue_s(b2, n + 2);
+          if (ok) issue_dp(b1, n + 1);
+          if (ok && b2.ok && late) issue_s(b2, n + 2);
+          b0 = b1;
+          b1 = b2;
+          b2 = next(b2);
+        }
+      } else {
+        // acc += A . streamed, A = 64 columns of TMEM from `col` on
+        auto sum = [&](uint32_t acc, uint32_t col, const uint8_t* streamed, bool fresh) {
+          tc_fence_after();
+          const uint64_t sd = smem_desc_mn_sw128(smem_u32(streamed));
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-          umma_f16_ts(tmem + acc, tmem + col + k * 8, sd + static_cast<uint64_t>(k * (2048 >> 4)), idA, fresh && k == 0 ? 0u : 1u);
-      };
-      auto acc_ready = [&](const Blk& k) {  // the last item's accumulators have been read
-        return k.j > 0 || k.c == 0 || wait(acc_free, k.c - 1);
-      };
-      auto next_s = [&](const Blk& k, uint32_t n) {  // S of block n, once block n - 1's has been read
-        if (ready(k, n) && wait(s_free, n - 1)) issue_s(k, n);
-      };
-      Blk b0 = load(blockIdx.x, 0), b1 = next(b0), b2 = next(b1);
-      if (b0.ok && ready(b0, 0)) {
-        issue_s(b0, 0);
-        issue_dp(b0, 0);
-      }
-      if (ok && b1.ok) next_s(b1, 1);
-      for (uint32_t n = 0; ok && b0.ok; ++n) {
-        if constexpr (!DQ) {
-          if (!wait(p_full, n) || !acc_ready(b0)) break;
-          sum(COL_ACC, COL_P, s2 + n % ST * TILE_B, b0.j == 0);  // dv += P^T d_out
-          umma_commit(p_free);
+          for (int k = 0; k < 8; ++k)
+            umma_f16_ts(tmem + acc, tmem + col + k * 8, sd + static_cast<uint64_t>(k * (2048 >> 4)), idA, fresh && k == 0 ? 0u : 1u);
+        };
+        auto acc_ready = [&](const Blk& k) {  // the last item's accumulators have been read
+          return k.j > 0 || k.c == 0 || wait(acc_free, k.c - 1);
+        };
+        for (uint32_t n = 0; b0.ok; ++n) {
+          if constexpr (!DQ) {
+            if (!wait(p_full, n) || !acc_ready(b0)) break;
+            sum(COL_ACC, COL_P, s2 + n % ST * TILE_B, b0.j == 0);  // dv += P^T d_out
+            umma_commit(&p_free[n & 1]);
+          }
+          if (!wait(&ds_full[n & 1], n >> 1) || (DQ && !acc_ready(b0))) break;
+          if constexpr (DQ)
+            sum(COL_ACC, COL_P + (n & 1) * 64, s1 + n % ST * TILE_B, b0.j == 0);  // dq += dS k
+          else
+            sum(COL_ACC + 64, COL_P + 64, s1 + n % ST * TILE_B, b0.j == 0);  // dk += dS^T q
+          umma_commit(&ds_free[n & 1]);
+          umma_commit(&st_empty[n % ST]);
+          if (b0.j + 1 == b0.nb) umma_commit(&acc_full[b0.c & 1]);
+          b0 = next(b0);
         }
-        // S(n+2) early -- unless its item takes over the tiles of block n's
-        const bool late = b2.c >= b0.c + 2;
-        if (b2.ok && !late) next_s(b2, n + 2);
-        if (b1.ok && wait(dp_free, n)) issue_dp(b1, n + 1);
-        if (!wait(&ds_full[n & 1], n >> 1) || (DQ && !acc_ready(b0))) break;
-        if constexpr (DQ) {
-          sum(COL_ACC, COL_P + (n & 1) * 64, s1 + n % ST * TILE_B, b0.j == 0);  // dq += dS k
-        } else {
-          sum(COL_ACC + 64, COL_P + 64, s1 + n % ST * TILE_B, b0.j == 0);  // dk += dS^T q
-          umma_commit(ds_free);
-        }
-        umma_commit(&st_empty[n % ST]);
-        if (b0.j + 1 == b0.nb) umma_commit(&acc_full[b0.c & 1]);
-        if (b2.ok && late) next_s(b2, n + 2);
-        b0 = b1;
-        b1 = b2;
-        b2 = next(b2);
       }
       if (!ok) {
-        umma_commit(stopped);
-        drain(stopped, 0);
+        umma_commit(&stopped[warp >> 1]);
+        drain(&stopped[warp >> 1], 0);
       }
     }
   } else if (warp == 2 && (DQ ? a.kv_lens : a.q_lens) != nullptr) {
@@ -822,18 +891,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         if (I.len - j * TR < TR) zero_tail(s1 + n % ST * TILE_B, s2 + n % ST * TILE_B, I.len - j * TR, lane);
         if (lane == 0) mbar_arrive(&st_clean[n % ST]);
       }
-  } else if (warp >= 4) {
-    regs_inc();
-    const int quad = warp & 3, grp = (warp - 4) >> 2;
+  } else if (warp >= 4 && warp < 8) {
+    const int quad = warp & 3, trow = quad * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
-    const uint32_t ts = tmem + lanes;
-    // dk/dv: P at COL_P, dS 64 columns on; dq: a dS for each group
-    const uint32_t tp = tmem + COL_P + lanes, td = tp + (DQ ? grp * 64 : 64);
-    const float sl2 = a.scale * LOG2E;
-    const int trow = quad * 32 + lane;
     auto skipped = [&](const Item& I) {  // no own rows, or nothing to stream: zeros
       const int row = I.r0 + trow;
-      if (grp != 0 || row >= total_own) return;
+      if (row >= total_own) return;
       const int b = by_batch(I.bh), h = I.bh - b * a.heads;
       store_zeros(static_cast<__nv_bfloat16*>(g1.p) + b * g1.sb + h * g1.sh + row * g1.st);
       if constexpr (DQ)
@@ -841,55 +904,82 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
       else
         store_zeros(static_cast<__nv_bfloat16*>(g2.p) + b * g2.sb + h * g2.sh + row * g2.st);
     };
-    auto own_lse = [&](const Item& I) {
-      const int row = I.r0 + trow;
-      return I.it < items && row < I.own ? lse[static_cast<size_t>(I.bh) * a.nq + row] : 0.0f;
-    };
-    int owed = -1;  // the item whose staged output is still leaving its own tiles
-    auto settle = [&]() {
-      if (owed >= 0 && lane == 0) {
-        bulk_wait_read<0>();
-        mbar_arrive(&own_empty[owed & 1]);
+    // dq: an item's delta from its tiles of out and d_out, a row per thread
+    auto row_delta = [&](const Item& I, uint32_t c) {
+      if (!warp_wait(&own_full[c & 1], (c >> 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE)) return false;
+      const uint8_t* og = sOwn + ((c & 1) * 2 + 1) * TILE_B;
+      float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int at = trow * 128 + ((i ^ trow) & 7) * 16;
+        const uint4 ov = *reinterpret_cast<const uint4*>(sOut + at), gv = *reinterpret_cast<const uint4*>(og + at);
+        const uint32_t o[4] = {ov.x, ov.y, ov.z, ov.w}, g[4] = {gv.x, gv.y, gv.z, gv.w};
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          x[u & 1] = fmaf(__uint_as_float(o[u] << 16), __uint_as_float(g[u] << 16), x[u & 1]);
+          x[2 + (u & 1)] = fmaf(__uint_as_float(o[u] & 0xffff0000u), __uint_as_float(g[u] & 0xffff0000u), x[2 + (u & 1)]);
+        }
       }
-      owed = -1;
+      const float dl = (x[0] + x[1]) + (x[2] + x[3]);
+      sDelta[(c & 1) * TR + trow] = dl;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&part_full[c & 1]);
+      const int row = I.r0 + trow;
+      if (row < total_own) delta[static_cast<size_t>(I.bh) * a.nq + row] = row < I.own ? dl : 0.0f;
+      return true;
     };
-    // An item's accumulators to memory, by the group that had its last block,
-    // staged over its own tiles (every product is done with them).
-    auto finish = [&](const Item& I, uint32_t c) {
-      if (!warp_wait(&acc_full[c & 1], (c >> 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE)) return false;
+    Item I = seek(blockIdx.x, skipped);
+    bool ok = !DQ || I.it >= items || row_delta(I, 0);
+    for (uint32_t c = 0; ok && I.it < items; ++c) {
+      const Item N = seek(I.it + gridDim.x, skipped);
+      if (DQ && N.it < items && !(ok = row_delta(N, c + 1))) break;
+      // the item's accumulators to memory, staged over its own tiles (every product is done with them)
+      if (!(ok = warp_wait(&acc_full[c & 1], (c >> 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
       tc_fence_after();
-      settle();
       const bool live = I.r0 + trow < I.own;
       const int b = by_batch(I.bh), h = I.bh - b * a.heads, y = I.r0 + quad * 32;
       uint8_t* stage = sOwn + (c & 1) * 2 * TILE_B + quad * 4096;
       stage_row(stage, lane, tmem + COL_ACC + lanes, DQ ? a.scale : 1.0f, live);
       if constexpr (!DQ) stage_row(stage + TILE_B, lane, tmem + COL_ACC + 64 + lanes, a.scale, live);
       tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(acc_free);
       send_rows(&tmG1, stage, y, total_own, h, b, lane);
       if constexpr (!DQ) send_rows(&tmG2, stage + TILE_B, y, total_own, h, b, lane);
-      owed = static_cast<int>(c);
-      if (lane == 0) mbar_arrive(acc_free);
-      return true;
+      if (lane == 0) {
+        bulk_wait_read<0>();
+        mbar_arrive(&own_empty[c & 1]);
+      }
+      I = N;
+    }
+    if (lane == 0) bulk_wait<0>();
+  } else if (warp >= 8) {
+    regs_inc<184>();
+    const int quad = warp & 3, grp = (warp - 8) >> 2;
+    const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
+    const uint32_t ts = tmem + lanes;
+    // dk/dv: P at COL_P, dS 64 columns on; dq: a dS for each group
+    const uint32_t tp = tmem + COL_P + lanes, td = tp + (DQ ? grp * 64 : 64);
+    const float sl2 = a.scale * LOG2E;
+    const int trow = quad * 32 + lane;
+    auto own_lse = [&](const Item& I) {
+      const int row = I.r0 + trow;
+      return I.it < items && row < I.own ? lse[static_cast<size_t>(I.bh) * a.nq + row] : 0.0f;
     };
-    Item I = seek(blockIdx.x, skipped);
+    Item I = seek(blockIdx.x, nothing);
     uint32_t n0 = 0, c = 0;  // blocks and items before this one
     bool ok = true;
     float lse_next = DQ ? own_lse(I) : 0.0f;
     while (ok && I.it < items) {
-      const Item N = seek(I.it + gridDim.x, skipped);
-      float2 shift2, delta2 = make_float2(0.0f, 0.0f);
+      const Item N = seek(I.it + gridDim.x, nothing);
+      float2 shift2 = make_float2(0.0f, 0.0f), delta2 = shift2;
       if constexpr (DQ) {
         shift2.x = shift2.y = lse_next == -INFINITY ? 0.0f : -lse_next * LOG2E;
         lse_next = own_lse(N);
       }
       bool fresh = true;  // this group has had no block of the item yet
       for (int j = (n0 ^ grp) & 1; j < I.nb; j += 2) {
-        const uint32_t n = n0 + j, st = n % ST;
-        // (after items of one block, this item's tiles may be the ones still owed)
-        if (owed >= 0 && static_cast<int>(c) >= owed + 2) settle();
-        if constexpr (!DQ) {  // the statistics came with the block
-          if (!(ok = warp_wait(&st_full[st], (n / ST) & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
-        }
+        const uint32_t n = n0 + j;
         if (!(ok = warp_wait(&s_full[grp], (n >> 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
         tc_fence_after();
         float p[128];
@@ -902,60 +992,27 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
           if constexpr (DQ) {
             if (I.len - j * TR < TR) mask_columns(r, I.len - j * TR);
           }
-          const float4* sl = reinterpret_cast<const float4*>(sStat + st * 2 * TR);
 #pragma unroll
           for (int i = 0; i < 64; ++i) {
-            float2 sh = shift2;
-            if constexpr (!DQ) {
-              const float4 v = sl[i / 2];
-              sh = i & 1 ? make_float2(v.z, v.w) : make_float2(v.x, v.y);
-            }
-            const float2 e = exp2_pair<B_MASK>(
-                ffma2(make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), make_float2(sl2, sl2), sh), i);
+            const float2 s = make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), f = make_float2(sl2, sl2);
+            const float2 e = exp2_pair<B_MASK>(DQ ? ffma2(s, f, shift2) : fmul2(s, f), i);
             p[2 * i] = e.x, p[2 * i + 1] = e.y;
           }
         }
-        settle();
         if (DQ && fresh) {
-          // delta, from the tiles of out and d_out, by the group that has the item's first block
-          float* row_delta = sStat + (c & 1) * TR;
-          if (j == 0) {
-            if (!(ok = warp_wait(&own_full[c & 1], (c >> 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
-            const uint8_t* og = sOwn + ((c & 1) * 2 + 1) * TILE_B;
-            float x = 0.0f, y = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int at = trow * 128 + ((i ^ trow) & 7) * 16;
-              const uint4 ov = *reinterpret_cast<const uint4*>(sOut + at), gv = *reinterpret_cast<const uint4*>(og + at);
-              const uint32_t o[4] = {ov.x, ov.y, ov.z, ov.w}, g[4] = {gv.x, gv.y, gv.z, gv.w};
-#pragma unroll
-              for (int u = 0; u < 4; ++u) {
-                x = fmaf(__uint_as_float(o[u] << 16), __uint_as_float(g[u] << 16), x);
-                y = fmaf(__uint_as_float(o[u] & 0xffff0000u), __uint_as_float(g[u] & 0xffff0000u), y);
-              }
-            }
-            delta2.x = x + y;
-            row_delta[trow] = delta2.x;
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&part_full[c & 1]);
-            const int row = I.r0 + trow;
-            if (row < total_own) delta[static_cast<size_t>(I.bh) * a.nq + row] = row < I.own ? delta2.x : 0.0f;
-          } else {
-            if (!(ok = warp_wait(&part_full[c & 1], (c >> 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
-            delta2.x = row_delta[trow];
-          }
-          delta2.y = delta2.x;
+          if (!(ok = warp_wait(&part_full[c & 1], (c >> 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
+          delta2.x = delta2.y = sDelta[(c & 1) * TR + trow];
+          fresh = false;
         }
-        fresh = false;
         if constexpr (!DQ) {
-          if (n > 0 && !(ok = warp_wait(p_free, (n - 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
+          if (n > 0 && !(ok = warp_wait(&p_free[(n - 1) & 1], ((n - 1) >> 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
           tc_fence_after();
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint32_t pk[16];
+          for (int q = 0; q < 8; ++q) {
+            uint32_t pk[8];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) pk[i] = pack_bf16x2(p[q * 32 + 2 * i], p[q * 32 + 2 * i + 1]);
-            tmem_st16(tp + q * 16, pk);
+            for (int i = 0; i < 8; ++i) pk[i] = pack_bf16x2(p[q * 16 + 2 * i], p[q * 16 + 2 * i + 1]);
+            tmem_st8(tp + q * 8, pk);
           }
           tmem_wait_st();
           tc_fence_before();
@@ -963,44 +1020,43 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
           if (lane == 0) mbar_arrive(p_full);
         }
         if (!(ok = warp_wait(&dp_full[grp], (n >> 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
-        // (dq: this group's last dS was used before dP(n) was computed)
-        if (!DQ && n > 0 && !(ok = warp_wait(ds_free, (n - 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
+        if constexpr (DQ) {
+          if (n > 1 && !(ok = warp_wait(&ds_free[grp], ((n >> 1) - 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
+        } else {
+          if (n > 0 && !(ok = warp_wait(&ds_free[(n - 1) & 1], ((n - 1) >> 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
+        }
         tc_fence_after();
+        uint32_t r[2][16];
+        tmem_ld16(ts + COL_DP, r[0]);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          uint32_t r[32], pk[16];
-          tmem_ld32(ts + COL_DP + q * 32, r);
+        for (int q = 0; q < 8; ++q) {
           tmem_wait_ld();
-          if (q == 3) {
+          if (q < 7) tmem_ld16(ts + COL_DP + (q + 1) * 16, r[(q + 1) & 1]);
+          if (q == 7) {
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(dp_free);
           }
-          const float4* sd = reinterpret_cast<const float4*>(sStat + st * 2 * TR + TR + q * 32);
+          const uint32_t(&d)[16] = r[q & 1];
+          uint32_t pk[8];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            float2 dl = delta2;
-            if constexpr (!DQ) {
-              const float4 v = sd[i / 2];
-              dl = i & 1 ? make_float2(v.z, v.w) : make_float2(v.x, v.y);
-            }
-            const float2 ds = fmul2(fsub2(make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), dl),
-                                    make_float2(p[q * 32 + 2 * i], p[q * 32 + 2 * i + 1]));
+          for (int i = 0; i < 8; ++i) {
+            float2 dp = make_float2(__uint_as_float(d[2 * i]), __uint_as_float(d[2 * i + 1]));
+            if constexpr (DQ) dp = fsub2(dp, delta2);
+            const float2 ds = fmul2(dp, make_float2(p[q * 16 + 2 * i], p[q * 16 + 2 * i + 1]));
             pk[i] = pack_bf16x2(ds.x, ds.y);
           }
-          tmem_st16(td + q * 16, pk);
+          tmem_st8(td + q * 8, pk);
         }
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&ds_full[grp]);
-        if (j + 1 == I.nb && !(ok = finish(I, c))) break;
       }
       n0 += I.nb;
       ++c;
       I = N;
     }
-    if (lane == 0) bulk_wait<0>();
   }
   __syncthreads();
   if (warp == 1) {
@@ -1038,7 +1094,7 @@ cudaError_t attention_forward_tc(const AttnShape& a, HeadsView q, HeadsView k, H
     items = mixed_from + (bh + 1) / 2;
   }
   const int grid = items < num_sms() ? items : num_sms();
-  k_attn_forward_tc<<<grid, TC_THREADS, F_SMEM, s>>>(mq, mk, mv, mo, a, out, lse, items, per_head, mixed_from,
+  k_attn_forward_tc<<<grid, F_THREADS, F_SMEM, s>>>(mq, mk, mv, mo, a, out, lse, items, per_head, mixed_from,
                                                      FastDiv(per_head > 0 ? per_head : 1), FastDiv(a.heads), tpi, err);
   return cudaGetLastError();
 }
@@ -1057,11 +1113,11 @@ cudaError_t attention_backward_tc(const AttnShape& a, HeadsView q, HeadsView k, 
   if (e != cudaSuccess) return e;
   const int bh = a.batch * a.heads, sms = num_sms();
   const int qt = (a.nq + TR - 1) / TR, kt = (a.nk + TR - 1) / TR;
-  k_attn_backward_tc<true><<<qt * bh < sms ? qt * bh : sms, TC_THREADS, B_SMEM, s>>>(
+  k_attn_backward_tc<true><<<qt * bh < sms ? qt * bh : sms, B_THREADS, B_SMEM, s>>>(
       mq, mg, mk, mv, mo, mdq, mdq, a, lse, delta, dq, dq, qt * bh, qt, FastDiv(qt), FastDiv(a.heads), err);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  k_attn_backward_tc<false><<<kt * bh < sms ? kt * bh : sms, TC_THREADS, B_SMEM, s>>>(
+  k_attn_backward_tc<false><<<kt * bh < sms ? kt * bh : sms, B_THREADS, B_SMEM, s>>>(
       mk, mv, mq, mg, mo, mdv, mdk, a, lse, delta, dv, dk, kt * bh, kt, FastDiv(kt), FastDiv(a.heads), err);
   return cudaGetLastError();
 }

@@ -594,8 +594,7 @@ __global__ void __launch_bounds__(F_THREADS, 1)
 // ------------------------------------------------------------------ backward
 // Both backward kernels run one pipeline.  A CTA walks its items (tiles of
 // 128 own rows) and the blocks of 128 streamed rows of each as one sequence of
-// blocks n = 0, 1, ...  TMEM: S [0, 128), dP [128, 256), P and dS as bf16
-// [256, 384), accumulators [384, 512).  The two groups of warps take the even
+// blocks n = 0, 1, ...  The two groups of warps take the even
 // and the odd blocks; for each a warp
 //   reads S and hands it back   -> MMA: the next block's S = own1 . streamed1
 //   p = 2^(S scale log2e - lse log2e); dk/dv: writes P
@@ -613,6 +612,8 @@ __global__ void __launch_bounds__(F_THREADS, 1)
 // S - lse / scale and dP becomes dP - delta for two more MMAs a block.
 namespace {
 constexpr uint32_t B_MASK = 0x0u;
+// TMEM: S [0, 128); dq: dP twice [128, 384), dS [384, 448), dq [448, 512);
+// dk/dv: dP [128, 256), P [256, 320), dS [320, 384), dv [384, 448), dk [448, 512)
 constexpr uint32_t COL_DP = 128, COL_P = 256, COL_ACC = 384;
 constexpr int EXT_B = TR * 32;                // 128 rows of 16 bf16
 constexpr int B_EXTRA = (ST + 2) * EXT_B;     // dk/dv: lse and delta of the streamed blocks, ones; dq: the tile of `out`, delta
@@ -650,9 +651,9 @@ __global__ void __launch_bounds__(B_THREADS, 1)
   uint64_t* ds_free = p_free + 2;       // [2] group: its dS used
   uint64_t* acc_full = ds_free + 2;     // [2] item parity: the item's last products done
   uint64_t* part_full = acc_full + 2;   // [2] item parity, dq: delta written, the item's tile of `out` read
-  uint64_t* s_free = part_full + 2;     // S read
-  uint64_t* dp_free = s_free + 1;       // dP read
-  uint64_t* p_full = dp_free + 1;       // dk/dv: P written
+  uint64_t* dp_free = part_full + 2;    // [2] group: dP read
+  uint64_t* s_free = dp_free + 2;       // S read
+  uint64_t* p_full = s_free + 1;       // dk/dv: P written
   uint64_t* acc_free = p_full + 1;      // the item's accumulators read
   uint64_t* stopped = acc_free + 1;     // [2] every product of a thread done, after an error
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(stopped + 2);
@@ -694,10 +695,10 @@ __global__ void __launch_bounds__(B_THREADS, 1)
       mbar_init(&ds_free[i], 1);
       mbar_init(&acc_full[i], 1);
       mbar_init(&part_full[i], 4);
+      mbar_init(&dp_free[i], 4);
       mbar_init(&stopped[i], 1);
     }
     mbar_init(s_free, 4);
-    mbar_init(dp_free, 4);
     mbar_init(p_full, 4);
     mbar_init(acc_free, 4);
     for (int i = 0; i < ST; ++i) {
@@ -828,25 +829,33 @@ __global__ void __launch_bounds__(B_THREADS, 1)
           umma_commit(&s_full[n & 1]);
         };
         auto issue_dp = [&](const Blk& k, uint32_t n) {
-          if (n > 0 && !wait(dp_free, n - 1)) return;
-          product(COL_DP, sOwn + ((k.c & 1) * 2 + 1) * TILE_B, s2 + n % ST * TILE_B, n % ST, 1);
+          // (dq has two of them)
+          if (DQ ? n > 1 && !wait(&dp_free[n & 1], (n >> 1) - 1) : n > 0 && !wait(&dp_free[(n - 1) & 1], (n - 1) >> 1)) return;
+          product(COL_DP + (DQ ? (n & 1) * TR : 0), sOwn + ((k.c & 1) * 2 + 1) * TILE_B, s2 + n % ST * TILE_B, n % ST, 1);
           umma_commit(&dp_full[n & 1]);
         };
-        Blk b1 = next(b0), b2 = next(b1);
-        if (b0.ok) {
-          issue_s(b0, 0);
-          if (ok) issue_dp(b0, 0);
-        }
-        if (ok && b1.ok) issue_s(b1, 1);
-        for (uint32_t n = 0; ok && b1.ok; ++n) {
-          // S(n+2) early -- unless its item takes over the tiles of block n's
-          const bool late = b2.c >= b0.c + 2;
-          if (b2.ok && !late) issue_s(b2, n + 2);
-          if (ok) issue_dp(b1, n + 1);
-          if (ok && b2.ok && late) issue_s(b2, n + 2);
-          b0 = b1;
-          b1 = b2;
-          b2 = next(b2);
+        if constexpr (DQ) {
+          for (uint32_t n = 0; ok && b0.ok; ++n, b0 = next(b0)) {
+            issue_s(b0, n);
+            if (ok) issue_dp(b0, n);
+          }
+        } else {
+          Blk b1 = next(b0), b2 = next(b1);
+          if (b0.ok) {
+            issue_s(b0, 0);
+            if (ok) issue_dp(b0, 0);
+          }
+          if (ok && b1.ok) issue_s(b1, 1);
+          for (uint32_t n = 0; ok && b1.ok; ++n) {
+            // S(n+2) early -- unless its item takes over the tiles of block n's
+            const bool late = b2.c >= b0.c + 2;
+            if (b2.ok && !late) issue_s(b2, n + 2);
+            if (ok) issue_dp(b1, n + 1);
+            if (ok && b2.ok && late) issue_s(b2, n + 2);
+            b0 = b1;
+            b1 = b2;
+            b2 = next(b2);
+          }
         }
       } else {
         // acc += A . streamed, A = 64 columns of TMEM from `col` on
@@ -868,7 +877,7 @@ __global__ void __launch_bounds__(B_THREADS, 1)
           }
           if (!wait(&ds_full[n & 1], n >> 1) || (DQ && !acc_ready(b0))) break;
           if constexpr (DQ)
-            sum(COL_ACC, COL_P + (n & 1) * 64, s1 + n % ST * TILE_B, b0.j == 0);  // dq += dS k
+            sum(COL_ACC + 64, COL_ACC, s1 + n % ST * TILE_B, b0.j == 0);  // dq += dS k
           else
             sum(COL_ACC + 64, COL_P + 64, s1 + n % ST * TILE_B, b0.j == 0);  // dk += dS^T q
           umma_commit(&ds_free[n & 1]);
@@ -939,7 +948,7 @@ __global__ void __launch_bounds__(B_THREADS, 1)
       const bool live = I.r0 + trow < I.own;
       const int b = by_batch(I.bh), h = I.bh - b * a.heads, y = I.r0 + quad * 32;
       uint8_t* stage = sOwn + (c & 1) * 2 * TILE_B + quad * 4096;
-      stage_row(stage, lane, tmem + COL_ACC + lanes, DQ ? a.scale : 1.0f, live);
+      stage_row(stage, lane, tmem + COL_ACC + (DQ ? 64 : 0) + lanes, DQ ? a.scale : 1.0f, live);
       if constexpr (!DQ) stage_row(stage + TILE_B, lane, tmem + COL_ACC + 64 + lanes, a.scale, live);
       tc_fence_before();
       __syncwarp();
@@ -958,8 +967,8 @@ __global__ void __launch_bounds__(B_THREADS, 1)
     const int quad = warp & 3, grp = (warp - 8) >> 2;
     const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
     const uint32_t ts = tmem + lanes;
-    // dk/dv: P at COL_P, dS 64 columns on; dq: a dS for each group
-    const uint32_t tp = tmem + COL_P + lanes, td = tp + (DQ ? grp * 64 : 64);
+    const uint32_t tp = tmem + COL_P + lanes, td = tmem + (DQ ? COL_ACC : COL_P + 64) + lanes;
+    const uint32_t tdp = tmem + COL_DP + (DQ ? grp * TR : 0) + lanes;
     const float sl2 = a.scale * LOG2E;
     const int trow = quad * 32 + lane;
     auto own_lse = [&](const Item& I) {
@@ -1020,22 +1029,17 @@ __global__ void __launch_bounds__(B_THREADS, 1)
           if (lane == 0) mbar_arrive(p_full);
         }
         if (!(ok = warp_wait(&dp_full[grp], (n >> 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
-        if constexpr (DQ) {
-          if (n > 1 && !(ok = warp_wait(&ds_free[grp], ((n >> 1) - 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
-        } else {
-          if (n > 0 && !(ok = warp_wait(&ds_free[(n - 1) & 1], ((n - 1) >> 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
-        }
         tc_fence_after();
         uint32_t r[2][16];
-        tmem_ld16(ts + COL_DP, r[0]);
+        tmem_ld16(tdp, r[0]);
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
           tmem_wait_ld();
-          if (q < 7) tmem_ld16(ts + COL_DP + (q + 1) * 16, r[(q + 1) & 1]);
+          if (q < 7) tmem_ld16(tdp + (q + 1) * 16, r[(q + 1) & 1]);
           if (q == 7) {
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(dp_free);
+            if (lane == 0) mbar_arrive(&dp_free[grp]);
           }
           const uint32_t(&d)[16] = r[q & 1];
           uint32_t pk[8];
@@ -1046,8 +1050,13 @@ __global__ void __launch_bounds__(B_THREADS, 1)
             const float2 ds = fmul2(dp, make_float2(p[q * 16 + 2 * i], p[q * 16 + 2 * i + 1]));
             pk[i] = pack_bf16x2(ds.x, ds.y);
           }
+          if (q == 0 && n > 0) {
+            if (!(ok = warp_wait(&ds_free[(n - 1) & 1], ((n - 1) >> 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
+            tc_fence_after();
+          }
           tmem_st8(td + q * 8, pk);
         }
+        if (!ok) break;
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();

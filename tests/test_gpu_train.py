@@ -209,6 +209,27 @@ def test_attention_scores_that_grow(vk, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("ragged", [False, True])
+def test_attention_scores_far_below_zero(vk, dtype, ragged):
+    """Every score near -100: the columns past the sequence's end (a score of 0 there) must not count."""
+    t = TYPES[dtype]
+    q, k, v, _, _, _, _ = attention_case(t, 2, 2, 140, 300, 64, "head", False, 60)
+    q, k = (q.abs() + 3).to(t), (-k.abs() - 3).to(t)
+    ql, kl = ([140, 100], [201, 90]) if ragged else ([140, 140], [300, 300])
+    qt, kt = (lens(ql), lens(kl)) if ragged else (None, None)
+    want, bound, lse_want, lse_bound = forward_reference(q, k, v, ql, kl, 0.125)
+    out, lse = run_forward(vk, q, k, v, qt, kt)
+    within(out, want, bound, "out")
+    live = lse_want != -math.inf
+    assert lse_want[live].max() < -80
+    within(lse[live], lse_want[live], lse_bound[live], "lse")
+    g = make((2, 2, 140, 64), t, gen(61))
+    grads = run_backward(vk, q, k, v, out, lse, g, qt, kt)
+    for name, x, (w, b) in zip(("dq", "dk", "dv"), grads, backward_reference(q, k, v, out, lse, g, ql, kl, 0.125)):
+        within(x, w, b, name)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_attention_scores_of_minus_infinity(vk, dtype):
     """Keys that score -inf have no weight; NaN stays in its own batch entry and head."""
     q, k, v, ql, kl, _, _ = attention_case(TYPES[dtype], 2, 2, 140, 300, 64, "head", False, 6)

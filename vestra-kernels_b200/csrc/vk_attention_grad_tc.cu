@@ -34,6 +34,7 @@ namespace {
 constexpr int TR = 128;                 // rows of a tile, columns of a block
 constexpr int TILE_B = TR * 128;        // bytes of 128 rows of 64 bf16
 constexpr int ST = 4;                   // streamed blocks in flight
+constexpr int EXT_B = TR * 32;          // bytes of 128 rows of 16 bf16
 constexpr int F_THREADS = 12 * 32, B_THREADS = 16 * 32;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
@@ -101,6 +102,10 @@ __device__ __forceinline__ void regs_dec() {
 __device__ __forceinline__ uint64_t smem_desc_k16(uint32_t saddr) {
   return static_cast<uint64_t>((saddr >> 4) & 0x3FFFu) | static_cast<uint64_t>(128u >> 4) << 16 |
          static_cast<uint64_t>(256u >> 4) << 32 | static_cast<uint64_t>(1u) << 46;
+}
+// Piece k of row r of such a tile.
+__device__ __forceinline__ uint4* ext_piece(uint8_t* s, int r, int k) {
+  return reinterpret_cast<uint4*>(s + (r >> 3) * 256 + k * 128 + (r & 7) * 16);
 }
 // x = hi + mid + lo in bf16, 24 bits of it; not finite: hi alone.
 __device__ __forceinline__ void split3(float x, float& hi, float& mid, float& lo) {
@@ -206,11 +211,9 @@ __device__ __forceinline__ void tmem_ld128(uint32_t taddr, uint32_t (&r)[128]) {
 // Where they are all -inf any finite one will do: it keeps 2^(-inf) at 0.
 __device__ __forceinline__ float finite_ref(float top) { return top == -INFINITY ? -1e30f : top; }
 
-// Scores of columns from `valid` on become -inf.  The empty statement keeps
-// this a branch of the rare last block: as selects it would cost every block
-// two instructions a column.
+// Scores of columns from `valid` on become -inf.
 __device__ __forceinline__ void mask_columns(uint32_t (&r)[128], int valid) {
-  asm volatile("" ::: "memory");
+  asm volatile("" ::: "memory");  // (a branch, not selects in every block)
 #pragma unroll
   for (int i = 0; i < 128; ++i)
     if (i >= valid) r[i] = 0xff800000u;
@@ -233,12 +236,16 @@ __device__ __forceinline__ float2 exp2_pair(float2 x, int i) {
 // [128, 256), P as bf16 [256, 320) and [320, 384), O [384, 448) and [448, 512).
 // S is handed back as soon as it is in registers, so that the next block's is
 // there when the warps ask for it: they are bound by their exponentials.
+//
+// The columns past a sequence's end get their -inf from the tensor core: one
+// more MMA in the last block, a column of ones against a column of 0 and -inf.
+// (As selects in the warps it took as long as the block's exponentials.)
 namespace {
 // Pairs of columns (of each 16) whose exponentials go to the FMA pipe:
 // measured at 64 images, 298 us for none, 293 for 4, 309 for 6.
 constexpr uint32_t F_MASK = 0x1111u;
 constexpr uint32_t F_P = 256, F_O = 384;
-constexpr size_t F_SMEM = 1024 + TILE_B * (4 + 2 * ST) + 512;
+constexpr size_t F_SMEM = 1024 + TILE_B * (4 + 2 * ST) + (ST + 1) * EXT_B + 512;
 }  // namespace
 
 __global__ void __launch_bounds__(F_THREADS, 1)
@@ -251,7 +258,8 @@ __global__ void __launch_bounds__(F_THREADS, 1)
   uint8_t* sQ = smem;  // [item parity][tile], then the tile's output on its way out
   uint8_t* sK = smem + 4 * TILE_B;
   uint8_t* sV = sK + ST * TILE_B;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sV + ST * TILE_B);
+  uint8_t* sMask = sV + ST * TILE_B;  // [ST] the keys' column of 0 and -inf (without lengths the first serves all), then the ones
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sMask + (ST + 1) * EXT_B);
   uint64_t* q_full = bars;             // [2 item parities][2 tiles]
   uint64_t* q_empty = q_full + 4;      // [2 item parities][2 tiles]
   uint64_t* kv_full = q_empty + 4;     // [ST]
@@ -317,6 +325,14 @@ __global__ void __launch_bounds__(F_THREADS, 1)
     mbar_init(&stopped[1], 1);
     fence_mbar_init();
   }
+  for (int i = threadIdx.x; i < (ST + 1) * TR * 2; i += F_THREADS) {
+    const int tile = i / (TR * 2), r = i / 2 % TR;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if ((i & 1) == 0 && tile == ST) v.x = 0x3f80u;                                                      // 1
+    if ((i & 1) == 0 && tile == 0 && a.kv_lens == nullptr && r >= (a.nk - 1) % TR + 1) v.x = 0xff80u;   // -inf
+    *ext_piece(sMask + tile * EXT_B, r, i & 1) = v;
+  }
+  fence_proxy_async();
   if (warp == 1) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
@@ -383,7 +399,7 @@ __global__ void __launch_bounds__(F_THREADS, 1)
       struct Slot {
         int it, tiles, kvs, j, nb;
         uint32_t c, g;  // ordinals of the item and of the slot
-        bool mine;
+        bool mine, ragged;  // ragged: the sequence's last block is not full
       };
       auto load = [&](Slot k) {
         for (; k.it < items; k.it += gridDim.x) {
@@ -391,6 +407,7 @@ __global__ void __launch_bounds__(F_THREADS, 1)
           k.tiles = I.tiles;
           k.kvs = I.kvs;
           k.nb = I.nb * I.kvs;
+          k.ragged = I.nk % TR != 0;
           if (I.tiles > 0) break;
         }
         k.j = 0;
@@ -428,9 +445,12 @@ __global__ void __launch_bounds__(F_THREADS, 1)
         const uint64_t kd = smem_desc_k_sw128(smem_u32(sK + k.g % ST * TILE_B));
 #pragma unroll
         for (int i = 0; i < 4; ++i) umma_f16(tmem + t * TR, qd + i * 2, kd + i * 2, idS, i > 0 ? 1u : 0u);
+        if (k.ragged && k.j + k.kvs >= k.nb)
+          umma_f16(tmem + t * TR, smem_desc_k16(smem_u32(sMask + ST * EXT_B)),
+                   smem_desc_k16(smem_u32(sMask + (a.kv_lens != nullptr ? k.g % ST : 0) * EXT_B)), idS, 1u);
         umma_commit(&s_full[t]);
       };
-      Slot k = load(Slot{static_cast<int>(blockIdx.x), 0, 1, 0, 0, 0, 0, false});
+      Slot k = load(Slot{static_cast<int>(blockIdx.x), 0, 1, 0, 0, 0, 0, false, false});
       // Tile 1 starts when tile 0 is about to take its exponentials: half a
       // block apart, the two share MUFU in turn (in step they took 3600 cycles
       // for a block of both, 2048 of them MUFU's).
@@ -475,7 +495,12 @@ __global__ void __launch_bounds__(F_THREADS, 1)
       if (I.tiles == 0) continue;
       for (int j = 0; j < I.nb; ++j, ++g) {  // (with lengths, an item streams one sequence)
         if (!(ok = warp_wait(&kv_full[g % ST], (g / ST) & 1, err, VK_DEV_TIMEOUT_OTHER))) break;
-        if (I.nk - j * TR < TR) zero_tail(sK + g % ST * TILE_B, sV + g % ST * TILE_B, I.nk - j * TR, lane);
+        const int valid = I.nk - j * TR;
+        if (valid < TR) {
+          for (int r = lane; r < TR; r += 32)
+            *ext_piece(sMask + g % ST * EXT_B, r, 0) = make_uint4(r < valid ? 0u : 0xff80u, 0, 0, 0);
+          zero_tail(sK + g % ST * TILE_B, sV + g % ST * TILE_B, valid, lane);
+        }
         if (lane == 0) mbar_arrive(&kv_clean[g % ST]);
       }
     }
@@ -518,7 +543,6 @@ __global__ void __launch_bounds__(F_THREADS, 1)
         uint32_t r[128];
         tmem_ld128(ts, r);
         tc_fence_before();
-        if (I.nk - j * TR < TR) mask_columns(r, I.nk - j * TR);
         float pm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int i = 0; i < 128; i += 2)
@@ -615,7 +639,6 @@ constexpr uint32_t B_MASK = 0x0u;
 // TMEM: S [0, 128); dq: dP twice [128, 384), dS [384, 448), dq [448, 512);
 // dk/dv: dP [128, 256), P [256, 320), dS [320, 384), dv [384, 448), dk [448, 512)
 constexpr uint32_t COL_DP = 128, COL_P = 256, COL_ACC = 384;
-constexpr int EXT_B = TR * 32;                // 128 rows of 16 bf16
 constexpr int B_EXTRA = (ST + 2) * EXT_B;     // dk/dv: lse and delta of the streamed blocks, ones; dq: the tile of `out`, delta
 constexpr size_t B_SMEM = 1024 + TILE_B * (4 + 2 * ST) + B_EXTRA + 512;
 }  // namespace
@@ -715,7 +738,7 @@ __global__ void __launch_bounds__(B_THREADS, 1)
       uint4 v = make_uint4(0, 0, 0, 0);
       if (k == 0 && tile == ST) v = make_uint4(0x3f803f80u, 0x00003f80u, 0, 0);          // 1 1 1 0 0 0 0 0
       if (k == 0 && tile == ST + 1) v = make_uint4(0, 0x3f800000u, 0x3f803f80u, 0);      // 0 0 0 1 1 1 0 0
-      *reinterpret_cast<uint4*>(sExt + tile * EXT_B + (r >> 3) * 256 + k * 128 + (r & 7) * 16) = v;
+      *ext_piece(sExt + tile * EXT_B, r, k) = v;
     }
     fence_proxy_async();
   }
@@ -770,7 +793,7 @@ __global__ void __launch_bounds__(B_THREADS, 1)
             float x[6];
             split3(l[i], x[0], x[1], x[2]);
             split3(d[i], x[3], x[4], x[5]);
-            *reinterpret_cast<uint4*>(sExt + st * EXT_B + (r >> 3) * 256 + (r & 7) * 16) =
+            *ext_piece(sExt + st * EXT_B, r, 0) =
                 make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), 0u);
           }
           fence_proxy_async();
@@ -999,7 +1022,10 @@ __global__ void __launch_bounds__(B_THREADS, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive(s_free);
           if constexpr (DQ) {
-            if (I.len - j * TR < TR) mask_columns(r, I.len - j * TR);
+            // Keys past the end are zero rows of k: whatever finite dS a
+            // score of 0 gives there counts nothing.  It stays finite unless
+            // the row's lse is far below 0.
+            if (I.len - j * TR < TR && __any_sync(0xffffffffu, !(shift2.x < 60.0f))) mask_columns(r, I.len - j * TR);
           }
 #pragma unroll
           for (int i = 0; i < 64; ++i) {

@@ -660,7 +660,7 @@ __global__ void __launch_bounds__(B_THREADS, 1)
   uint8_t* s2 = s1 + ST * TILE_B;
   uint8_t* sExt = s2 + ST * TILE_B;                             // dk/dv: [ST] lse and delta, then the ones of S and of dP
   uint8_t* sOut = sExt;                                         // dq: the item's tile of `out`, for delta
-  float* sDelta = reinterpret_cast<float*>(sOut + TILE_B);      // dq: [item parity][row]
+  float2* sRow = reinterpret_cast<float2*>(sOut + TILE_B);      // dq: [item parity][row] (-lse log2e, delta)
   uint64_t* bars = reinterpret_cast<uint64_t*>(sExt + B_EXTRA);
   uint64_t* own_full = bars;            // [2] item parity
   uint64_t* own_empty = own_full + 2;   // [2]
@@ -936,8 +936,12 @@ __global__ void __launch_bounds__(B_THREADS, 1)
       else
         store_zeros(static_cast<__nv_bfloat16*>(g2.p) + b * g2.sb + h * g2.sh + row * g2.st);
     };
-    // dq: an item's delta from its tiles of out and d_out, a row per thread
+    // dq: the rows' -lse log2e and delta (from the tiles of out and d_out), a
+    // row per thread, an item ahead of the warps that use them
     auto row_delta = [&](const Item& I, uint32_t c) {
+      const int row = I.r0 + trow;
+      const size_t at = static_cast<size_t>(I.bh) * a.nq + row;
+      const float e = row < I.own ? lse[at] : 0.0f;
       if (!warp_wait(&own_full[c & 1], (c >> 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE)) return false;
       const uint8_t* og = sOwn + ((c & 1) * 2 + 1) * TILE_B;
       float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -953,11 +957,11 @@ __global__ void __launch_bounds__(B_THREADS, 1)
         }
       }
       const float dl = (x[0] + x[1]) + (x[2] + x[3]);
-      sDelta[(c & 1) * TR + trow] = dl;
+      // lse = -inf: a row of scores of -inf only, whose p is 2^(-inf - 0) = 0
+      sRow[(c & 1) * TR + trow] = make_float2(e == -INFINITY ? 0.0f : -e * LOG2E, dl);
       __syncwarp();
       if (lane == 0) mbar_arrive(&part_full[c & 1]);
-      const int row = I.r0 + trow;
-      if (row < total_own) delta[static_cast<size_t>(I.bh) * a.nq + row] = row < I.own ? dl : 0.0f;
+      if (row < total_own) delta[at] = row < I.own ? dl : 0.0f;
       return true;
     };
     Item I = seek(blockIdx.x, skipped);
@@ -994,24 +998,21 @@ __global__ void __launch_bounds__(B_THREADS, 1)
     const uint32_t tdp = tmem + COL_DP + (DQ ? grp * TR : 0) + lanes;
     const float sl2 = a.scale * LOG2E;
     const int trow = quad * 32 + lane;
-    auto own_lse = [&](const Item& I) {
-      const int row = I.r0 + trow;
-      return I.it < items && row < I.own ? lse[static_cast<size_t>(I.bh) * a.nq + row] : 0.0f;
-    };
     Item I = seek(blockIdx.x, nothing);
     uint32_t n0 = 0, c = 0;  // blocks and items before this one
     bool ok = true;
-    float lse_next = DQ ? own_lse(I) : 0.0f;
-    while (ok && I.it < items) {
-      const Item N = seek(I.it + gridDim.x, nothing);
+    for (; ok && I.it < items; n0 += I.nb, ++c, I = seek(I.it + gridDim.x, nothing)) {
       float2 shift2 = make_float2(0.0f, 0.0f), delta2 = shift2;
-      if constexpr (DQ) {
-        shift2.x = shift2.y = lse_next == -INFINITY ? 0.0f : -lse_next * LOG2E;
-        lse_next = own_lse(N);
-      }
       bool fresh = true;  // this group has had no block of the item yet
       for (int j = (n0 ^ grp) & 1; j < I.nb; j += 2) {
         const uint32_t n = n0 + j;
+        if (DQ && fresh) {
+          if (!(ok = warp_wait(&part_full[c & 1], (c >> 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
+          const float2 x = sRow[(c & 1) * TR + trow];
+          shift2 = make_float2(x.x, x.x);
+          delta2 = make_float2(x.y, x.y);
+          fresh = false;
+        }
         if (!(ok = warp_wait(&s_full[grp], (n >> 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
         tc_fence_after();
         float p[128];
@@ -1033,11 +1034,6 @@ __global__ void __launch_bounds__(B_THREADS, 1)
             const float2 e = exp2_pair<B_MASK>(DQ ? ffma2(s, f, shift2) : fmul2(s, f), i);
             p[2 * i] = e.x, p[2 * i + 1] = e.y;
           }
-        }
-        if (DQ && fresh) {
-          if (!(ok = warp_wait(&part_full[c & 1], (c >> 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
-          delta2.x = delta2.y = sDelta[(c & 1) * TR + trow];
-          fresh = false;
         }
         if constexpr (!DQ) {
           if (n > 0 && !(ok = warp_wait(&p_free[(n - 1) & 1], ((n - 1) >> 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
@@ -1088,9 +1084,6 @@ __global__ void __launch_bounds__(B_THREADS, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&ds_full[grp]);
       }
-      n0 += I.nb;
-      ++c;
-      I = N;
     }
   }
   __syncthreads();

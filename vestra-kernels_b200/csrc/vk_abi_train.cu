@@ -237,8 +237,8 @@ extern "C" int vk_rope_axes(vk_ctx* ctx, const vk_rope_axes_shape* shape, const 
     }
     p.rotated = static_cast<int>(at);
     if (r.batch == 0 || r.heads == 0 || r.tokens == 0) return VK_OK;
-    // four tokens of all heads are counted in an int, and so are the blocks
-    if (r.heads > static_cast<size_t>(INT_MAX) / 1024 || r.batch > static_cast<size_t>(INT_MAX) / (r.tokens / 4 + 1))
+    // the pieces of all tokens are counted in an int, and so are the heads' splits in a grid dimension
+    if (r.heads > 65535 * 4 || r.batch > static_cast<size_t>(INT_MAX) / (2 * ROPE_MAX_PAIRS) / r.tokens)
       return vk_fail(VK_UNSUPPORTED_SHAPE, "%s: too many heads or tokens", name);
     if (positions == nullptr || reinterpret_cast<uintptr_t>(positions) % 8 != 0)
       return vk_fail(VK_ERR_INVALID_ARGUMENT, "%s: positions are NULL or not aligned", name);

@@ -72,19 +72,6 @@ __device__ __forceinline__ void zero_tail(uint8_t* a, uint8_t* b, int valid, int
   __syncwarp();
 }
 
-// Division of n < 2^31 by a constant: a few instructions where the general
-// one takes a hundred, at every item.
-struct FastDiv {
-  uint32_t mul, shift;
-  FastDiv(uint32_t d) : mul(0), shift(0) {
-    while ((uint64_t{1} << shift) < d) ++shift;
-    mul = static_cast<uint32_t>((((uint64_t{1} << shift) - d) << 32) / d + 1);
-  }
-  __device__ __forceinline__ int operator()(int n) const {
-    return static_cast<int>((__umulhi(static_cast<uint32_t>(n), mul) + static_cast<uint32_t>(n)) >> shift);
-  }
-};
-
 // Register shares of the warps with the elementwise work and of the others.
 // Forward: 256 * 208 + 128 * 88 = 384 * 168, the launch's.  Backward:
 // 256 * 184 + 256 * 72 = 512 * 128.

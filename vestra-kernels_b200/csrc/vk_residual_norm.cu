@@ -7,13 +7,19 @@
 //   column sums: d_gamma = sum d_y y^, d_beta = sum d_y, P = sum dh n per
 //   group (d_scale = sum_groups gate P, d_gate = scale P), and the post norm's.
 // Both are HBM-bound: at 768 columns, f32 stream and bf16 branch, 9.2 KB a row
-// forward and 13.8 KB backward.  Rows live in registers; sums are f32.
+// forward and 13.8 KB backward.  Rows live in registers; sums are f32.  What
+// holds them back is the load and store path (three quarters busy when the
+// vectors of a row were read as 16-byte halves) and the wait for a row, so
+// eight f32 move at once and the next row is fetched while this one is worked
+// on.  55,360 rows of that kind: forward 134 us with neither, 125 with the
+// fetch, 105 with both (4.9 TB/s); backward 176, 156, 146 (5.2 TB/s).
 //
 // The column sums are split over blocks that own consecutive rows of one
 // group and join in a second small kernel in a fixed order: no atomics, the
 // same bits every time.
 #include <cuda_bf16.h>
 
+#include <algorithm>
 #include <initializer_list>
 
 #include "vk_common.cuh"
@@ -24,6 +30,9 @@ namespace vk {
 
 namespace {
 constexpr int RN_BLOCK = 256;
+// Values a thread may have of a row for the next row to be fetched while this
+// one is worked on: above it the registers run out.
+constexpr int RN_AHEAD = 24;
 
 __device__ __forceinline__ float warp_total(float v) {
 #pragma unroll
@@ -31,35 +40,53 @@ __device__ __forceinline__ float warp_total(float v) {
   return v;
 }
 
-// VEC (8 or 1) consecutive values.
+// VEC (8 or 1) consecutive values as they lie in memory.  Eight f32 go as one
+// 32-byte access: as two of 16, each would use half of the lines it touches.
+template <class T, int VEC>
+struct Lanes {
+  static constexpr int WORDS = VEC * sizeof(T) >= 4 ? VEC * sizeof(T) / 4 : 1;
+  uint32_t w[WORDS];
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (WORDS == 8) {
+      asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                   : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                   : "l"(__cvta_generic_to_global(p)));
+    } else if constexpr (WORDS == 4) {
+      const uint4 u = *reinterpret_cast<const uint4*>(p);
+      w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+    } else if constexpr (sizeof(T) == 4) {
+      w[0] = __float_as_uint(*reinterpret_cast<const float*>(p));
+    } else {
+      w[0] = *reinterpret_cast<const uint16_t*>(p);
+    }
+  }
+  __device__ __forceinline__ void get(float (&d)[VEC]) const {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) d[i] = __uint_as_float(w[i]);
+    } else if constexpr (VEC == 8) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        d[2 * i] = __uint_as_float(w[i] << 16);
+        d[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      }
+    } else {
+      d[0] = __uint_as_float(w[0] << 16);
+    }
+  }
+};
 template <int VEC>
 __device__ __forceinline__ void get(float (&d)[VEC], const float* p) {
-  if constexpr (VEC == 8) {
-    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-    d[0] = a.x, d[1] = a.y, d[2] = a.z, d[3] = a.w, d[4] = b.x, d[5] = b.y, d[6] = b.z, d[7] = b.w;
-  } else {
-    d[0] = *p;
-  }
-}
-template <int VEC>
-__device__ __forceinline__ void get(float (&d)[VEC], const __nv_bfloat16* p) {
-  if constexpr (VEC == 8) {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      d[2 * i] = __uint_as_float(w[i] << 16);
-      d[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
-  } else {
-    d[0] = __bfloat162float(*p);
-  }
+  Lanes<float, VEC> l;
+  l.load(p);
+  l.get(d);
 }
 template <int VEC>
 __device__ __forceinline__ void put(float* p, const float (&d)[VEC]) {
   if constexpr (VEC == 8) {
-    *reinterpret_cast<float4*>(p) = make_float4(d[0], d[1], d[2], d[3]);
-    *reinterpret_cast<float4*>(p + 4) = make_float4(d[4], d[5], d[6], d[7]);
+    asm volatile("st.global.v8.f32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::"f"(d[0]), "f"(d[1]), "f"(d[2]), "f"(d[3]),
+                 "f"(d[4]), "f"(d[5]), "f"(d[6]), "f"(d[7]), "l"(__cvta_generic_to_global(p))
+                 : "memory");
   } else {
     *p = d[0];
   }
@@ -79,13 +106,12 @@ __device__ __forceinline__ void put(__nv_bfloat16* p, const float (&d)[VEC]) {
 // per thread.
 template <class XT, class BT, int VEC, int T, int NV>
 __global__ void __launch_bounds__(RN_BLOCK)
-    k_residual_norm(ResidualNorm r, int rows, const XT* x, const BT* __restrict__ branch, XT* h, BT* y,
+    k_residual_norm(ResidualNorm r, unsigned rows, FastDiv by_group, const XT* x, const BT* __restrict__ branch, XT* h, BT* y,
                     float* __restrict__ stats, float* __restrict__ post_stats) {
   constexpr int ROWS = RN_BLOCK / T, WARPS = T / 32;
+  constexpr bool AHEAD = VEC * NV <= RN_AHEAD;
   __shared__ float part[4][RN_BLOCK / 32];
   const int in_row = threadIdx.x % T, slot = threadIdx.x / T;
-  const int row = blockIdx.x * ROWS + slot;
-  const bool live = row < rows;
   // sum over the T threads of a row; `which` names a slot of its own per call
   auto row_total = [&](float v, int which) {
     v = warp_total(v);
@@ -98,81 +124,101 @@ __global__ void __launch_bounds__(RN_BLOCK)
     return s;
   };
   const float inv_cols = 1.0f / static_cast<float>(r.cols);
-  const size_t base = static_cast<size_t>(live ? row : 0) * r.cols;
-  const float* gate = r.gate != nullptr && live ? r.gate + static_cast<size_t>(row / r.rows_per_group) * r.cols : nullptr;
-  float n[NV][VEC], v[NV][VEC];
-  bool has[NV];
+  Lanes<XT, VEC> raw_x[NV];
+  Lanes<BT, VEC> raw_b[NV];
   int col[NV];
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    col[j] = (j * T + in_row) * VEC;
-    has[j] = live && col[j] < r.cols;
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) n[j][e] = v[j][e] = 0.0f;
-    if (has[j]) {
-      get<VEC>(n[j], branch + base + col[j]);
-      get<VEC>(v[j], x + base + col[j]);
-    }
-  }
-  auto mean_rstd = [&](float (&u)[NV][VEC], int which) {
-    float s = 0.0f;
+  for (int j = 0; j < NV; ++j) col[j] = (j * T + in_row) * VEC;
+  auto fetch = [&](unsigned row) {
 #pragma unroll
     for (int j = 0; j < NV; ++j)
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) s += u[j][e];
-    const float mean = row_total(s, which) * inv_cols;
-    float q = 0.0f;
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-      if (has[j])
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) q = fmaf(u[j][e] - mean, u[j][e] - mean, q);
-    const float var = row_total(q, which + 1) * inv_cols;
-    return make_float2(mean, 1.0f / sqrtf(var + r.eps));
+      if (row < rows && col[j] < r.cols) {
+        raw_b[j].load(branch + static_cast<size_t>(row) * r.cols + col[j]);
+        raw_x[j].load(x + static_cast<size_t>(row) * r.cols + col[j]);
+      }
   };
-  if (r.post_gamma != nullptr) {
-    const float2 mr = mean_rstd(n, 0);
-    if (live && in_row == 0) *reinterpret_cast<float2*>(post_stats + 2 * static_cast<size_t>(row)) = mr;
+  if (AHEAD) fetch(blockIdx.x * ROWS + slot);
+  // (the rows of a block go in step: its sums meet in shared memory)
+  for (unsigned row0 = blockIdx.x * ROWS; row0 < rows; row0 += gridDim.x * ROWS) {
+    const unsigned row = row0 + slot;
+    if (!AHEAD) fetch(row);
+    const bool live = row < rows;
+    const size_t base = static_cast<size_t>(live ? row : 0) * r.cols;
+    const float* gate = r.gate != nullptr && live ? r.gate + static_cast<size_t>(by_group(row)) * r.cols : nullptr;
+    float n[NV][VEC], v[NV][VEC];
+    bool has[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      has[j] = live && col[j] < r.cols;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) n[j][e] = v[j][e] = 0.0f;
+      if (has[j]) {
+        raw_b[j].get(n[j]);
+        raw_x[j].get(v[j]);
+      }
+    }
+    if (AHEAD) fetch(row + gridDim.x * ROWS);
+    auto mean_rstd = [&](float (&u)[NV][VEC], int which) {
+      float s = 0.0f;
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) s += u[j][e];
+      const float mean = row_total(s, which) * inv_cols;
+      float q = 0.0f;
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        if (has[j])
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) q = fmaf(u[j][e] - mean, u[j][e] - mean, q);
+      const float var = row_total(q, which + 1) * inv_cols;
+      return make_float2(mean, 1.0f / sqrtf(var + r.eps));
+    };
+    if (r.post_gamma != nullptr) {
+      const float2 mr = mean_rstd(n, 0);
+      if (live && in_row == 0) *reinterpret_cast<float2*>(post_stats + 2 * static_cast<size_t>(row)) = mr;
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        if (has[j]) {
+          float g[VEC], b[VEC];
+          get<VEC>(g, r.post_gamma + col[j]);
+          get<VEC>(b, r.post_beta + col[j]);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) n[j][e] = fmaf((n[j][e] - mr.x) * mr.y, g[e], b[e]);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+      if (has[j]) {
+        float f[VEC];
+        if (r.scale != nullptr) {
+          get<VEC>(f, r.scale + col[j]);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) n[j][e] *= f[e];
+        }
+        if (gate != nullptr) {
+          get<VEC>(f, gate + col[j]);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) n[j][e] *= f[e];
+        }
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[j][e] += n[j][e];
+        put<VEC>(h + base + col[j], v[j]);
+      }
+    const float2 mr = mean_rstd(v, 2);
+    if (live && in_row == 0) *reinterpret_cast<float2*>(stats + 2 * static_cast<size_t>(row)) = mr;
 #pragma unroll
     for (int j = 0; j < NV; ++j)
       if (has[j]) {
         float g[VEC], b[VEC];
-        get<VEC>(g, r.post_gamma + col[j]);
-        get<VEC>(b, r.post_beta + col[j]);
+        get<VEC>(g, r.gamma + col[j]);
+        get<VEC>(b, r.beta + col[j]);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) n[j][e] = fmaf((n[j][e] - mr.x) * mr.y, g[e], b[e]);
+        for (int e = 0; e < VEC; ++e) v[j][e] = fmaf((v[j][e] - mr.x) * mr.y, g[e], b[e]);
+        put<VEC>(y + base + col[j], v[j]);
       }
+    if constexpr (WARPS > 1) __syncthreads();  // before the next row's sums
   }
-#pragma unroll
-  for (int j = 0; j < NV; ++j)
-    if (has[j]) {
-      float f[VEC];
-      if (r.scale != nullptr) {
-        get<VEC>(f, r.scale + col[j]);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) n[j][e] *= f[e];
-      }
-      if (gate != nullptr) {
-        get<VEC>(f, gate + col[j]);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) n[j][e] *= f[e];
-      }
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) v[j][e] += n[j][e];
-      put<VEC>(h + base + col[j], v[j]);
-    }
-  const float2 mr = mean_rstd(v, 2);
-  if (live && in_row == 0) *reinterpret_cast<float2*>(stats + 2 * static_cast<size_t>(row)) = mr;
-#pragma unroll
-  for (int j = 0; j < NV; ++j)
-    if (has[j]) {
-      float g[VEC], b[VEC];
-      get<VEC>(g, r.gamma + col[j]);
-      get<VEC>(b, r.beta + col[j]);
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) v[j][e] = fmaf((v[j][e] - mr.x) * mr.y, g[e], b[e]);
-      put<VEC>(y + base + col[j], v[j]);
-    }
 }
 
 namespace {
@@ -266,9 +312,29 @@ __global__ void __launch_bounds__(RN_BLOCK)
       }
     }
   }
-  for (int i = 0; i < nrows; ++i) {
+  Lanes<BT, VEC> raw_t[NV], raw_n[NV];
+  Lanes<XT, VEC> raw_h[NV], raw_d[NV];
+  float2 mr_next = make_float2(0.0f, 0.0f), pr_next = mr_next;
+  auto fetch = [&](int i) {
+    if (i >= nrows) return;
     const size_t row = static_cast<size_t>(first + i), base = row * r.cols;
-    const float2 mr = *reinterpret_cast<const float2*>(stats + 2 * row);
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+      if (has[j]) {
+        raw_t[j].load(d_y + base + col[j]);
+        raw_h[j].load(h + base + col[j]);
+        raw_n[j].load(branch + base + col[j]);
+        if (d_h != nullptr) raw_d[j].load(d_h + base + col[j]);
+      }
+    mr_next = *reinterpret_cast<const float2*>(stats + 2 * row);
+    if (sm.post >= 0) pr_next = *reinterpret_cast<const float2*>(post_stats + 2 * row);
+  };
+  constexpr bool AHEAD = VEC * NV <= RN_AHEAD;
+  if (AHEAD) fetch(0);
+  for (int i = 0; i < nrows; ++i) {
+    if (!AHEAD) fetch(i);
+    const size_t row = static_cast<size_t>(first + i), base = row * r.cols;
+    const float2 mr = mr_next, pr = pr_next;
     float t[NV][VEC], hat[NV][VEC], dh[NV][VEC], n[NV][VEC];
     float s0 = 0.0f, s1 = 0.0f;
 #pragma unroll
@@ -276,12 +342,13 @@ __global__ void __launch_bounds__(RN_BLOCK)
 #pragma unroll
       for (int e = 0; e < VEC; ++e) t[j][e] = hat[j][e] = dh[j][e] = n[j][e] = 0.0f;
       if (has[j]) {
-        get<VEC>(t[j], d_y + base + col[j]);
-        get<VEC>(hat[j], h + base + col[j]);
-        get<VEC>(n[j], branch + base + col[j]);
-        if (d_h != nullptr) get<VEC>(dh[j], d_h + base + col[j]);
+        raw_t[j].get(t[j]);
+        raw_h[j].get(hat[j]);
+        raw_n[j].get(n[j]);
+        if (d_h != nullptr) raw_d[j].get(dh[j]);
       }
     }
+    if (AHEAD) fetch(i + 1);
 #pragma unroll
     for (int j = 0; j < NV; ++j)
       if (has[j]) {
@@ -299,8 +366,6 @@ __global__ void __launch_bounds__(RN_BLOCK)
       }
     const float2 tot = row_totals(s0, s1);
     const float m0 = tot.x * inv_cols, m1 = tot.y * inv_cols;
-    float2 pr = make_float2(0.0f, 0.0f);
-    if (sm.post >= 0) pr = *reinterpret_cast<const float2*>(post_stats + 2 * row);
     s0 = s1 = 0.0f;
 #pragma unroll
     for (int j = 0; j < NV; ++j)
@@ -377,9 +442,13 @@ __global__ void __launch_bounds__(1024)
   float s = 0.0f;
   if (col < r.cols) {
     const float* p = part + static_cast<size_t>(q) * count * r.cols + col;
-    for (int c = from + lot; c < to; c += 32) {
-      const float v = p[static_cast<size_t>(c) * r.cols];
-      s = weighted ? fmaf(v, r.gate[static_cast<size_t>(c / ck.per_group) * r.cols + col], s) : s + v;
+    if (weighted) {
+#pragma unroll 4
+      for (int c = from + lot; c < to; c += 32)
+        s = fmaf(p[static_cast<size_t>(c) * r.cols], r.gate[static_cast<size_t>(c / ck.per_group) * r.cols + col], s);
+    } else {
+#pragma unroll 8
+      for (int c = from + lot; c < to; c += 32) s += p[static_cast<size_t>(c) * r.cols];
     }
   }
   tree[lot][lane] = s;
@@ -402,21 +471,32 @@ __global__ void __launch_bounds__(1024)
 }
 
 namespace {
-bool aligned16(std::initializer_list<const void*> ps) {
+// (a row of f32 is read 32 bytes at a time)
+bool aligned32(std::initializer_list<const void*> ps) {
   for (const void* p : ps)
-    if (reinterpret_cast<uintptr_t>(p) % 16 != 0) return false;
+    if (reinterpret_cast<uintptr_t>(p) % 32 != 0) return false;
   return true;
+}
+
+// Blocks that are resident at once, at most `want`.
+template <class F>
+int resident_grid(F* fn, int want) {
+  int* per_sm = per_device_slot(reinterpret_cast<const void*>(fn));
+  if (*per_sm == 0 && (cudaOccupancyMaxActiveBlocksPerMultiprocessor(per_sm, fn, RN_BLOCK, 0) != cudaSuccess || *per_sm < 1))
+    *per_sm = 1;
+  return std::min(want, *per_sm * num_sms());
 }
 
 template <class XT, class BT>
 cudaError_t forward(const ResidualNorm& r, const void* x, const void* branch, void* h, void* y, float* stats,
                     float* post_stats, cudaStream_t s) {
   const int rows = r.groups * r.rows_per_group;
-  const bool wide = r.cols % 8 == 0 && aligned16({x, branch, h, y, r.gamma, r.beta, r.scale, r.gate, r.post_gamma, r.post_beta});
+  const bool wide = r.cols % 8 == 0 && aligned32({x, branch, h, y, r.gamma, r.beta, r.scale, r.gate, r.post_gamma, r.post_beta});
 #define VK_RN(VEC, T, NV)                                                                                          \
-  k_residual_norm<XT, BT, VEC, T, NV><<<(rows + RN_BLOCK / T - 1) / (RN_BLOCK / T), RN_BLOCK, 0, s>>>(             \
-      r, rows, static_cast<const XT*>(x), static_cast<const BT*>(branch), static_cast<XT*>(h), static_cast<BT*>(y), \
-      stats, post_stats)
+  k_residual_norm<XT, BT, VEC, T, NV>                                                                              \
+      <<<resident_grid(k_residual_norm<XT, BT, VEC, T, NV>, (rows + RN_BLOCK / T - 1) / (RN_BLOCK / T)), RN_BLOCK, 0, \
+         s>>>(r, rows, FastDiv(r.rows_per_group), static_cast<const XT*>(x), static_cast<const BT*>(branch),       \
+              static_cast<XT*>(h), static_cast<BT*>(y), stats, post_stats)
   if (wide) {
     const int v = r.cols / 8;
     if (v <= 32)
@@ -452,7 +532,7 @@ cudaError_t backward(const ResidualNorm& r, const void* d_h, const void* d_y, co
                      cudaStream_t s) {
   const Chunks ck = chunks_of(r);
   const Sums sm = sums_of(r);
-  const bool wide = r.cols % 8 == 0 && aligned16({d_h, d_y, h, branch, g.d_x, g.d_branch, r.gamma, r.scale, r.gate,
+  const bool wide = r.cols % 8 == 0 && aligned32({d_h, d_y, h, branch, g.d_x, g.d_branch, r.gamma, r.scale, r.gate,
                                                   r.post_gamma, r.post_beta, part});
   const int vecs = wide ? r.cols / 8 : r.cols;
   const int threads = vecs >= RN_BLOCK ? RN_BLOCK : (vecs + 31) / 32 * 32;

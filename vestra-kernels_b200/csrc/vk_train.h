@@ -10,6 +10,19 @@
 
 namespace vk {
 
+// Division of n < 2^31 by a constant: a few instructions where the general
+// one takes a hundred, at every step.
+struct FastDiv {
+  uint32_t mul, shift;
+  explicit FastDiv(uint32_t d) : mul(0), shift(0) {
+    while ((uint64_t{1} << shift) < d) ++shift;
+    mul = static_cast<uint32_t>((((uint64_t{1} << shift) - d) << 32) / d + 1);
+  }
+  __device__ __forceinline__ int operator()(int n) const {
+    return static_cast<int>((__umulhi(static_cast<uint32_t>(n), mul) + static_cast<uint32_t>(n)) >> shift);
+  }
+};
+
 // A [batch, heads, tokens, head_dim] tensor, strides in elements.
 struct HeadsView {
   void* p = nullptr;

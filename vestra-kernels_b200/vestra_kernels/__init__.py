@@ -618,8 +618,19 @@ class _ResidualNormGrads(ctypes.Structure):
                 ("d_post_gamma", _P), ("d_post_beta", _P)]
 
 
-_on_stream = {}
+_on_stream = {}  # device: [a context, the stream it follows now]
 _on_stream_lock = threading.Lock()
+
+
+def _torch_stream(device) -> int:
+    """The cudaStream_t that torch's work on `device` goes to now."""
+    import torch
+
+    # (without the Stream object that torch.cuda.current_stream makes: 3 us of a call's 13)
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    stream = raw(device) if raw is not None else torch.cuda.current_stream(device).cuda_stream
+    # a NULL stream would mean the context's own: torch's default stream goes by its other name, cudaStreamLegacy (1)
+    return stream or 1
 
 
 def _launch(name, device, ctx, *args) -> None:
@@ -628,17 +639,18 @@ def _launch(name, device, ctx, *args) -> None:
     if ctx is not None:
         status = fn(ctx.handle, *args)
     else:
-        import torch
-
-        # a NULL stream would mean the context's own: torch's default stream goes by its other name, cudaStreamLegacy (1)
-        stream = torch.cuda.current_stream(device).cuda_stream or 1
+        stream = _torch_stream(device)
         with _on_stream_lock:  # the stream and the call that is meant for it, whichever threads call
             own = _on_stream.get(device)
             if own is None:
+                import torch
+
                 with torch.cuda.device(device):
-                    own = _on_stream[device] = Context(device)
-            own.set_stream(stream)
-            status = fn(own.handle, *args)
+                    own = _on_stream[device] = [Context(device), None]
+            if own[1] != stream:
+                own[0].set_stream(stream)
+                own[1] = stream
+            status = fn(own[0].handle, *args)
     if status != VK_OK:
         raise VestraError(status, last_error())
 
@@ -658,16 +670,17 @@ def _device_of(t, ctx):
 
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise TypeError("expected CUDA tensors")
-    if ctx is not None and ctx.device != t.device.index:
-        raise ValueError(f"the context is on device {ctx.device}, the tensors on device {t.device.index}")
-    return t.device.index
+    device = t.get_device()
+    if ctx is not None and ctx.device != device:
+        raise ValueError(f"the context is on device {ctx.device}, the tensors on device {device}")
+    return device
 
 
 def _view(t, name, shape, like):
     """A vk_heads of a [batch, heads, tokens, head_dim] tensor of any strides but the last."""
-    if t.device != like.device or t.dtype != like.dtype:
+    if t.get_device() != like.get_device() or t.dtype != like.dtype:
         raise TypeError(f"{name} must be {like.dtype} on {like.device}, got {t.dtype} on {t.device}")
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
     b, h, n, d = t.stride()
     if d != 1 and shape[3] > 1:
@@ -679,9 +692,9 @@ def _flat(t, name, shape, dtype, device):
     """The pointer of a contiguous tensor of this shape and type, None for None."""
     if t is None:
         return None
-    if t.device.type != "cuda" or t.device.index != device or t.dtype != dtype:
+    if not t.is_cuda or t.get_device() != device or t.dtype != dtype:
         raise TypeError(f"{name} must be {dtype} on cuda:{device}, got {t.dtype} on {t.device}")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
@@ -802,6 +815,10 @@ def residual_norm_workspace(x, branch, scale=None, gate=None, post_gamma=None, c
     shape = _ResidualNormShape(_dtype_code(x, "x"), _dtype_code(branch, "branch"), g, t, c, 0.0, any_vector, any_vector,
                                None if scale is None else any_vector, None if gate is None else any_vector,
                                None if post_gamma is None else any_vector, None if post_gamma is None else any_vector)
+    return _workspace_bytes(shape, dev, ctx)
+
+
+def _workspace_bytes(shape, dev, ctx) -> int:
     need = _S()
     _launch("vk_residual_norm_workspace", dev, ctx, ctypes.byref(shape), ctypes.byref(need))
     return need.value
@@ -825,7 +842,7 @@ def residual_norm_backward(d_h, d_y, h, branch, stats, gamma, d_x, d_branch, d_g
     if workspace is None:
         if ctx is not None:
             raise ValueError("with a ctx, the workspace is given by the caller")
-        need = residual_norm_workspace(h, branch, scale, gate, post_gamma)
+        need = _workspace_bytes(shape, dev, None)
         workspace = torch.empty(need, dtype=torch.uint8, device=h.device)
     grads = _ResidualNormGrads(_flat(d_x, "d_x", s, h.dtype, dev), _flat(d_branch, "d_branch", s, branch.dtype, dev),
                                _flat(d_gamma, "d_gamma", vec, f, dev), _flat(d_beta, "d_beta", vec, f, dev),

@@ -78,6 +78,11 @@ ATTENTION = [
     ("f32", 1, 1, 1, 1, 8, "head", False), ("f32", 2, 3, 5, 70, 16, "token", True), ("f32", 1, 2, 64, 64, 32, "head", False),
     ("f32", 2, 2, 65, 129, 64, "token", False), ("f32", 4, 6, 197, 197, 64, "head", True), ("f32", 1, 2, 1, 300, 64, "head", False),
     ("f32", 1, 2, 130, 1, 64, "token", False),
+    # few rows, whose long side is split over blocks (shares that are empty among them); many rows, 128 to a block
+    ("f32", 1, 1, 1, 3457, 64, "head", False), ("f32", 3, 2, 20, 700, 32, "token", True), ("f32", 2, 6, 100, 1000, 64, "head", True),
+    ("f32", 1, 1, 3, 600, 8, "head", False), ("f32", 3, 2, 40, 900, 16, "token", True), ("f32", 1, 2, 500, 500, 64, "head", False),
+    ("bf16", 2, 1, 70, 600, 32, "head", True), ("f32", 37, 8, 128, 70, 8, "head", True), ("f32", 37, 8, 128, 70, 16, "token", False),
+    ("f32", 37, 8, 127, 130, 32, "head", True), ("f32", 3, 12, 865, 865, 64, "token", True),
     ("bf16", 1, 1, 1, 1, 64, "head", False), ("bf16", 1, 2, 61, 61, 64, "token", False), ("bf16", 1, 2, 127, 128, 64, "head", False),
     ("bf16", 1, 2, 128, 129, 64, "token", False), ("bf16", 2, 3, 129, 127, 64, "head", False), ("bf16", 3, 5, 257, 385, 64, "token", True),
     ("bf16", 2, 2, 300, 1, 64, "token", False), ("bf16", 2, 2, 1, 1000, 64, "head", False), ("bf16", 1, 12, 865, 865, 64, "token", False),

@@ -97,8 +97,8 @@ int attention_shape(const char* name, const vk_attention_shape* s, AttnShape* a)
     return vk_fail(VK_UNSUPPORTED_SHAPE, "%s: head_dim %zu (supported: 8, 16, 32, 64)", name, s->head_dim);
   // tiles of 64 rows are counted in an int
   const size_t tiles = std::max(s->q_tokens, s->kv_tokens) / 64 + 1;
-  if (s->batch != 0 && s->heads > static_cast<size_t>(INT_MAX) / s->batch / tiles)
-    return vk_fail(VK_UNSUPPORTED_SHAPE, "%s: more than 2^31 tiles", name);
+  if (tiles > (1 << 24) || (s->batch != 0 && s->heads > static_cast<size_t>(INT_MAX) / s->batch / tiles))
+    return vk_fail(VK_UNSUPPORTED_SHAPE, "%s: more than 2^30 tokens or 2^31 tiles", name);
   if (!(std::isfinite(s->scale) && s->scale > 0.0f))
     return vk_fail(VK_ERR_INVALID_ARGUMENT, "%s: scale must be finite and positive", name);
   if (reinterpret_cast<uintptr_t>(s->q_lens) % 4 != 0 || reinterpret_cast<uintptr_t>(s->kv_lens) % 4 != 0)

@@ -9,14 +9,22 @@
 //   dv_j = sum_i p_ij d_out_i       dk_j = scale sum_i ds_ij q_i
 //   dq_i = scale sum_j ds_ij k_j
 //
-// A block owns 64 rows (queries for the forward pass and dq, keys for dk and
-// dv) and streams the other side in tiles of 64, so every sum has one owner
+// A block owns 16 RM rows (queries for the forward pass and dq, keys for dk
+// and dv) and streams the other side in tiles of 64, so every sum has one owner
 // and a fixed order: no atomics, the same bits every time.  The price is that
 // the backward pass computes s and dp twice (7 products instead of 5).
 //
-// 256 threads hold a 4 x 4 piece of each 64 x 64 product.  Tiles are f32 in
-// shared memory with rows of D + 4 floats, which puts the 16 rows that a
-// half-warp reads at once on different banks.
+// 16 x TX threads hold an RM x 64 / TX piece of each product.  Tiles are f32 in
+// shared memory with rows of D + 4 floats, which puts the rows that a warp
+// reads at once on different banks.
+//
+// What bounds it is what shared memory returns: 128 bytes a cycle whether or
+// not lanes read the same word, so a thread's RM x CN piece costs RM + CN
+// cycles of it for RM CN / 4 of the FMA pipe (4 x 4: 8 for 4, 8 x 8: 16 for
+// 16).  Five times 12 heads of 865 x 865 x 64 in f32: forward 8 x 8 325 us
+// (35 TFLOP/s of the 74 that the FMA pipe has), 4 x 4 368, 2 x 4 530; backward
+// 4 x 4 1206 us (33 TFLOP/s), 4 x 8 in half the threads 1246.  An 8 x 8 piece
+// of the backward pass does not leave room for two blocks on an SM.
 #include <cuda_bf16.h>
 
 #include "vk_common.cuh"
@@ -26,9 +34,26 @@
 namespace vk {
 
 namespace {
-constexpr int GT = 64;         // rows and columns of a tile
-constexpr int G_THREADS = 256; // 16 x 16
-constexpr int LDP = GT + 4;    // row of a 64 x 64 tile
+constexpr int GT = 64;          // rows of a streamed tile
+constexpr int LDP = GT + 4;     // row of a tile of scores
+
+// Two f32 products and sums in one instruction, each rounded as fmaf rounds.
+// (It halves what an 8 x 8 piece issues: 443 us without it against 325.)
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+  return d;
+}
+__device__ __forceinline__ float2 unpair(uint64_t x) {
+  float2 d;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(x));
+  return d;
+}
 
 __device__ __forceinline__ float4 load4(const float* p) { return *reinterpret_cast<const float4*>(p); }
 __device__ __forceinline__ float4 load4(const __nv_bfloat16* p) {
@@ -38,6 +63,12 @@ __device__ __forceinline__ float4 load4(const __nv_bfloat16* p) {
   return make_float4(a.x, a.y, b.x, b.y);
 }
 __device__ __forceinline__ void store1(float* p, float x) { *p = x; }
+__device__ __forceinline__ void store4(float* p, float a, float b, float c, float d) {
+  *reinterpret_cast<float4*>(p) = make_float4(a, b, c, d);
+}
+__device__ __forceinline__ void store4(__nv_bfloat16* p, float a, float b, float c, float d) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(a, b), pack_bf16x2(c, d));
+}
 __device__ __forceinline__ void store1(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
 
 template <class T>
@@ -45,13 +76,13 @@ __device__ __forceinline__ T* head_of(const HeadsView& v, int b, int h) {
   return static_cast<T*>(v.p) + b * v.sb + h * v.sh;
 }
 
-// Rows [r0, r0 + 64) of one head into shared memory; rows from n on are zero.
-template <class T, int D>
+// Rows [r0, r0 + ROWS) of one head into shared memory; rows from n on are zero.
+template <class T, int D, int ROWS, int THREADS>
 __device__ __forceinline__ void load_tile(float* dst, const T* src, int64_t st, int r0, int n) {
 #pragma unroll
-  for (int i = 0; i < GT * D / 4; i += G_THREADS) {
+  for (int i = 0; i < ROWS * D / 4; i += THREADS) {
     const int idx = i + threadIdx.x;
-    if (GT * D / 4 % G_THREADS != 0 && idx >= GT * D / 4) break;
+    if (ROWS * D / 4 % THREADS != 0 && idx >= ROWS * D / 4) break;
     const int row = idx / (D / 4), c = idx % (D / 4) * 4;
     float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (r0 + row < n) x = load4(src + static_cast<int64_t>(r0 + row) * st + c);
@@ -59,249 +90,399 @@ __device__ __forceinline__ void load_tile(float* dst, const T* src, int64_t st, 
   }
 }
 
-// s[i][j] = a[4 ty + i] . b[tx + 16 j]
-template <int D>
-__device__ __forceinline__ void product_rows(float (&s)[4][4], const float* a, const float* b, int ty, int tx) {
+// s[i][j] = a[ty + 16 i] . b[tx + TX j]
+template <int D, int RM, int TX>
+__device__ __forceinline__ void product_rows(float (&s)[RM][GT / TX], const float* a, const float* b, int ty, int tx) {
+  constexpr int CN = GT / TX;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < RM; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) s[i][j] = 0.0f;
-#pragma unroll 4
+    for (int j = 0; j < CN; ++j) s[i][j] = 0.0f;
+#pragma unroll(RM == 8 ? 2 : 4)
   for (int k = 0; k < D; k += 4) {
-    float4 x[4], y[4];
+    float4 y[CN];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const float4*>(a + (4 * ty + i) * (D + 4) + k);
+    for (int j = 0; j < CN; ++j) y[j] = load4(b + (tx + TX * j) * (D + 4) + k);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) y[j] = *reinterpret_cast<const float4*>(b + (tx + 16 * j) * (D + 4) + k);
+    for (int i = 0; i < RM; ++i) {
+      const float4 x = load4(a + (ty + 16 * i) * (D + 4) + k);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        s[i][j] = fmaf(x[i].x, y[j].x, s[i][j]);
-        s[i][j] = fmaf(x[i].y, y[j].y, s[i][j]);
-        s[i][j] = fmaf(x[i].z, y[j].z, s[i][j]);
-        s[i][j] = fmaf(x[i].w, y[j].w, s[i][j]);
-      }
-  }
-}
-
-// acc[i][c] += sum_j p[4 ty + i][j] b[j][CPT tx + c]
-template <int D, int CPT>
-__device__ __forceinline__ void product_sum(float (&acc)[4][CPT], const float* p, const float* b, int ty, int tx) {
-  if (CPT * tx >= D) return;
-#pragma unroll 4
-  for (int j = 0; j < GT; j += 4) {
-    float4 x[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const float4*>(p + (4 * ty + i) * LDP + j);
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      float y[CPT];
-      const float* row = b + (j + u) * (D + 4) + CPT * tx;
-      if constexpr (CPT == 4) {
-        const float4 v = *reinterpret_cast<const float4*>(row);
-        y[0] = v.x, y[1] = v.y, y[2] = v.z, y[3] = v.w;
-      } else if constexpr (CPT == 2) {
-        const float2 v = *reinterpret_cast<const float2*>(row);
-        y[0] = v.x, y[1] = v.y;
-      } else {
-        y[0] = *row;
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float pv = u == 0 ? x[i].x : u == 1 ? x[i].y : u == 2 ? x[i].z : x[i].w;
-#pragma unroll
-        for (int c = 0; c < CPT; ++c) acc[i][c] = fmaf(pv, y[c], acc[i][c]);
+      for (int j = 0; j < CN; ++j) {
+        s[i][j] = fmaf(x.x, y[j].x, s[i][j]);
+        s[i][j] = fmaf(x.y, y[j].y, s[i][j]);
+        s[i][j] = fmaf(x.z, y[j].z, s[i][j]);
+        s[i][j] = fmaf(x.w, y[j].w, s[i][j]);
       }
     }
   }
 }
 
-__device__ __forceinline__ float half_warp_sum(float x) {
+// A thread's columns of an output row: groups of up to four neighbours, the
+// groups 4 TX apart (neighbouring threads read neighbouring addresses).
+template <int D, int TX>
+struct OutCols {
+  static constexpr int N = D >= TX ? D / TX : 1, GROUP = N < 4 ? N : 4;
+  float v[N];
+  __device__ __forceinline__ static bool any(int tx) { return D >= TX || tx < D; }
+  __device__ __forceinline__ static int column(int c, int tx) { return c / GROUP * GROUP * TX + GROUP * tx + c % GROUP; }
+  __device__ __forceinline__ void zero() {
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-  return x;
-}
-__device__ __forceinline__ float half_warp_max(float x) {
+    for (int c = 0; c < N; ++c) v[c] = 0.0f;
+  }
+  __device__ __forceinline__ void scale(float f) {
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
-  return x;
+    for (int c = 0; c < N; ++c) v[c] *= f;
+  }
+  template <class T>
+  __device__ __forceinline__ void store(T* row, int tx, float f) const {
+    if (!any(tx)) return;
+#pragma unroll
+    for (int g = 0; g < N; g += GROUP) {
+      T* p = row + g * TX + GROUP * tx;
+      if constexpr (GROUP == 4) {
+        store4(p, v[g] * f, v[g + 1] * f, v[g + 2] * f, v[g + 3] * f);
+      } else {
+#pragma unroll
+        for (int c = 0; c < GROUP; ++c) store1(p + c, v[c] * f);
+      }
+    }
+  }
+};
+
+// acc[i] += sum_j p[ty + 16 i][j] b[j]
+template <int D, int RM, int TX>
+__device__ __forceinline__ void product_sum(OutCols<D, TX> (&acc)[RM], const float* p, const float* b, int ty, int tx) {
+  using Cols = OutCols<D, TX>;
+  if (!Cols::any(tx)) return;
+  constexpr int PAIRS = Cols::N / 2;
+  uint64_t a2[RM][PAIRS > 0 ? PAIRS : 1];
+#pragma unroll
+  for (int i = 0; i < RM; ++i)
+#pragma unroll
+    for (int c = 0; c < PAIRS; ++c) a2[i][c] = pair(acc[i].v[2 * c], acc[i].v[2 * c + 1]);
+#pragma unroll(RM == 8 ? 2 : 4)
+  for (int j = 0; j < GT; j += 4) {
+    float4 x[RM];
+#pragma unroll
+    for (int i = 0; i < RM; ++i) x[i] = load4(p + (ty + 16 * i) * LDP + j);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float* row = b + (j + u) * (D + 4) + Cols::GROUP * tx;
+      uint64_t y[PAIRS > 0 ? PAIRS : 1];
+      if constexpr (Cols::GROUP == 4) {
+#pragma unroll
+        for (int g = 0; g < Cols::N; g += 4) {
+          const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(row + g * TX);
+          y[g / 2] = w.x;
+          y[g / 2 + 1] = w.y;
+        }
+      } else if constexpr (PAIRS == 1) {
+        y[0] = *reinterpret_cast<const uint64_t*>(row);
+      }
+#pragma unroll
+      for (int i = 0; i < RM; ++i) {
+        const float w = u == 0 ? x[i].x : u == 1 ? x[i].y : u == 2 ? x[i].z : x[i].w;
+        if constexpr (PAIRS == 0) {
+          acc[i].v[0] = fmaf(w, *row, acc[i].v[0]);
+        } else {
+          const uint64_t ww = pair(w, w);
+#pragma unroll
+          for (int c = 0; c < PAIRS; ++c) a2[i][c] = fma2(ww, y[c], a2[i][c]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < RM; ++i)
+#pragma unroll
+    for (int c = 0; c < PAIRS; ++c) {
+      const float2 v = unpair(a2[i][c]);
+      acc[i].v[2 * c] = v.x;
+      acc[i].v[2 * c + 1] = v.y;
+    }
 }
 
-template <int D>
-constexpr int cols_per_thread = D >= 16 ? D / 16 : 1;
+// The streamed tiles a block takes: all, or its share of a cluster's.
+struct Share {
+  int rank, from, to;
+  __device__ __forceinline__ Share(int split, int n) : rank(static_cast<int>(blockIdx.x % split)) {
+    const int tiles = (n + GT - 1) / GT, each = (tiles + split - 1) / split;
+    from = min(rank * each, tiles) * GT;
+    to = min(from + each * GT, n);
+  }
+};
+// The blocks of a cluster join what their shares gave: every thread leaves its
+// values in its own block's memory, THREADS floats apart, and block `rank`
+// takes up some of the threads' elements from all blocks.
+constexpr int MAX_SPLIT = 8;
+__device__ __forceinline__ float left_by(const float* mine, int rank) {
+  float x;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(mapa_shared(mine, rank)));
+  return x;
+}
+__device__ __forceinline__ void left_by_all(float (&x)[MAX_SPLIT], const float* mine, int split, float none) {
+#pragma unroll
+  for (int r = 0; r < MAX_SPLIT; ++r) x[r] = r < split ? left_by(mine, r) : none;
+}
+// Calls fn(i, column, sum) for the elements of this block, summed in the order of the blocks.
+template <int D, int TX, int RM, class F>
+__device__ __forceinline__ void join_shares(const OutCols<D, TX> (&acc)[RM], float* buf, int rank, int split, F&& fn) {
+  using Cols = OutCols<D, TX>;
+  constexpr int N = Cols::N, THREADS = 16 * TX;
+  static_assert(RM * N * THREADS <= 2 * GT * (D + 4), "buf is two streamed tiles");
+  const int tx = threadIdx.x % TX;
+  __syncthreads();
+  float* mine = buf + threadIdx.x;
+#pragma unroll
+  for (int e = 0; e < RM * N; ++e) mine[e * THREADS] = acc[e / N].v[e % N];
+  cluster_sync();
+  const int per = max(1, RM * N / split);
+  if (Cols::any(tx))
+    for (int e = rank * per; e < min((rank + 1) * per, RM * N); ++e) {
+      float x[MAX_SPLIT], sum = 0.0f;
+      left_by_all(x, mine + e * THREADS, split, 0.0f);
+#pragma unroll
+      for (int r = 0; r < MAX_SPLIT; ++r) sum += x[r];
+      fn(e / N, Cols::column(e % N, tx), sum);
+    }
+  cluster_sync();  // until then the others read this block's memory
+}
+
+// over the TX threads of a row
+template <int TX>
+__device__ __forceinline__ float lanes_sum(float x) {
+#pragma unroll
+  for (int o = TX / 2; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
+}
+template <int TX>
+__device__ __forceinline__ float lanes_max(float x) {
+#pragma unroll
+  for (int o = TX / 2; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+  return x;
+}
 }  // namespace
 
-template <class T, int D>
-__global__ void __launch_bounds__(G_THREADS)
-    k_attn_forward_simt(AttnShape a, HeadsView q, HeadsView k, HeadsView v, HeadsView out, float* __restrict__ lse) {
+template <class T, int D, int RM, int TX>
+__global__ void __launch_bounds__(16 * TX, 2)
+    k_attn_forward_simt(AttnShape a, int split, HeadsView q, HeadsView k, HeadsView v, HeadsView out,
+                        float* __restrict__ lse) {
   extern __shared__ float sm[];
-  constexpr int CPT = cols_per_thread<D>;
+  constexpr int ROWS = 16 * RM, THREADS = 16 * TX, CN = GT / TX;
   float* sQ = sm;
-  float* sK = sQ + GT * (D + 4);
+  float* sK = sQ + ROWS * (D + 4);
   float* sV = sK + GT * (D + 4);
   float* sP = sV + GT * (D + 4);
-  const int tiles = (a.nq + GT - 1) / GT;
-  const int bh = blockIdx.x / tiles, r0 = (blockIdx.x - bh * tiles) * GT;
+  const int tiles = (a.nq + ROWS - 1) / ROWS;
+  const int tile = blockIdx.x / split, bh = tile / tiles, r0 = (tile - bh * tiles) * ROWS;
   const int b = bh / a.heads, h = bh - b * a.heads;
   const int nq = seq_len(a.q_lens, b, a.nq), nk = r0 < nq ? seq_len(a.kv_lens, b, a.nk) : 0;
-  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+  const int ty = threadIdx.x / TX, tx = threadIdx.x % TX;
   const T* kp = head_of<T>(k, b, h);
   const T* vp = head_of<T>(v, b, h);
-  load_tile<T, D>(sQ, head_of<T>(q, b, h), q.st, r0, nq);
-  float m[4], l[4], acc[4][CPT];
+  load_tile<T, D, ROWS, THREADS>(sQ, head_of<T>(q, b, h), q.st, r0, nq);
+  float m[RM], l[RM];
+  OutCols<D, TX> acc[RM];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < RM; ++i) {
     m[i] = -INFINITY;
     l[i] = 0.0f;
-#pragma unroll
-    for (int c = 0; c < CPT; ++c) acc[i][c] = 0.0f;
+    acc[i].zero();
   }
-  for (int c0 = 0; c0 < nk; c0 += GT) {
+  const Share share(split, nk);
+  for (int c0 = share.from; c0 < share.to; c0 += GT) {
     __syncthreads();
-    load_tile<T, D>(sK, kp, k.st, c0, nk);
-    load_tile<T, D>(sV, vp, v.st, c0, nk);
+    load_tile<T, D, GT, THREADS>(sK, kp, k.st, c0, nk);
+    load_tile<T, D, GT, THREADS>(sV, vp, v.st, c0, nk);
     __syncthreads();
-    float s[4][4];
-    product_rows<D>(s, sQ, sK, ty, tx);
+    float s[RM][CN];
+    product_rows<D, RM, TX>(s, sQ, sK, ty, tx);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < RM; ++i) {
       float top = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        s[i][j] = c0 + tx + 16 * j < nk ? s[i][j] * a.scale : -INFINITY;
+      for (int j = 0; j < CN; ++j) {
+        s[i][j] = c0 + tx + TX * j < nk ? s[i][j] * a.scale : -INFINITY;
         top = fmaxf(top, s[i][j]);
       }
-      const float m_new = fmaxf(m[i], half_warp_max(top));
+      const float m_new = fmaxf(m[i], lanes_max<TX>(top));
       const float ref = m_new == -INFINITY ? 0.0f : m_new;  // a row of -inf so far: exp(-inf - 0) = 0
       const float f = expf(m[i] - ref);
       m[i] = m_new;
       l[i] *= f;  // this thread's columns; joined over the row at the end
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < CN; ++j) {
         const float p = expf(s[i][j] - ref);
         l[i] += p;
-        sP[(4 * ty + i) * LDP + tx + 16 * j] = p;
+        sP[(ty + 16 * i) * LDP + tx + TX * j] = p;
       }
-#pragma unroll
-      for (int c = 0; c < CPT; ++c) acc[i][c] *= f;
+      acc[i].scale(f);
     }
     __syncthreads();
-    product_sum<D, CPT>(acc, sP, sV, ty, tx);
+    product_sum<D, RM, TX>(acc, sP, sV, ty, tx);
   }
-  T* op = head_of<T>(out, b, h);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = r0 + 4 * ty + i;
-    const float sum = half_warp_sum(l[i]);
+  for (int i = 0; i < RM; ++i) l[i] = lanes_sum<TX>(l[i]);
+  T* op = head_of<T>(out, b, h);
+  if constexpr (RM <= 4)
+    if (split > 1) {
+      // every block has its share's maximum, sum and result of each row
+      using Cols = OutCols<D, TX>;
+      constexpr int N = Cols::N, PER = N + 2;
+      static_assert(RM * PER * THREADS <= 2 * GT * (D + 4) + ROWS * LDP, "fits the tiles");
+      __syncthreads();
+      float* mine = sK + threadIdx.x;
+#pragma unroll
+      for (int i = 0; i < RM; ++i) {
+        mine[i * PER * THREADS] = m[i], mine[(i * PER + 1) * THREADS] = l[i];
+#pragma unroll
+        for (int c = 0; c < N; ++c) mine[(i * PER + 2 + c) * THREADS] = acc[i].v[c];
+      }
+      cluster_sync();
+      const int per = max(1, RM * N / split);
+      for (int e = share.rank * per; e < min((share.rank + 1) * per, RM * N); ++e) {
+        const int i = e / N, c = e % N, row = r0 + ty + 16 * i;
+        const float* at = mine + i * PER * THREADS;
+        float ms[MAX_SPLIT], ls[MAX_SPLIT], x[MAX_SPLIT];
+        left_by_all(ms, at, split, -INFINITY);
+        left_by_all(ls, at + THREADS, split, 0.0f);
+        left_by_all(x, at + (2 + c) * THREADS, split, 0.0f);
+        float top = -INFINITY, sum = 0.0f, total = 0.0f;
+#pragma unroll
+        for (int r = 0; r < MAX_SPLIT; ++r) top = fmaxf(top, ms[r]);
+        const float ref = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+        for (int r = 0; r < MAX_SPLIT; ++r) {
+          const float f = expf(ms[r] - ref);
+          sum = fmaf(ls[r], f, sum);
+          total = fmaf(x[r], f, total);
+        }
+        if (row >= a.nq) continue;
+        const bool live = row < nq && sum != 0.0f;
+        if (tx == 0 && c == 0) lse[static_cast<size_t>(bh) * a.nq + row] = live ? top + logf(sum) : -INFINITY;
+        if (Cols::any(tx)) store1(op + row * out.st + Cols::column(c, tx), live ? total / sum : 0.0f);
+      }
+      cluster_sync();  // until then the others read this block's memory
+      return;
+    }
+#pragma unroll
+  for (int i = 0; i < RM; ++i) {
+    const int row = r0 + ty + 16 * i;
+    const float sum = l[i];
     if (row >= a.nq) continue;
     const bool live = row < nq && sum != 0.0f;
     const float inv = live ? 1.0f / sum : 0.0f;
     if (tx == 0) lse[static_cast<size_t>(bh) * a.nq + row] = live ? m[i] + logf(sum) : -INFINITY;
-#pragma unroll
-    for (int c = 0; c < CPT; ++c)
-      if (CPT * tx + c < D) store1(op + row * out.st + CPT * tx + c, live ? acc[i][c] * inv : 0.0f);
+    if (!live) acc[i].zero();  // (a sum of 0 has no values, but 0 * inf)
+    acc[i].store(op + row * out.st, tx, inv);
   }
 }
 
-// dq and delta: a block owns 64 queries and streams the keys.
-template <class T, int D>
-__global__ void __launch_bounds__(G_THREADS)
-    k_attn_dq_simt(AttnShape a, HeadsView q, HeadsView k, HeadsView v, HeadsView out, const float* __restrict__ lse,
+// dq and delta: a block owns 16 RM queries and streams the keys.
+template <class T, int D, int RM, int TX>
+__global__ void __launch_bounds__(16 * TX, 2)
+    k_attn_dq_simt(AttnShape a, int split, HeadsView q, HeadsView k, HeadsView v, HeadsView out, const float* __restrict__ lse,
                    HeadsView d_out, HeadsView dq, float* __restrict__ delta) {
   extern __shared__ float sm[];
-  constexpr int CPT = cols_per_thread<D>;
+  constexpr int ROWS = 16 * RM, THREADS = 16 * TX, CN = GT / TX;
   float* sQ = sm;
-  float* sG = sQ + GT * (D + 4);
-  float* sK = sG + GT * (D + 4);
+  float* sG = sQ + ROWS * (D + 4);
+  float* sK = sG + ROWS * (D + 4);
   float* sV = sK + GT * (D + 4);
   float* sP = sV + GT * (D + 4);
-  const int tiles = (a.nq + GT - 1) / GT;
-  const int bh = blockIdx.x / tiles, r0 = (blockIdx.x - bh * tiles) * GT;
+  const int tiles = (a.nq + ROWS - 1) / ROWS;
+  const int tile = blockIdx.x / split, bh = tile / tiles, r0 = (tile - bh * tiles) * ROWS;
   const int b = bh / a.heads, h = bh - b * a.heads;
   const int nq = seq_len(a.q_lens, b, a.nq), nk = r0 < nq ? seq_len(a.kv_lens, b, a.nk) : 0;
-  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+  const int ty = threadIdx.x / TX, tx = threadIdx.x % TX;
   const T* kp = head_of<T>(k, b, h);
   const T* vp = head_of<T>(v, b, h);
-  load_tile<T, D>(sQ, head_of<T>(q, b, h), q.st, r0, nq);
-  load_tile<T, D>(sG, head_of<T>(d_out, b, h), d_out.st, r0, nq);
-  load_tile<T, D>(sK, head_of<T>(out, b, h), out.st, r0, nq);  // for delta only
+  load_tile<T, D, ROWS, THREADS>(sQ, head_of<T>(q, b, h), q.st, r0, nq);
+  load_tile<T, D, ROWS, THREADS>(sG, head_of<T>(d_out, b, h), d_out.st, r0, nq);
+  load_tile<T, D, ROWS, THREADS>(sK, head_of<T>(out, b, h), out.st, r0, nq);  // for delta only
   __syncthreads();
-  float ref[4], dl[4], acc[4][CPT];
+  float ref[RM], dl[RM];
+  OutCols<D, TX> acc[RM];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = r0 + 4 * ty + i;
+  for (int i = 0; i < RM; ++i) {
+    const int row = r0 + ty + 16 * i;
     float x = 0.0f;
-    for (int c = tx; c < D; c += 16) x = fmaf(sG[(4 * ty + i) * (D + 4) + c], sK[(4 * ty + i) * (D + 4) + c], x);
-    dl[i] = half_warp_sum(x);
+    for (int c = tx; c < D; c += TX) x = fmaf(sG[(ty + 16 * i) * (D + 4) + c], sK[(ty + 16 * i) * (D + 4) + c], x);
+    dl[i] = lanes_sum<TX>(x);
     const float e = row < nq ? lse[static_cast<size_t>(bh) * a.nq + row] : 0.0f;
     ref[i] = e == -INFINITY ? 0.0f : e;  // such a row has scores of -inf only: exp(-inf - 0) = 0
-    if (tx == 0 && row < a.nq) delta[static_cast<size_t>(bh) * a.nq + row] = dl[i];
-#pragma unroll
-    for (int c = 0; c < CPT; ++c) acc[i][c] = 0.0f;
+    if (tx == 0 && row < a.nq && blockIdx.x % split == 0) delta[static_cast<size_t>(bh) * a.nq + row] = dl[i];
+    acc[i].zero();
   }
-  for (int c0 = 0; c0 < nk; c0 += GT) {
+  const Share share(split, nk);
+  for (int c0 = share.from; c0 < share.to; c0 += GT) {
     __syncthreads();
-    load_tile<T, D>(sK, kp, k.st, c0, nk);
-    load_tile<T, D>(sV, vp, v.st, c0, nk);
+    load_tile<T, D, GT, THREADS>(sK, kp, k.st, c0, nk);
+    load_tile<T, D, GT, THREADS>(sV, vp, v.st, c0, nk);
     __syncthreads();
-    float s[4][4], dp[4][4];
-    product_rows<D>(s, sQ, sK, ty, tx);
-    product_rows<D>(dp, sG, sV, ty, tx);
+    float s[RM][CN], dp[RM][CN];
+    product_rows<D, RM, TX>(s, sQ, sK, ty, tx);
+    product_rows<D, RM, TX>(dp, sG, sV, ty, tx);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < RM; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float p = c0 + tx + 16 * j < nk ? expf(fmaf(s[i][j], a.scale, -ref[i])) : 0.0f;
-        sP[(4 * ty + i) * LDP + tx + 16 * j] = p * (dp[i][j] - dl[i]);
+      for (int j = 0; j < CN; ++j) {
+        const float p = c0 + tx + TX * j < nk ? expf(fmaf(s[i][j], a.scale, -ref[i])) : 0.0f;
+        sP[(ty + 16 * i) * LDP + tx + TX * j] = p * (dp[i][j] - dl[i]);
       }
     __syncthreads();
-    product_sum<D, CPT>(acc, sP, sK, ty, tx);
+    product_sum<D, RM, TX>(acc, sP, sK, ty, tx);
   }
   T* dqp = head_of<T>(dq, b, h);
+  if (split > 1) {
+    join_shares(acc, sK, share.rank, split, [&](int i, int col, float sum) {
+      const int row = r0 + ty + 16 * i;
+      if (row < a.nq) store1(dqp + row * dq.st + col, row < nq ? sum * a.scale : 0.0f);
+    });
+    return;
+  }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = r0 + 4 * ty + i;
+  for (int i = 0; i < RM; ++i) {
+    const int row = r0 + ty + 16 * i;
     if (row >= a.nq) continue;
-#pragma unroll
-    for (int c = 0; c < CPT; ++c)
-      if (CPT * tx + c < D) store1(dqp + row * dq.st + CPT * tx + c, row < nq ? acc[i][c] * a.scale : 0.0f);
+    if (row >= nq) acc[i].zero();
+    acc[i].store(dqp + row * dq.st, tx, a.scale);
   }
 }
 
-// dk and dv: a block owns 64 keys and streams the queries.
-template <class T, int D>
-__global__ void __launch_bounds__(G_THREADS)
-    k_attn_dkdv_simt(AttnShape a, HeadsView q, HeadsView k, HeadsView v, const float* __restrict__ lse, HeadsView d_out,
+// dk and dv: a block owns 16 RM keys and streams the queries.
+template <class T, int D, int RM, int TX>
+__global__ void __launch_bounds__(16 * TX, 2)
+    k_attn_dkdv_simt(AttnShape a, int split, HeadsView q, HeadsView k, HeadsView v, const float* __restrict__ lse, HeadsView d_out,
                      HeadsView dk, HeadsView dv, const float* __restrict__ delta) {
   extern __shared__ float sm[];
-  constexpr int CPT = cols_per_thread<D>;
+  constexpr int ROWS = 16 * RM, THREADS = 16 * TX, CN = GT / TX;
   float* sK = sm;
-  float* sV = sK + GT * (D + 4);
-  float* sQ = sV + GT * (D + 4);
+  float* sV = sK + ROWS * (D + 4);
+  float* sQ = sV + ROWS * (D + 4);
   float* sG = sQ + GT * (D + 4);
   float* sP = sG + GT * (D + 4);
-  float* sD = sP + GT * LDP;
-  float* sRef = sD + GT * LDP;
+  float* sD = sP + ROWS * LDP;
+  float* sRef = sD + ROWS * LDP;
   float* sDelta = sRef + GT;
-  const int tiles = (a.nk + GT - 1) / GT;
-  const int bh = blockIdx.x / tiles, r0 = (blockIdx.x - bh * tiles) * GT;
+  const int tiles = (a.nk + ROWS - 1) / ROWS;
+  const int tile = blockIdx.x / split, bh = tile / tiles, r0 = (tile - bh * tiles) * ROWS;
   const int b = bh / a.heads, h = bh - b * a.heads;
   const int nk = seq_len(a.kv_lens, b, a.nk), nq = r0 < nk ? seq_len(a.q_lens, b, a.nq) : 0;
-  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+  const int ty = threadIdx.x / TX, tx = threadIdx.x % TX;
   const T* qp = head_of<T>(q, b, h);
   const T* gp = head_of<T>(d_out, b, h);
-  load_tile<T, D>(sK, head_of<T>(k, b, h), k.st, r0, nk);
-  load_tile<T, D>(sV, head_of<T>(v, b, h), v.st, r0, nk);
-  float ak[4][CPT], av[4][CPT];
+  load_tile<T, D, ROWS, THREADS>(sK, head_of<T>(k, b, h), k.st, r0, nk);
+  load_tile<T, D, ROWS, THREADS>(sV, head_of<T>(v, b, h), v.st, r0, nk);
+  OutCols<D, TX> ak[RM], av[RM];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int c = 0; c < CPT; ++c) ak[i][c] = av[i][c] = 0.0f;
-  for (int c0 = 0; c0 < nq; c0 += GT) {
+  for (int i = 0; i < RM; ++i)
+    ak[i].zero(), av[i].zero();
+  const Share share(split, nq);
+  for (int c0 = share.from; c0 < share.to; c0 += GT) {
     __syncthreads();
-    load_tile<T, D>(sQ, qp, q.st, c0, nq);
-    load_tile<T, D>(sG, gp, d_out.st, c0, nq);
+    load_tile<T, D, GT, THREADS>(sQ, qp, q.st, c0, nq);
+    load_tile<T, D, GT, THREADS>(sG, gp, d_out.st, c0, nq);
     if (threadIdx.x < GT) {
       const int row = c0 + threadIdx.x;
       const size_t at = static_cast<size_t>(bh) * a.nq + row;
@@ -310,34 +491,42 @@ __global__ void __launch_bounds__(G_THREADS)
       sDelta[threadIdx.x] = row < nq ? delta[at] : 0.0f;
     }
     __syncthreads();
-    float s[4][4], dp[4][4];
-    product_rows<D>(s, sK, sQ, ty, tx);
-    product_rows<D>(dp, sV, sG, ty, tx);
+    float s[RM][CN], dp[RM][CN];
+    product_rows<D, RM, TX>(s, sK, sQ, ty, tx);
+    product_rows<D, RM, TX>(dp, sV, sG, ty, tx);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < RM; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int c = tx + 16 * j;
+      for (int j = 0; j < CN; ++j) {
+        const int c = tx + TX * j;
         const float p = c0 + c < nq ? expf(fmaf(s[i][j], a.scale, -sRef[c])) : 0.0f;
-        sP[(4 * ty + i) * LDP + c] = p;
-        sD[(4 * ty + i) * LDP + c] = p * (dp[i][j] - sDelta[c]);
+        sP[(ty + 16 * i) * LDP + c] = p;
+        sD[(ty + 16 * i) * LDP + c] = p * (dp[i][j] - sDelta[c]);
       }
     __syncthreads();
-    product_sum<D, CPT>(av, sP, sG, ty, tx);
-    product_sum<D, CPT>(ak, sD, sQ, ty, tx);
+    product_sum<D, RM, TX>(av, sP, sG, ty, tx);
+    product_sum<D, RM, TX>(ak, sD, sQ, ty, tx);
   }
   T* dkp = head_of<T>(dk, b, h);
   T* dvp = head_of<T>(dv, b, h);
+  if (split > 1) {
+    join_shares(ak, sQ, share.rank, split, [&](int i, int col, float sum) {
+      const int row = r0 + ty + 16 * i;
+      if (row < a.nk) store1(dkp + row * dk.st + col, row < nk ? sum * a.scale : 0.0f);
+    });
+    join_shares(av, sQ, share.rank, split, [&](int i, int col, float sum) {
+      const int row = r0 + ty + 16 * i;
+      if (row < a.nk) store1(dvp + row * dv.st + col, row < nk ? sum : 0.0f);
+    });
+    return;
+  }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = r0 + 4 * ty + i;
+  for (int i = 0; i < RM; ++i) {
+    const int row = r0 + ty + 16 * i;
     if (row >= a.nk) continue;
-#pragma unroll
-    for (int c = 0; c < CPT; ++c)
-      if (CPT * tx + c < D) {
-        store1(dkp + row * dk.st + CPT * tx + c, row < nk ? ak[i][c] * a.scale : 0.0f);
-        store1(dvp + row * dv.st + CPT * tx + c, row < nk ? av[i][c] : 0.0f);
-      }
+    if (row >= nk) ak[i].zero(), av[i].zero();
+    ak[i].store(dkp + row * dk.st, tx, a.scale);
+    av[i].store(dvp + row * dv.st, tx, 1.0f);
   }
 }
 
@@ -378,36 +567,93 @@ cudaError_t fill_f32(float* x, size_t n, float value, cudaStream_t s) {
 }
 
 namespace {
-template <int D>
-constexpr int tile_bytes(int tiles, int squares, int rows) {
-  return (tiles * GT * (D + 4) + squares * GT * LDP + rows * GT) * static_cast<int>(sizeof(float));
+// `own` tiles of 16 RM rows, `streamed` ones of 64, `scores` of 16 RM x 64, `rows` vectors of 64
+template <int D, int RM>
+constexpr int tile_bytes(int own, int streamed, int scores, int rows) {
+  return ((own * 16 * RM + streamed * GT) * (D + 4) + scores * 16 * RM * LDP + rows * GT) * static_cast<int>(sizeof(float));
+}
+int blocks_of(const AttnShape& a, int tokens, int rows) { return a.batch * a.heads * ((tokens + rows - 1) / rows); }
+
+template <class... P, class... A>
+cudaError_t launch(void (*fn)(P...), int tiles, int split, int threads, int bytes, cudaStream_t s, A... args) {
+  cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(fn), bytes);
+  if (e != cudaSuccess) return e;
+  cudaLaunchAttribute cluster{};
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim.x = split, cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(tiles * split);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = s;
+  cfg.attrs = &cluster;
+  cfg.numAttrs = split > 1 ? 1 : 0;
+  e = cudaLaunchKernelEx(&cfg, fn, args...);
+  return e == cudaSuccess ? cudaGetLastError() : e;
+}
+
+// How a product of `own` rows per head with `streamed` ones is laid out: 16 rm
+// rows per block, the streamed rows split over a cluster of `split` blocks.
+//
+// 8 (forward only) where the SM with the most rows has no more of them than
+// with 4: 36 heads of 865 tokens 214 against 247 us, but 12 heads of 3457, 1243
+// against 1180.  With fewer blocks than SMs the streamed side is split, to fill
+// the SMs, and beyond that while a share has two tiles: 18 heads of 197 tokens
+// 27 us as one block per 64 rows, 20 split by 2; 6 heads of 433, 41 and 31; 12
+// heads of 100 queries and 3000 keys, 231 and 61.  2 for a few rows: one query
+// of 3457 keys 266 us with 64 rows in one block, 209 with 32, 35 split by 8.
+struct Layout {
+  int rm, split;
+};
+Layout layout_of(const AttnShape& a, int own, int streamed, bool wide) {
+  const int sms = num_sms(), n8 = blocks_of(a, own, 128), n4 = blocks_of(a, own, 64);
+  if (wide && n8 > sms && (n8 + sms - 1) / sms * 2 <= (n4 + sms - 1) / sms) return {8, 1};
+  if (n4 >= sms) return {4, 1};
+  const int rm = own <= 32 ? 2 : 4;
+  const int tiles = (streamed + GT - 1) / GT;
+  int split = 1;
+  while (split < MAX_SPLIT && split * 2 <= tiles &&
+         (n4 * split * 2 <= sms || (n4 * split <= sms && split * 4 <= tiles)))
+    split *= 2;
+  return {rm, split};
 }
 
 template <class T, int D>
 cudaError_t forward(const AttnShape& a, HeadsView q, HeadsView k, HeadsView v, HeadsView out, float* lse,
                     cudaStream_t s) {
-  constexpr int bytes = tile_bytes<D>(3, 1, 0);
-  auto* fn = k_attn_forward_simt<T, D>;
-  const cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(fn), bytes);
-  if (e != cudaSuccess) return e;
-  fn<<<a.batch * a.heads * ((a.nq + GT - 1) / GT), G_THREADS, bytes, s>>>(a, q, k, v, out, lse);
-  return cudaGetLastError();
+  const Layout l = layout_of(a, a.nq, a.nk, true);
+  const int tiles = blocks_of(a, a.nq, 16 * l.rm);
+  if (l.rm == 8)
+    return launch(k_attn_forward_simt<T, D, 8, 8>, tiles, 1, 128, tile_bytes<D, 8>(1, 2, 1, 0), s, a, 1, q, k, v, out, lse);
+  if (l.rm == 4)
+    return launch(k_attn_forward_simt<T, D, 4, 16>, tiles, l.split, 256, tile_bytes<D, 4>(1, 2, 1, 0), s, a, l.split, q, k,
+                  v, out, lse);
+  return launch(k_attn_forward_simt<T, D, 2, 16>, tiles, l.split, 256, tile_bytes<D, 2>(1, 2, 1, 0), s, a, l.split, q, k, v,
+                out, lse);
 }
 
+template <class T, int D, int RM>
+cudaError_t backward_dq(int split, const AttnShape& a, HeadsView q, HeadsView k, HeadsView v, HeadsView out,
+                        const float* lse, HeadsView d_out, HeadsView dq, float* delta, cudaStream_t s) {
+  return launch(k_attn_dq_simt<T, D, RM, 16>, blocks_of(a, a.nq, 16 * RM), split, 256, tile_bytes<D, RM>(2, 2, 1, 0), s, a,
+                split, q, k, v, out, lse, d_out, dq, delta);
+}
+template <class T, int D, int RM>
+cudaError_t backward_dkdv(int split, const AttnShape& a, HeadsView q, HeadsView k, HeadsView v, const float* lse,
+                          HeadsView d_out, HeadsView dk, HeadsView dv, const float* delta, cudaStream_t s) {
+  return launch(k_attn_dkdv_simt<T, D, RM, 16>, blocks_of(a, a.nk, 16 * RM), split, 256, tile_bytes<D, RM>(2, 2, 2, 2), s,
+                a, split, q, k, v, lse, d_out, dk, dv, delta);
+}
 template <class T, int D>
 cudaError_t backward(const AttnShape& a, HeadsView q, HeadsView k, HeadsView v, HeadsView out, const float* lse,
                      HeadsView d_out, HeadsView dq, HeadsView dk, HeadsView dv, float* delta, cudaStream_t s) {
-  constexpr int bytes_q = tile_bytes<D>(4, 1, 0), bytes_k = tile_bytes<D>(4, 2, 2);
-  auto* fq = k_attn_dq_simt<T, D>;
-  auto* fk = k_attn_dkdv_simt<T, D>;
-  cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(fq), bytes_q);
-  if (e == cudaSuccess) e = ensure_smem_limit(reinterpret_cast<const void*>(fk), bytes_k);
+  Layout l = layout_of(a, a.nq, a.nk, false);
+  const cudaError_t e = l.rm == 4 ? backward_dq<T, D, 4>(l.split, a, q, k, v, out, lse, d_out, dq, delta, s)
+                                  : backward_dq<T, D, 2>(l.split, a, q, k, v, out, lse, d_out, dq, delta, s);
   if (e != cudaSuccess) return e;
-  fq<<<a.batch * a.heads * ((a.nq + GT - 1) / GT), G_THREADS, bytes_q, s>>>(a, q, k, v, out, lse, d_out, dq, delta);
-  e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
-  fk<<<a.batch * a.heads * ((a.nk + GT - 1) / GT), G_THREADS, bytes_k, s>>>(a, q, k, v, lse, d_out, dk, dv, delta);
-  return cudaGetLastError();
+  l = layout_of(a, a.nk, a.nq, false);
+  return l.rm == 4 ? backward_dkdv<T, D, 4>(l.split, a, q, k, v, lse, d_out, dk, dv, delta, s)
+                   : backward_dkdv<T, D, 2>(l.split, a, q, k, v, lse, d_out, dk, dv, delta, s);
 }
 }  // namespace
 

@@ -523,6 +523,9 @@ NORMS = [  # stream, branch, groups, rows, cols, scale, gate, post, d_h
     ("f32", "f32", 1, 9, 8192, True, True, True, True), ("f32", "f32", 1, 6, 8191, True, True, True, False),
     ("f32", "bf16", 2, 433, 768, True, True, True, False), ("f32", "bf16", 70, 2, 128, True, True, False, True),
     ("f32", "bf16", 1, 11, 512, True, False, True, True), ("bf16", "bf16", 1, 11, 100, False, False, False, True),
+    # more rows than blocks have at once, of one warp and of four, with pieces of eight and of one
+    ("f32", "bf16", 4, 3501, 72, True, True, True, True), ("bf16", "bf16", 2, 1701, 1104, True, True, False, True),
+    ("f32", "f32", 3, 1100, 201, True, False, True, True),
 ]
 
 
@@ -765,6 +768,77 @@ def test_residual_norm_empty_capture_and_refusals(vk):
         run_norm_backward(vk, s, h, stats, post_stats, None, d_y, workspace=torch.empty(64, dtype=torch.uint8, device="cuda"))
     with pytest.raises(ValueError):
         run_norm_backward(vk, s, h, stats, post_stats, None, d_y, ctx=vk.Context(0))
+
+
+def test_residual_norm_in_place_and_at_odd_addresses(vk):
+    """h written over x and the gradients over d_h and d_y, with more rows than blocks have at once: the same bits.
+    Matrices that start 4 or 2 bytes off take another path; it sums in another order, within a few roundings."""
+    s = norm_inputs("f32", "bf16", 3, 4001, 136, True, True, True, 50)
+    h, y, stats, post_stats = run_norm(vk, s)
+    g = gen(51)
+    d_h, d_y = torch.randn(h.shape, device="cuda", generator=g), torch.randn(y.shape, device="cuda", generator=g).bfloat16()
+    want = run_norm_backward(vk, s, h, stats, post_stats, d_h, d_y)
+    x, y2 = s["x"].clone(), torch.empty_like(y)
+    vk.residual_norm_forward(x, s["branch"], s["gamma"], s["beta"], EPS, x, y2, torch.empty_like(stats), scale=s["scale"],
+                             gate=s["gate"], post_gamma=s["post_gamma"], post_beta=s["post_beta"],
+                             post_stats=torch.empty_like(post_stats))
+    assert torch.equal(x, h) and torch.equal(y2, y)
+    dh2, dy2 = d_h.clone(), d_y.clone()
+    got = run_norm_backward(vk, s, h, stats, post_stats, dh2, dy2, d_x=dh2, d_branch=dy2)
+    assert all(torch.equal(got[n], want[n]) for n in want)
+
+    def off(t):  # the same values, one element further
+        return torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")[1:].view(t.shape).copy_(t)
+
+    moved = {n: (v if v is None else off(v)) for n, v in s.items()}
+    h3, y3, stats3, post3 = run_norm(vk, moved)
+    # h: a norm whose two sums of 136 and few products round differently, then three products and a sum
+    within(h3, h, 2.0 ** -24 * (2 * 136 + 16) * (1 + h.abs() + s["x"].abs()).double() * 4, "h")
+    got = run_norm_backward(vk, moved, off(h), stats, post_stats, off(d_h), off(d_y))
+    # the same formulas on the same values: sums of 136 in another order, of terms no larger than the largest
+    most = want["d_x"].abs().amax().double()
+    within(got["d_x"], want["d_x"], 2.0 ** -24 * 4 * 136 * most, "d_x")
+
+
+def test_residual_norm_refuses_shared_vectors(vk):
+    s = norm_inputs("f32", "bf16", 2, 40, 256, True, True, True, 52)
+    h, y, stats, post_stats = run_norm(vk, s)
+    with pytest.raises(vk.VestraError):
+        vk.residual_norm_forward(s["x"], s["branch"], s["gamma"], s["beta"], EPS, h, y, stats, post_gamma=s["post_gamma"],
+                                 post_beta=s["post_beta"], post_stats=stats)
+    for name in ("scale", "gate", "post_gamma"):
+        with pytest.raises(vk.VestraError):
+            run_norm_backward(vk, s, h, stats, post_stats, None, y, **{"d_" + name: s[name]})
+
+
+def test_two_threads_on_streams_of_their_own(vk):
+    """Calls without a ctx from two threads at once: each goes to its thread's stream, and none reports an error."""
+    import threading
+
+    inputs = [attention_case(torch.bfloat16, 2, 4, 300, 300, 64, "head", False, 60 + i)[:3] for i in range(2)]
+    want = [run_forward(vk, *x, None, None) for x in inputs]
+    torch.cuda.synchronize()
+    got, errors = [None, None], []
+
+    def work(i):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(50):
+                    got[i] = run_forward(vk, *inputs[i], None, None)
+            stream.synchronize()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    vk.synchronize()
+    for (out, lse), (w, wl) in zip(got, want):
+        assert torch.equal(out, w) and torch.equal(lse, wl)
 
 
 # ------------------------------------------------------------------ a run of them together

@@ -122,9 +122,10 @@ int floats_ok(const char* name, const char* what, const float* p, size_t align =
 }
 
 // Outputs that start where an input or another output does would be written
-// while they are read.
+// while they are read.  (NULL: not there.)
 int apart(const char* name, std::initializer_list<const void*> outs, std::initializer_list<const void*> ins) {
   for (const void* const* o = outs.begin(); o != outs.end(); ++o) {
+    if (*o == nullptr) continue;
     for (const void* i : ins)
       if (*o == i) return vk_fail(VK_ERR_INVALID_ARGUMENT, "%s: an output is one of the inputs", name);
     for (const void* const* p = outs.begin(); p != o; ++p)
@@ -329,7 +330,8 @@ extern "C" int vk_residual_norm_forward(vk_ctx* ctx, const vk_residual_norm_shap
     VK_TRY(matrix_ok(name, "y", y, shape->branch_dtype));
     VK_TRY(floats_ok(name, "stats", stats, 8));
     if (r.post_gamma != nullptr) VK_TRY(floats_ok(name, "post_stats", post_stats, 8));
-    VK_TRY(apart(name, {h, y, stats}, {branch}));
+    VK_TRY(apart(name, {h, y, stats, r.post_gamma != nullptr ? post_stats : nullptr},
+                 {branch, r.gamma, r.beta, r.scale, r.gate, r.post_gamma, r.post_beta}));
     if (y == x) return vk_fail(VK_ERR_INVALID_ARGUMENT, "%s: y is x", name);
     return vk_cuda_status(residual_norm_forward(r, shape->stream_dtype == VK_DTYPE_BF16, shape->branch_dtype == VK_DTYPE_BF16,
                                                 x, branch, h, y, stats, post_stats, ctx->stream),
@@ -385,7 +387,9 @@ extern "C" int vk_residual_norm_backward(vk_ctx* ctx, const vk_residual_norm_sha
     const size_t need = residual_norm_workspace(r);
     if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 != 0 || workspace_bytes < need)
       return vk_fail(VK_ERR_INVALID_ARGUMENT, "%s: workspace of %zu bytes, 16-byte aligned, is needed (got %zu)", name, need, workspace_bytes);
-    VK_TRY(apart(name, {grads->d_x, grads->d_branch, workspace}, {h, branch}));
+    VK_TRY(apart(name, {grads->d_x, grads->d_branch, workspace, grads->d_gamma, grads->d_beta, grads->d_scale, grads->d_gate,
+                        grads->d_post_gamma, grads->d_post_beta},
+                 {h, branch, stats, r.gamma, r.scale, r.gate, r.post_gamma, r.post_beta}));
     if (grads->d_x == d_y || grads->d_branch == d_h)
       return vk_fail(VK_ERR_INVALID_ARGUMENT, "%s: d_x may be d_h and d_branch d_y, not the other way round", name);
     ResidualNormGrads g;

@@ -655,6 +655,18 @@ def _launch(name, device, ctx, *args) -> None:
         raise VestraError(status, last_error())
 
 
+def synchronize(device: int | None = None) -> None:
+    """Waits for the last of the calls that were made without a ctx on `device` (torch's current one) and raises the
+    error that a kernel of theirs reported (Context.synchronize does so for the calls on a ctx)."""
+    import torch
+
+    device = torch.cuda.current_device() if device is None else device
+    with _on_stream_lock:
+        own = _on_stream.get(device)
+        if own is not None:
+            own[0].synchronize()
+
+
 def _dtype_code(t, name):
     import torch
 

@@ -4,9 +4,11 @@
 //   lo' = lo cos a - hi sin a,  hi' = hi cos a + lo sin a
 // (the inverse, which is the gradient, with -sin).  HBM-bound: each element is
 // read and written once, and an angle is computed once for all heads of q and
-// k.  (With the angles of a few tokens in shared memory and the threads along
-// the heads, 16 clips of 3457 tokens, 12 heads of 64 each for q and k in bf16,
-// took 123 us; this way 75, 4.6 TB/s.)
+// k.  A thread keeps the angles of a few pairs of one token and goes along the
+// heads, three at a time.  16 clips of 3457 tokens, 12 heads of 64 each for q
+// and k in bf16: 64 us, 5.3 TB/s; with four heads at a time 68, with two 68,
+// with blocks of 256 threads 65, with the angles of a few tokens in shared
+// memory and the threads along the heads 123.
 //
 // Angles are formed and reduced by 2 pi in double precision: an f32 product
 // would be off by 2^-24 of the angle itself (2e-4 radians at position 4096).
@@ -20,8 +22,8 @@
 namespace vk {
 
 namespace {
-constexpr int RA_THREADS = 256;
-constexpr int RA_BATCH = 4;
+constexpr int RA_THREADS = 128;
+constexpr int RA_BATCH = 3;
 
 template <int BYTES>
 struct RawOf;

@@ -24,6 +24,8 @@
 // result); everything else is f32.  Rows and columns past a sequence's length
 // never reach a product: scores are masked, and the tail of a streamed tile is
 // zeroed in shared memory, because 0 * NaN would spread what lies there.
+#include <limits.h>
+
 #include "vk_common.cuh"
 #include "vk_internal.h"
 #include "vk_train.h"
@@ -214,6 +216,93 @@ __device__ __forceinline__ float2 exp2_pair(float2 x, int i) {
 }
 }  // namespace
 
+// ------------------------------------------------------------------ items
+// Without lengths a CTA takes every gridDim.x-th item: all are alike.
+//
+// Of a padded batch (LENS) each CTA lays out its items once in shared memory,
+// and its warps walk that list.  Those with work come first, sequences with the
+// most blocks in front, then the others (rows that only get zeros); they go
+// there and back over the CTAs, so that the one with the longest item of a
+// round has the shortest of the next.  In the batch's own order the shares
+// differ: of four sequences of 3457, 1729, 2283 and 829 tokens some CTAs had 160
+// blocks of dq where the mean is 110.  That batch: forward 148 us in the
+// batch's order, 109 this way, backward 332 and 296; 16 images of 865 to 115
+// tokens forward 51 and 43.  (Batches without lengths only lose by the list: 64
+// images backward 612 us and 650, so each form is a kernel of its own.)
+// The steps are written out where they are taken: with named integers the
+// kernels without lengths came out 3 to 5% slower.
+namespace {
+constexpr int LIST_MAX = 128;   // items of a CTA in a launch
+constexpr int ORDER_MAX = 128;  // sequences that are ordered; more of them even out by themselves
+template <bool LENS>
+struct ItemList {
+  int4 item[LIST_MAX];
+  short2 len[ORDER_MAX];       // a sequence's items with work per head, and its blocks
+  int first[2][ORDER_MAX];     // by rank: ordinal of a sequence's first item with work / without
+  short2 sequence[ORDER_MAX];  // by rank: the sequence, its items with work per head
+  int live;                    // items with work
+
+  // `rows` own rows per item, `per_head` items per head, `count` of them from
+  // `base` on in this launch; make((sequence, head), item of the head) gives
+  // an entry.  Returns the length of the list.
+  template <class F>
+  __device__ __forceinline__ int build(const AttnShape& a, const int32_t* own_lens, int own, const int32_t* other_lens,
+                                       int other, int rows, int per_head, int base, int count, F make) {
+    const bool ordered = a.batch <= ORDER_MAX && per_head <= SHRT_MAX && other <= SHRT_MAX * TR;
+    const int i = threadIdx.x;
+    if (ordered) {
+      if (i < a.batch) {
+        const int nb = (seq_len(other_lens, i, other) + TR - 1) / TR;
+        len[i] = make_short2(nb == 0 ? 0 : (seq_len(own_lens, i, own) + rows - 1) / rows, nb);
+      }
+      __syncthreads();
+      if (i < a.batch) {
+        const short2 mine = len[i];
+        int rank = 0, with = 0, without = 0;
+        for (int j = 0; j < a.batch; ++j) {
+          const short2 o = len[j];
+          if (o.y > mine.y || (o.y == mine.y && j < i)) {
+            ++rank;
+            with += o.x;
+            without += per_head - o.x;
+          }
+        }
+        first[0][rank] = with * a.heads;
+        first[1][rank] = without * a.heads;
+        sequence[rank] = make_short2(i, mine.x);
+        if (rank == a.batch - 1) live = (with + mine.x) * a.heads;
+      }
+      __syncthreads();
+    }
+    const int g = gridDim.x, c = blockIdx.x, rounds = count / g;
+    const int mine = rounds + ((rounds & 1 ? g - 1 - c : c) < count - rounds * g ? 1 : 0);
+    for (int k = i; k < mine; k += blockDim.x) {
+      const int it = base + k * g + (k & 1 ? g - 1 - c : c);
+      int bh = it / per_head, n = it - bh * per_head;
+      if (ordered) {
+        const bool rest = it >= live;
+        const int* f = first[rest];
+        const int x = rest ? it - live : it;
+        int r = 0;  // the last rank whose first item is not past x
+        for (int left = a.batch; left > 1;) {
+          const int half = left / 2;
+          if (f[r + half] <= x) r += half;
+          left -= half;
+        }
+        const short2 s = sequence[r];
+        const int each = rest ? per_head - s.y : s.y, h = (x - f[r]) / each;
+        bh = s.x * a.heads + h;
+        n = x - f[r] - h * each + (rest ? s.y : 0);
+      }
+      item[k] = make(bh, n);
+    }
+    return mine;
+  }
+};
+template <>
+struct ItemList<false> {};
+}  // namespace
+
 // ------------------------------------------------------------------ forward
 // An item is two query tiles, each with its own group of four warps, that
 // share the K / V blocks of their head (one tile where pairs would leave SMs
@@ -235,12 +324,16 @@ constexpr uint32_t F_P = 256, F_O = 384;
 constexpr size_t F_SMEM = 1024 + TILE_B * (4 + 2 * ST) + (ST + 1) * EXT_B + 512;
 }  // namespace
 
+template <bool LENS>
 __global__ void __launch_bounds__(F_THREADS, 1)
     k_attn_forward_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                       const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO, AttnShape a,
                       HeadsView out, float* __restrict__ lse, int items, int per_head, int mixed_from, FastDiv by_head,
                       FastDiv by_batch, int tpi, int* err) {
   extern __shared__ uint8_t smem_raw[];
+  __shared__ ItemList<LENS> list;
+  // LENS: the launch has `items` items from `mixed_from` on (there is no mixing), `mine` of them are this CTA's
+  [[maybe_unused]] int mine = 0;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;  // [item parity][tile], then the tile's output on its way out
   uint8_t* sK = smem + 4 * TILE_B;
@@ -270,6 +363,17 @@ __global__ void __launch_bounds__(F_THREADS, 1)
   auto item_of = [&](int it) {
     Item r;
     r.kvs = 1;
+    if constexpr (LENS) {
+      const int4 e = list.item[it];
+      r.bh[0] = r.bh[1] = e.x;
+      r.q0[0] = e.y;
+      r.q0[1] = r.q0[0] + TR;
+      r.nq = e.z;
+      r.nk = e.w;
+      r.nb = (r.nk + TR - 1) / TR;
+      r.tiles = r.nb == 0 || r.q0[0] >= r.nq ? 0 : tpi == 2 && r.q0[1] < r.nq ? 2 : 1;
+      return r;
+    }
     if (it < mixed_from) {
       r.bh[0] = r.bh[1] = by_head(it);
       r.q0[0] = (it - r.bh[0] * per_head) * tpi * TR;
@@ -324,6 +428,11 @@ __global__ void __launch_bounds__(F_THREADS, 1)
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
+  if constexpr (LENS)
+    mine = list.build(a, a.q_lens, a.nq, a.kv_lens, a.nk, tpi * TR, per_head, mixed_from, items, [&](int bh, int n) {
+      const int b = bh / a.heads;
+      return make_int4(bh, n * tpi * TR, seq_len(a.q_lens, b, a.nq), seq_len(a.kv_lens, b, a.nk));
+    });
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -335,7 +444,7 @@ __global__ void __launch_bounds__(F_THREADS, 1)
       uint32_t g = 0, c = 0;                   // blocks, items with work
       uint32_t used[2][2] = {{0, 0}, {0, 0}};  // [parity][tile]
       bool ok = true;
-      for (int it = blockIdx.x; it < items && ok; it += gridDim.x) {
+      for (int it = LENS ? 0u : blockIdx.x; it < (LENS ? mine : items) && ok; it += (LENS ? 1u : gridDim.x)) {
         const Item I = item_of(it);
         if (I.tiles == 0) continue;
         const int qb = c & 1;
@@ -389,7 +498,7 @@ __global__ void __launch_bounds__(F_THREADS, 1)
         bool mine, ragged;  // ragged: the sequence's last block is not full
       };
       auto load = [&](Slot k) {
-        for (; k.it < items; k.it += gridDim.x) {
+        for (; k.it < (LENS ? mine : items); k.it += (LENS ? 1u : gridDim.x)) {
           const Item I = item_of(k.it);
           k.tiles = I.tiles;
           k.kvs = I.kvs;
@@ -407,7 +516,7 @@ __global__ void __launch_bounds__(F_THREADS, 1)
           if (k.kvs == 2) k.mine = !k.mine;
           return k;
         }
-        k.it += gridDim.x;
+        k.it += (LENS ? 1u : gridDim.x);
         ++k.c;
         return load(k);
       };
@@ -415,7 +524,7 @@ __global__ void __launch_bounds__(F_THREADS, 1)
       auto wait = [&](uint64_t* bar, uint32_t parity) { return ok = ok && thread_wait(bar, parity & 1, err, VK_DEV_TIMEOUT_MMA); };
       // Lets slots of the other tile go (each is waited for, so that no phase is missed).
       auto skip = [&](Slot& k) {
-        while (k.it < items && !k.mine && wait(&kv_ready[k.g % ST], k.g / ST)) {
+        while (k.it < (LENS ? mine : items) && !k.mine && wait(&kv_ready[k.g % ST], k.g / ST)) {
           umma_commit(&kv_empty[k.g % ST]);
           k = next(k);
         }
@@ -423,7 +532,7 @@ __global__ void __launch_bounds__(F_THREADS, 1)
       // S of this tile's n-th block, once its last S has been read
       uint32_t uses[2] = {0, 0};  // of the tile's two query buffers
       auto issue_s = [&](const Slot& k, uint32_t n) {
-        if (k.it >= items || !wait(&kv_ready[k.g % ST], k.g / ST)) return;
+        if (k.it >= (LENS ? mine : items) || !wait(&kv_ready[k.g % ST], k.g / ST)) return;
         if (k.j < k.kvs) wait(&q_full[(k.c & 1) * 2 + t], k.c & 1 ? uses[1]++ : uses[0]++);
         if (n > 0) wait(&s_free[t], n - 1);
         if (!ok) return;
@@ -437,18 +546,18 @@ __global__ void __launch_bounds__(F_THREADS, 1)
                    smem_desc_k16(smem_u32(sMask + (a.kv_lens != nullptr ? k.g % ST : 0) * EXT_B)), idS, 1u);
         umma_commit(&s_full[t]);
       };
-      Slot k = load(Slot{static_cast<int>(blockIdx.x), 0, 1, 0, 0, 0, 0, false, false});
+      Slot k = load(Slot{static_cast<int>(LENS ? 0u : blockIdx.x), 0, 1, 0, 0, 0, 0, false, false});
       // Tile 1 starts when tile 0 is about to take its exponentials: half a
       // block apart, the two share MUFU in turn (in step they took 3600 cycles
       // for a block of both, 2048 of them MUFU's).
-      if (t == 1 && k.it < items) wait(started, 0);
+      if (t == 1 && k.it < (LENS ? mine : items)) wait(started, 0);
       skip(k);
       issue_s(k, 0);
-      for (uint32_t n = 0; ok && k.it < items; ++n) {
+      for (uint32_t n = 0; ok && k.it < (LENS ? mine : items); ++n) {
         // The next S goes first where it needs at most the slot after the next:
         // further on, the ring would wait for this block's.
         Slot b = next(k);
-        const bool near = b.it < items && (b.mine || b.kvs == 2);
+        const bool near = b.it < (LENS ? mine : items) && (b.mine || b.kvs == 2);
         if (near) {
           skip(b);
           issue_s(b, n + 1);
@@ -477,7 +586,7 @@ __global__ void __launch_bounds__(F_THREADS, 1)
   } else if (warp == 2 && a.kv_lens != nullptr) {
     uint32_t g = 0;
     bool ok = true;
-    for (int it = blockIdx.x; it < items && ok; it += gridDim.x) {
+    for (int it = LENS ? 0u : blockIdx.x; it < (LENS ? mine : items) && ok; it += (LENS ? 1u : gridDim.x)) {
       const Item I = item_of(it);
       if (I.tiles == 0) continue;
       for (int j = 0; j < I.nb; ++j, ++g) {  // (with lengths, an item streams one sequence)
@@ -508,7 +617,7 @@ __global__ void __launch_bounds__(F_THREADS, 1)
       owed = -1;
     };
     bool ok = true;
-    for (int it = blockIdx.x; it < items && ok && t < tpi; it += gridDim.x) {
+    for (int it = LENS ? 0u : blockIdx.x; it < (LENS ? mine : items) && ok && t < tpi; it += (LENS ? 1u : gridDim.x)) {
       const Item I = item_of(it);
       const int bh = t ? I.bh[1] : I.bh[0], q0 = t ? I.q0[1] : I.q0[0], row = q0 + trow;
       const int b = by_batch(bh), h = bh - b * a.heads;
@@ -633,14 +742,16 @@ constexpr size_t B_SMEM = 1024 + TILE_B * (4 + 2 * ST) + B_EXTRA + 512;
 // DQ: own rows are queries (own1 = q, own2 = d_out), streamed ones keys
 // (k, v), acc = dq.  Otherwise own rows are keys (k, v), streamed ones queries
 // (q, d_out), acc = dv, dk.
-template <bool DQ>
+template <bool DQ, bool LENS>
 __global__ void __launch_bounds__(B_THREADS, 1)
     k_attn_backward_tc(const __grid_constant__ CUtensorMap tmO1, const __grid_constant__ CUtensorMap tmO2,
                        const __grid_constant__ CUtensorMap tmS1, const __grid_constant__ CUtensorMap tmS2,
                        const __grid_constant__ CUtensorMap tmOut, const __grid_constant__ CUtensorMap tmG1,
                        const __grid_constant__ CUtensorMap tmG2, AttnShape a, const float* __restrict__ lse, float* delta,
-                       HeadsView g1, HeadsView g2, int items, int per_head, FastDiv by_head, FastDiv by_batch, int* err) {
+                       HeadsView g1, HeadsView g2, int base, int count, int per_head, FastDiv by_head, FastDiv by_batch,
+                       int* err) {
   extern __shared__ uint8_t smem_raw[];
+  __shared__ ItemList<LENS> list;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sOwn = smem;  // [item parity][own1, own2], then the item's output on its way out
   uint8_t* s1 = smem + 4 * TILE_B;
@@ -674,17 +785,27 @@ __global__ void __launch_bounds__(B_THREADS, 1)
   struct Item {
     int it, bh, r0, own, len, nb;  // own and streamed rows of the sequence, blocks
   };
-  // The first item from `it` on, in this CTA's steps, that has own rows and
-  // something to stream (it >= items: none); skipped(I) sees those before it.
+  // This CTA's items are the list's, or every gridDim.x-th one below `items`.
+  // seek: the one from `it` on that has own rows and something to stream
+  // (it >= items: none); skipped(I) sees those before it.
+  int items = count;
   auto seek = [&](int it, auto skipped) {
     Item I{};
-    for (; it < items; it += gridDim.x) {
-      I.bh = by_head(it);
-      I.r0 = (it - I.bh * per_head) * TR;
-      const int b = by_batch(I.bh);
-      const int nq = seq_len(a.q_lens, b, a.nq), nk = seq_len(a.kv_lens, b, a.nk);
-      I.own = DQ ? nq : nk;
-      I.len = DQ ? nk : nq;
+    for (; it < items; it += (LENS ? 1u : gridDim.x)) {
+      if constexpr (LENS) {
+        const int4 e = list.item[it];
+        I.bh = e.x;
+        I.r0 = e.y;
+        I.own = e.z;
+        I.len = e.w;
+      } else {
+        I.bh = by_head(it);
+        I.r0 = (it - I.bh * per_head) * TR;
+        const int b = by_batch(I.bh);
+        const int nq = seq_len(a.q_lens, b, a.nq), nk = seq_len(a.kv_lens, b, a.nk);
+        I.own = DQ ? nq : nk;
+        I.len = DQ ? nk : nq;
+      }
       I.nb = I.r0 < I.own ? (I.len + TR - 1) / TR : 0;
       if (I.nb > 0) break;
       skipped(I);
@@ -733,6 +854,14 @@ __global__ void __launch_bounds__(B_THREADS, 1)
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
+  if constexpr (LENS) {
+    const int32_t *own_lens = DQ ? a.q_lens : a.kv_lens, *other_lens = DQ ? a.kv_lens : a.q_lens;
+    const int total_other = DQ ? a.nk : a.nq;
+    items = list.build(a, own_lens, total_own, other_lens, total_other, TR, per_head, base, count, [&](int bh, int n) {
+      const int b = bh / a.heads;
+      return make_int4(bh, n * TR, seq_len(own_lens, b, total_own), seq_len(other_lens, b, total_other));
+    });
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -744,7 +873,7 @@ __global__ void __launch_bounds__(B_THREADS, 1)
     uint32_t sent = 0, owns = 0;  // how many of them are loaded or on their way
     bool ok = true;
     const float inv_scale = 1.0f / a.scale;
-    for (Item I = seek(blockIdx.x, nothing); ok && I.it < items; I = seek(I.it + gridDim.x, nothing), ++c) {
+    for (Item I = seek(LENS ? 0u : blockIdx.x, nothing); ok && I.it < items; I = seek(I.it + (LENS ? 1u : gridDim.x), nothing), ++c) {
       const uint32_t ob = c & 1;
       const int b = by_batch(I.bh), h = I.bh - b * a.heads;
       if (c >= 2 && !(ok = warp_wait(&own_empty[ob], ((c >> 1) - 1) & 1, err, VK_DEV_TIMEOUT_PRODUCER))) break;
@@ -815,12 +944,12 @@ __global__ void __launch_bounds__(B_THREADS, 1)
         return Blk{I.it, 0, I.nb, c, I.it < items};
       };
       auto next = [&](Blk k) {
-        if (k.ok && ++k.j == k.nb) k = load(k.it + gridDim.x, k.c + 1);
+        if (k.ok && ++k.j == k.nb) k = load(k.it + (LENS ? 1u : gridDim.x), k.c + 1);
         return k;
       };
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity) { return ok = ok && thread_wait(bar, parity & 1, err, VK_DEV_TIMEOUT_MMA); };
-      Blk b0 = load(blockIdx.x, 0);
+      Blk b0 = load(LENS ? 0u : blockIdx.x, 0);
       if (warp == 1) {
         auto product = [&](uint32_t col, const uint8_t* own, const uint8_t* streamed, uint32_t st, int ones) {
           tc_fence_after();
@@ -904,7 +1033,7 @@ __global__ void __launch_bounds__(B_THREADS, 1)
   } else if (warp == 2 && (DQ ? a.kv_lens : a.q_lens) != nullptr) {
     uint32_t n = 0;
     bool ok = true;
-    for (Item I = seek(blockIdx.x, nothing); ok && I.it < items; I = seek(I.it + gridDim.x, nothing))
+    for (Item I = seek(LENS ? 0u : blockIdx.x, nothing); ok && I.it < items; I = seek(I.it + (LENS ? 1u : gridDim.x), nothing))
       for (int j = 0; j < I.nb; ++j, ++n) {
         if (!(ok = warp_wait(&st_full[n % ST], (n / ST) & 1, err, VK_DEV_TIMEOUT_OTHER))) break;
         if (I.len - j * TR < TR) zero_tail(s1 + n % ST * TILE_B, s2 + n % ST * TILE_B, I.len - j * TR, lane);
@@ -951,10 +1080,10 @@ __global__ void __launch_bounds__(B_THREADS, 1)
       if (row < total_own) delta[at] = row < I.own ? dl : 0.0f;
       return true;
     };
-    Item I = seek(blockIdx.x, skipped);
+    Item I = seek(LENS ? 0u : blockIdx.x, skipped);
     bool ok = !DQ || I.it >= items || row_delta(I, 0);
     for (uint32_t c = 0; ok && I.it < items; ++c) {
-      const Item N = seek(I.it + gridDim.x, skipped);
+      const Item N = seek(I.it + (LENS ? 1u : gridDim.x), skipped);
       if (DQ && N.it < items && !(ok = row_delta(N, c + 1))) break;
       // the item's accumulators to memory, staged over its own tiles (every product is done with them)
       if (!(ok = warp_wait(&acc_full[c & 1], (c >> 1) & 1, err, VK_DEV_TIMEOUT_EPILOGUE))) break;
@@ -985,10 +1114,10 @@ __global__ void __launch_bounds__(B_THREADS, 1)
     const uint32_t tdp = tmem + COL_DP + (DQ ? grp * TR : 0) + lanes;
     const float sl2 = a.scale * LOG2E;
     const int trow = quad * 32 + lane;
-    Item I = seek(blockIdx.x, nothing);
+    Item I = seek(LENS ? 0u : blockIdx.x, nothing);
     uint32_t n0 = 0, c = 0;  // blocks and items before this one
     bool ok = true;
-    for (; ok && I.it < items; n0 += I.nb, ++c, I = seek(I.it + gridDim.x, nothing)) {
+    for (; ok && I.it < items; n0 += I.nb, ++c, I = seek(I.it + (LENS ? 1u : gridDim.x), nothing)) {
       float2 shift2 = make_float2(0.0f, 0.0f), delta2 = shift2;
       bool fresh = true;  // this group has had no block of the item yet
       for (int j = (n0 ^ grp) & 1; j < I.nb; j += 2) {
@@ -1088,6 +1217,18 @@ bool heads_map(CUtensorMap* m, const HeadsView& v, int batch, int heads, int tok
   const uint32_t box[4] = {64, rows, 1, 1};
   return make_tmap_nd(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, v.p, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
+// One CTA per SM; with lengths a launch takes as many items as the lists hold.
+template <class F>
+cudaError_t over_items(int items, bool lens, F launch) {
+  const int sms = num_sms(), most = lens ? sms * LIST_MAX : items;
+  for (int base = 0; base < items; base += most) {
+    const int count = items - base < most ? items - base : most;
+    launch(base, count, count < sms ? count : sms);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
+}
 }  // namespace
 
 cudaError_t attention_forward_tc(const AttnShape& a, HeadsView q, HeadsView k, HeadsView v, HeadsView out, float* lse,
@@ -1096,22 +1237,24 @@ cudaError_t attention_forward_tc(const AttnShape& a, HeadsView q, HeadsView k, H
   if (!heads_map(&mq, q, a.batch, a.heads, a.nq) || !heads_map(&mk, k, a.batch, a.heads, a.nk) ||
       !heads_map(&mv, v, a.batch, a.heads, a.nk) || !heads_map(&mo, out, a.batch, a.heads, a.nq, 32))
     return cudaErrorInvalidValue;
-  const void* fn = reinterpret_cast<const void*>(k_attn_forward_tc);
-  const cudaError_t e = ensure_smem_limit(fn, static_cast<int>(F_SMEM));
+  const bool lens = a.q_lens != nullptr || a.kv_lens != nullptr;
+  auto kernel = lens ? k_attn_forward_tc<true> : k_attn_forward_tc<false>;
+  const cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(kernel), static_cast<int>(F_SMEM));
   if (e != cudaSuccess) return e;
   // Two query tiles share each K / V block; one where pairs would leave SMs idle.
   const int nt = (a.nq + TR - 1) / TR, bh = a.batch * a.heads;
   const int tpi = (nt + 1) / 2 * bh < num_sms() ? 1 : 2;
   int per_head = (nt + tpi - 1) / tpi, items = per_head * bh, mixed_from = items;
-  if (tpi == 2 && nt % 2 == 1 && a.q_lens == nullptr && a.kv_lens == nullptr) {
+  if (tpi == 2 && nt % 2 == 1 && !lens) {
     per_head = nt / 2;
     mixed_from = per_head * bh;
     items = mixed_from + (bh + 1) / 2;
   }
-  const int grid = items < num_sms() ? items : num_sms();
-  k_attn_forward_tc<<<grid, F_THREADS, F_SMEM, s>>>(mq, mk, mv, mo, a, out, lse, items, per_head, mixed_from,
-                                                     FastDiv(per_head > 0 ? per_head : 1), FastDiv(a.heads), tpi, err);
-  return cudaGetLastError();
+  const FastDiv by_head(per_head > 0 ? per_head : 1), by_batch(a.heads);
+  return over_items(items, lens, [&](int base, int count, int grid) {
+    kernel<<<grid, F_THREADS, F_SMEM, s>>>(mq, mk, mv, mo, a, out, lse, count, per_head, lens ? base : mixed_from, by_head,
+                                           by_batch, tpi, err);
+  });
 }
 
 cudaError_t attention_backward_tc(const AttnShape& a, HeadsView q, HeadsView k, HeadsView v, HeadsView out,
@@ -1123,18 +1266,23 @@ cudaError_t attention_backward_tc(const AttnShape& a, HeadsView q, HeadsView k, 
       !heads_map(&mo, out, a.batch, a.heads, a.nq) || !heads_map(&mdq, dq, a.batch, a.heads, a.nq, 32) ||
       !heads_map(&mdk, dk, a.batch, a.heads, a.nk, 32) || !heads_map(&mdv, dv, a.batch, a.heads, a.nk, 32))
     return cudaErrorInvalidValue;
-  cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(k_attn_backward_tc<true>), static_cast<int>(B_SMEM));
-  if (e == cudaSuccess) e = ensure_smem_limit(reinterpret_cast<const void*>(k_attn_backward_tc<false>), static_cast<int>(B_SMEM));
+  const bool lens = a.q_lens != nullptr || a.kv_lens != nullptr;
+  const int bh = a.batch * a.heads, qt = (a.nq + TR - 1) / TR, kt = (a.nk + TR - 1) / TR;
+  const FastDiv by_batch(a.heads);
+  auto dq_kernel = lens ? k_attn_backward_tc<true, true> : k_attn_backward_tc<true, false>;
+  auto dkdv_kernel = lens ? k_attn_backward_tc<false, true> : k_attn_backward_tc<false, false>;
+  cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(dq_kernel), static_cast<int>(B_SMEM));
+  if (e == cudaSuccess) e = ensure_smem_limit(reinterpret_cast<const void*>(dkdv_kernel), static_cast<int>(B_SMEM));
+  if (e == cudaSuccess)
+    e = over_items(qt * bh, lens, [&](int base, int count, int grid) {
+      dq_kernel<<<grid, B_THREADS, B_SMEM, s>>>(mq, mg, mk, mv, mo, mdq, mdq, a, lse, delta, dq, dq, base, count, qt,
+                                                FastDiv(qt), by_batch, err);
+    });
   if (e != cudaSuccess) return e;
-  const int bh = a.batch * a.heads, sms = num_sms();
-  const int qt = (a.nq + TR - 1) / TR, kt = (a.nk + TR - 1) / TR;
-  k_attn_backward_tc<true><<<qt * bh < sms ? qt * bh : sms, B_THREADS, B_SMEM, s>>>(
-      mq, mg, mk, mv, mo, mdq, mdq, a, lse, delta, dq, dq, qt * bh, qt, FastDiv(qt), FastDiv(a.heads), err);
-  e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
-  k_attn_backward_tc<false><<<kt * bh < sms ? kt * bh : sms, B_THREADS, B_SMEM, s>>>(
-      mk, mv, mq, mg, mo, mdv, mdk, a, lse, delta, dv, dk, kt * bh, kt, FastDiv(kt), FastDiv(a.heads), err);
-  return cudaGetLastError();
+  return over_items(kt * bh, lens, [&](int base, int count, int grid) {
+    dkdv_kernel<<<grid, B_THREADS, B_SMEM, s>>>(mk, mv, mq, mg, mo, mdv, mdk, a, lse, delta, dv, dk, base, count, kt,
+                                                FastDiv(kt), by_batch, err);
+  });
 }
 
 }  // namespace vk

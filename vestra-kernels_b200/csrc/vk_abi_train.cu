@@ -197,7 +197,13 @@ extern "C" int vk_attention_backward(vk_ctx* ctx, const vk_attention_shape* shap
     VK_TRY(heads_view(name, "d_out", d_out, shape->dtype, B, H, a.nq, D, 16, &vg));
     VK_TRY(floats_ok(name, "lse", lse));
     VK_TRY(apart(name, {vdq.p, vdk.p, vdv.p, delta}, {vq.p, vk_.p, vv.p, vo.p, vg.p, lse}));
-    if (bf16 && a.dim == 64)
+    // The tensor cores take dS rounded to bf16.  Over many scores that adds up
+    // to 1.4 times the error that the rounding of the results has by itself; of
+    // a few scores one alone can carry a row, at up to 2.6 times.  Few scores
+    // are launch latency either way (1 x 61 x 61 14 us on the device there, 23
+    // here, 22 from the caller), so they keep f32 throughout.
+    const bool few = static_cast<int64_t>(a.batch) * a.heads * a.nq <= 8192 / a.nk;
+    if (bf16 && a.dim == 64 && !few)
       return vk_cuda_status(attention_backward_tc(a, vq, vk_, vv, vo, lse, vg, vdq, vdk, vdv, delta, ctx->d_err, s), name);
     return vk_cuda_status(attention_backward_simt(a, bf16, vq, vk_, vv, vo, lse, vg, vdq, vdk, vdv, delta, s), name);
   });

@@ -208,12 +208,10 @@ __device__ __forceinline__ void mask_columns(uint32_t (&r)[128], int valid) {
     if (i >= valid) r[i] = 0xff800000u;
 }
 
-// 2^x for a pair of lanes: pair `i` of 16 goes to the FMA pipe where MASK says
-// so, the others to MUFU.
-template <uint32_t MASK>
-__device__ __forceinline__ float2 exp2_pair(float2 x, int i) {
-  return (MASK >> (i & 15)) & 1 ? exp2_poly2(x) : make_float2(ex2_approx(x.x), ex2_approx(x.y));
-}
+// 2^x, by MUFU.  (A quarter of the pairs as a polynomial on the FMA pipe: of
+// degree 4, 230 us against 238 for the forward pass of 64 images, but 2.7e-6
+// off, which the row sums carry into lse; of degree 5, 2e-7 off, 240 us.)
+__device__ __forceinline__ float2 exp2_pair(float2 x) { return make_float2(ex2_approx(x.x), ex2_approx(x.y)); }
 }  // namespace
 
 // ------------------------------------------------------------------ items
@@ -317,9 +315,6 @@ struct ItemList<false> {};
 // more MMA in the last block, a column of ones against a column of 0 and -inf.
 // (As selects in the warps it took as long as the block's exponentials.)
 namespace {
-// Pairs of columns (of each 16) whose exponentials go to the FMA pipe:
-// measured at 64 images, 298 us for none, 293 for 4, 309 for 6.
-constexpr uint32_t F_MASK = 0x1111u;
 constexpr uint32_t F_P = 256, F_O = 384;
 constexpr size_t F_SMEM = 1024 + TILE_B * (4 + 2 * ST) + (ST + 1) * EXT_B + 512;
 }  // namespace
@@ -675,8 +670,8 @@ __global__ void __launch_bounds__(F_THREADS, 1)
         float2 ps[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
         for (int i = 0; i < 64; ++i) {
-          const float2 p = exp2_pair<F_MASK>(
-              ffma2(make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), scale2, shift2), i);
+          const float2 p = exp2_pair(
+              ffma2(make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), scale2, shift2));
           ps[i & 1] = fadd2(ps[i & 1], p);
           r[i] = pack_bf16x2(p.x, p.y);  // (over scores that are done with)
         }
@@ -731,7 +726,6 @@ __global__ void __launch_bounds__(F_THREADS, 1)
 // columns each (bf16 hi + mid + lo, 24 bits) against ones: S becomes
 // S - lse / scale and dP becomes dP - delta for two more MMAs a block.
 namespace {
-constexpr uint32_t B_MASK = 0x0u;
 // TMEM: S [0, 128); dq: dP twice [128, 384), dS [384, 448), dq [448, 512);
 // dk/dv: dP [128, 256), P [256, 320), dS [320, 384), dv [384, 448), dk [448, 512)
 constexpr uint32_t COL_DP = 128, COL_P = 256, COL_ACC = 384;
@@ -1147,7 +1141,7 @@ __global__ void __launch_bounds__(B_THREADS, 1)
 #pragma unroll
           for (int i = 0; i < 64; ++i) {
             const float2 s = make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), f = make_float2(sl2, sl2);
-            const float2 e = exp2_pair<B_MASK>(DQ ? ffma2(s, f, shift2) : fmul2(s, f), i);
+            const float2 e = exp2_pair(DQ ? ffma2(s, f, shift2) : fmul2(s, f));
             p[2 * i] = e.x, p[2 * i + 1] = e.y;
           }
         }

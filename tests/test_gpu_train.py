@@ -202,6 +202,51 @@ def test_attention_without_queries_or_keys(vk):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("side", ["q", "kv"])
+def test_attention_lengths_of_one_side(vk, dtype, side):
+    """Lengths of the queries or of the keys alone, out of range ones among them: as if the others were full."""
+    t = TYPES[dtype]
+    b, h, nq, nk = 5, 3, 260, 300
+    q, k, v, _, _, _, _ = attention_case(t, b, h, nq, nk, 64, "token", False, 70)
+    g = make((b, h, nq, 64), t, gen(71))
+    n = nq if side == "q" else nk
+    some, full = lens([n, -3, 0, 131, n + 9]), lens([nk if side == "q" else nq] * b)
+    ql, kl = (some, None) if side == "q" else (None, some)
+    qf, kf = (some, full) if side == "q" else (full, some)
+    out, lse = run_forward(vk, q, k, v, ql, kl)
+    want, want_lse = run_forward(vk, q, k, v, qf, kf)
+    assert torch.equal(out, want) and torch.equal(lse, want_lse)
+    clamped = [n, 0, 0, 131, n]
+    plain, bound, _, _ = forward_reference(q, k, v, clamped if side == "q" else [nq] * b, clamped if side == "kv" else [nk] * b, 0.125)
+    within(out, plain, bound, "out")
+    got, all_of_it = run_backward(vk, q, k, v, out, lse, g, ql, kl), run_backward(vk, q, k, v, out, lse, g, qf, kf)
+    assert all(torch.equal(x, y) for x, y in zip(got, all_of_it))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_attention_of_empty_sequences_only(vk, dtype):
+    t = TYPES[dtype]
+    q, k, v, _, _, _, _ = attention_case(t, 3, 2, 200, 150, 64, "head", False, 72)
+    none = lens([0, 0, 0])
+    for ql, kl in ((none, none), (None, none), (none, None)):
+        out, lse = run_forward(vk, q, k, v, ql, kl)
+        assert (out == 0).all() and (lse == -math.inf).all()
+        assert all((x == 0).all() for x in run_backward(vk, q, k, v, out, lse, q, ql, kl))
+
+
+def test_attention_of_a_sequence_by_itself(vk):
+    """A sequence of a padded batch has the same bits whatever the others' lengths are."""
+    q, k, v, _, _, _, _ = attention_case(torch.bfloat16, 6, 4, 700, 700, 64, "token", False, 73)
+    g = make((6, 4, 700, 64), torch.bfloat16, gen(74))
+    results = []
+    for others in ([700, 300, 1, 0, 513], [0, 0, 650, 700, 129], [400] * 5):
+        n = lens([450] + others)
+        out, lse = run_forward(vk, q, k, v, n, n)
+        results.append([x[0] for x in (out, lse, *run_backward(vk, q, k, v, out, lse, g, n, n))])
+    assert all(torch.equal(a, b) for r in results[1:] for a, b in zip(results[0], r))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_attention_scores_that_grow(vk, dtype):
     """Scores of very different size along the keys (each block outgrows the last by far), and a scale of its own."""
     d, n, m = 64, 150, 700

@@ -667,20 +667,30 @@ def synchronize(device: int | None = None) -> None:
             own[0].synchronize()
 
 
-def _dtype_code(t, name):
-    import torch
+_I32, _I64 = 2, 3  # element types of lengths and positions, beside DTYPE_F32 and DTYPE_BF16
+_TYPE_NAMES = ("float32", "bfloat16", "int32", "int64")
+_codes = {}  # torch's element types: their codes
 
-    if t.dtype == torch.float32:
-        return DTYPE_F32
-    if t.dtype == torch.bfloat16:
-        return DTYPE_BF16
-    raise TypeError(f"{name} must be float32 or bfloat16, got {t.dtype}")
+
+def _code(dtype) -> int:
+    code = _codes.get(dtype)
+    if code is None:
+        import torch
+
+        _codes.update({getattr(torch, name): i for i, name in enumerate(_TYPE_NAMES)})
+        code = _codes.get(dtype, -1)
+    return code
+
+
+def _dtype_code(t, name):
+    code = _code(t.dtype)
+    if code != DTYPE_F32 and code != DTYPE_BF16:
+        raise TypeError(f"{name} must be float32 or bfloat16, got {t.dtype}")
+    return code
 
 
 def _device_of(t, ctx):
-    import torch
-
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+    if not getattr(t, "is_cuda", False):
         raise TypeError("expected CUDA tensors")
     device = t.get_device()
     if ctx is not None and ctx.device != device:
@@ -700,12 +710,12 @@ def _view(t, name, shape, like):
     return ctypes.byref(_Heads(t.data_ptr(), b, h, n))
 
 
-def _flat(t, name, shape, dtype, device):
+def _flat(t, name, shape, code, device):
     """The pointer of a contiguous tensor of this shape and type, None for None."""
     if t is None:
         return None
-    if not t.is_cuda or t.get_device() != device or t.dtype != dtype:
-        raise TypeError(f"{name} must be {dtype} on cuda:{device}, got {t.dtype} on {t.device}")
+    if not t.is_cuda or t.get_device() != device or _code(t.dtype) != code:
+        raise TypeError(f"{name} must be {_TYPE_NAMES[code]} on cuda:{device}, got {t.dtype} on {t.device}")
     if t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
     if not t.is_contiguous():
@@ -714,14 +724,12 @@ def _flat(t, name, shape, dtype, device):
 
 
 def _attention_shape(q, k, scale, q_lens, kv_lens, device):
-    import torch
-
     if q.dim() != 4 or k.dim() != 4:
         raise ValueError("q and k must be [batch, heads, tokens, head_dim]")
     b, h, n, d = q.shape
     return _AttentionShape(_dtype_code(q, "q"), b, h, n, k.shape[2], d, d ** -0.5 if scale is None else scale,
-                           _flat(q_lens, "q_lens", (b,), torch.int32, device),
-                           _flat(kv_lens, "kv_lens", (b,), torch.int32, device))
+                           _flat(q_lens, "q_lens", (b,), _I32, device),
+                           _flat(kv_lens, "kv_lens", (b,), _I32, device))
 
 
 def attention_forward(q, k, v, out, lse, scale=None, q_lens=None, kv_lens=None, ctx: Context | None = None) -> None:
@@ -731,13 +739,12 @@ def attention_forward(q, k, v, out, lse, scale=None, q_lens=None, kv_lens=None, 
     with any order of the first three dimensions (a slice of a token-major QKV product transposed to it included);
     lse f32 [batch, heads, q_tokens].  q_lens / kv_lens: int32 CUDA tensors [batch], the valid tokens of each
     sequence.  Without a ctx the call runs on torch's current stream of the tensors' device."""
-    import torch
-
     dev = _device_of(q, ctx)
     shape = _attention_shape(q, k, scale, q_lens, kv_lens, dev)
-    qs, ks = tuple(q.shape), (*q.shape[:2], k.shape[2], q.shape[3])
+    b, h, n, d = qs = tuple(q.shape)
+    ks = (b, h, k.shape[2], d)
     _launch("vk_attention_forward", dev, ctx, ctypes.byref(shape), _view(q, "q", qs, q), _view(k, "k", ks, q),
-            _view(v, "v", ks, q), _view(out, "out", qs, q), _flat(lse, "lse", qs[:3], torch.float32, dev))
+            _view(v, "v", ks, q), _view(out, "out", qs, q), _flat(lse, "lse", (b, h, n), DTYPE_F32, dev))
 
 
 def attention_backward(q, k, v, out, lse, d_out, dq, dk, dv, scale=None, q_lens=None, kv_lens=None, delta=None,
@@ -746,19 +753,20 @@ def attention_backward(q, k, v, out, lse, d_out, dq, dk, dv, scale=None, q_lens=
 
     delta: f32 [batch, heads, q_tokens], scratch that receives the row sums of d_out * out; allocated on torch's
     current stream where there is no ctx (with a ctx, whose stream may be another one, it is the caller's)."""
-    import torch
-
     dev = _device_of(q, ctx)
     shape = _attention_shape(q, k, scale, q_lens, kv_lens, dev)
-    qs, ks = tuple(q.shape), (*q.shape[:2], k.shape[2], q.shape[3])
+    b, h, n, d = qs = tuple(q.shape)
+    ks = (b, h, k.shape[2], d)
     if delta is None:
         if ctx is not None:
             raise ValueError("with a ctx, delta is given by the caller")
-        delta = torch.empty(qs[:3], dtype=torch.float32, device=q.device)
+        import torch
+
+        delta = torch.empty((b, h, n), dtype=torch.float32, device=q.device)
     _launch("vk_attention_backward", dev, ctx, ctypes.byref(shape), _view(q, "q", qs, q), _view(k, "k", ks, q),
-            _view(v, "v", ks, q), _view(out, "out", qs, q), _flat(lse, "lse", qs[:3], torch.float32, dev),
+            _view(v, "v", ks, q), _view(out, "out", qs, q), _flat(lse, "lse", (b, h, n), DTYPE_F32, dev),
             _view(d_out, "d_out", qs, q), _view(dq, "dq", qs, q), _view(dk, "dk", ks, q), _view(dv, "dv", ks, q),
-            _flat(delta, "delta", qs[:3], torch.float32, dev))
+            _flat(delta, "delta", (b, h, n), DTYPE_F32, dev))
 
 
 def rope_axes(q, k, positions, sections, freq, q_out, k_out, inverse: bool = False, ctx: Context | None = None) -> None:
@@ -767,8 +775,6 @@ def rope_axes(q, k, positions, sections, freq, q_out, k_out, inverse: bool = Fal
     q, k (or None) [batch, heads, tokens, head_dim], f32 or bf16, any strides but the last; q_out, k_out may be q, k.
     positions int64 [tokens, axes], or [batch, tokens, axes] for each batch entry's own.  inverse=True turns back,
     which is the gradient."""
-    import torch
-
     dev = _device_of(q, ctx)
     if q.dim() != 4:
         raise ValueError("q must be [batch, heads, tokens, head_dim]")
@@ -776,7 +782,7 @@ def rope_axes(q, k, positions, sections, freq, q_out, k_out, inverse: bool = Fal
         raise ValueError(f"1 to {ROPE_MAX_AXES} sections, got {len(sections)}")
     b, h, n, d = qs = tuple(q.shape)
     own = positions.dim() == 3
-    pos = _flat(positions, "positions", (b, n, len(sections)) if own else (n, len(sections)), torch.int64, dev)
+    pos = _flat(positions, "positions", (b, n, len(sections)) if own else (n, len(sections)), _I64, dev)
     shape = _RopeAxesShape(_dtype_code(q, "q"), b, h, n, d, len(sections),
                            (_S * ROPE_MAX_AXES)(*sections), freq, int(inverse), int(own))
     if (k is None) != (k_out is None):
@@ -787,12 +793,10 @@ def rope_axes(q, k, positions, sections, freq, q_out, k_out, inverse: bool = Fal
 
 
 def _residual_norm_shape(stream, branch, gamma, beta, eps, scale, gate, post_gamma, post_beta, device):
-    import torch
-
     if stream.dim() != 3 or branch.dim() != 3:
         raise ValueError("the stream and the branch must be [groups, rows, cols]")
     g, t, c = stream.shape
-    f = torch.float32
+    f = DTYPE_F32
     return _ResidualNormShape(_dtype_code(stream, "the stream"), _dtype_code(branch, "the branch"), g, t, c, eps,
                               _flat(gamma, "gamma", (c,), f, device), _flat(beta, "beta", (c,), f, device),
                               _flat(scale, "scale", (c,), f, device), _flat(gate, "gate", (g, c), f, device),
@@ -808,14 +812,13 @@ def residual_norm_forward(x, branch, gamma, beta, eps, h, y, stats, scale=None, 
     x, h [groups, rows, cols] in the residual stream's type, branch, y the same shape in the branch's: (f32, f32),
     (f32, bf16) or (bf16, bf16), contiguous; vectors f32 [cols], gate f32 [groups, cols]; stats and post_stats f32
     [groups, rows, 2] receive (mean, 1 / sqrt(var + eps)).  h may be x."""
-    import torch
-
     dev = _device_of(x, ctx)
     shape = _residual_norm_shape(x, branch, gamma, beta, eps, scale, gate, post_gamma, post_beta, dev)
-    s, rows, f = x.shape, (*x.shape[:2], 2), torch.float32
-    _launch("vk_residual_norm_forward", dev, ctx, ctypes.byref(shape), _flat(x, "x", s, x.dtype, dev),
-            _flat(branch, "branch", s, branch.dtype, dev), _flat(h, "h", s, x.dtype, dev),
-            _flat(y, "y", s, branch.dtype, dev), _flat(stats, "stats", rows, f, dev),
+    g, t, c = s = tuple(x.shape)
+    rows, f = (g, t, 2), DTYPE_F32
+    _launch("vk_residual_norm_forward", dev, ctx, ctypes.byref(shape), _flat(x, "x", s, shape.stream_dtype, dev),
+            _flat(branch, "branch", s, shape.branch_dtype, dev), _flat(h, "h", s, shape.stream_dtype, dev),
+            _flat(y, "y", s, shape.branch_dtype, dev), _flat(stats, "stats", rows, f, dev),
             _flat(post_stats, "post_stats", rows, f, dev))
 
 
@@ -845,25 +848,26 @@ def residual_norm_backward(d_h, d_y, h, branch, stats, gamma, d_x, d_branch, d_g
     d_x may be d_h and d_branch may be d_y.  d_scale, d_gate, d_post_gamma and d_post_beta are given where their
     vectors are.  workspace: a uint8 tensor of residual_norm_workspace(...) bytes; allocated on torch's current
     stream where there is no ctx (with a ctx, whose stream may be another one, it is the caller's)."""
-    import torch
-
     dev = _device_of(h, ctx)
-    f = torch.float32
+    f = DTYPE_F32
     shape = _residual_norm_shape(h, branch, gamma, gamma, 0.0, scale, gate, post_gamma, post_beta, dev)
-    s, rows, vec = h.shape, (*h.shape[:2], 2), (h.shape[2],)
+    g, t, c = s = tuple(h.shape)
+    rows, vec = (g, t, 2), (c,)
     if workspace is None:
         if ctx is not None:
             raise ValueError("with a ctx, the workspace is given by the caller")
         need = _workspace_bytes(shape, dev, None)
+        import torch
+
         workspace = torch.empty(need, dtype=torch.uint8, device=h.device)
-    grads = _ResidualNormGrads(_flat(d_x, "d_x", s, h.dtype, dev), _flat(d_branch, "d_branch", s, branch.dtype, dev),
+    grads = _ResidualNormGrads(_flat(d_x, "d_x", s, shape.stream_dtype, dev), _flat(d_branch, "d_branch", s, shape.branch_dtype, dev),
                                _flat(d_gamma, "d_gamma", vec, f, dev), _flat(d_beta, "d_beta", vec, f, dev),
                                _flat(d_scale, "d_scale", vec, f, dev),
-                               _flat(d_gate, "d_gate", (s[0], s[2]), f, dev),
+                               _flat(d_gate, "d_gate", (g, c), f, dev),
                                _flat(d_post_gamma, "d_post_gamma", vec, f, dev),
                                _flat(d_post_beta, "d_post_beta", vec, f, dev))
-    _launch("vk_residual_norm_backward", dev, ctx, ctypes.byref(shape), _flat(d_h, "d_h", s, h.dtype, dev),
-            _flat(d_y, "d_y", s, branch.dtype, dev), _flat(h, "h", s, h.dtype, dev),
-            _flat(branch, "branch", s, branch.dtype, dev), _flat(stats, "stats", rows, f, dev),
+    _launch("vk_residual_norm_backward", dev, ctx, ctypes.byref(shape), _flat(d_h, "d_h", s, shape.stream_dtype, dev),
+            _flat(d_y, "d_y", s, shape.branch_dtype, dev), _flat(h, "h", s, shape.stream_dtype, dev),
+            _flat(branch, "branch", s, shape.branch_dtype, dev), _flat(stats, "stats", rows, f, dev),
             _flat(post_stats, "post_stats", rows, f, dev), ctypes.byref(grads), workspace.data_ptr(),
             workspace.numel() * workspace.element_size())

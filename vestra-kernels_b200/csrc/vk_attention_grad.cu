@@ -597,11 +597,14 @@ cudaError_t launch(void (*fn)(P...), int tiles, int split, int threads, int byte
 //
 // 8 (forward only) where the SM with the most rows has no more of them than
 // with 4: 36 heads of 865 tokens 214 against 247 us, but 12 heads of 3457, 1243
-// against 1180.  With fewer blocks than SMs the streamed side is split, to fill
-// the SMs, and beyond that while a share has two tiles: 18 heads of 197 tokens
-// 27 us as one block per 64 rows, 20 split by 2; 6 heads of 433, 41 and 31; 12
-// heads of 100 queries and 3000 keys, 231 and 61.  2 for a few rows: one query
-// of 3457 keys 266 us with 64 rows in one block, 209 with 32, 35 split by 8.
+// against 1180.  With fewer blocks than SMs the streamed side is split: up to
+// four blocks for three SMs (12 heads of 197 tokens backward 48 us split by 2,
+// 43 by 4), and up to two an SM where a share still has two tiles (18 heads of
+// 197 by 2, 49, by 4, 64) or where lengths make many blocks short (18 heads of
+// up to 197, 48 and 43).  6 heads of 433 tokens forward 41 us in one piece, 24
+// split by 4; 12 heads of 100 queries and 3000 keys, 231 and 58 by 8.  2 for a
+// few rows: one query of 3457 keys 266 us with 64 rows in one block, 209 with
+// 32, 31 split by 8.
 struct Layout {
   int rm, split;
 };
@@ -612,8 +615,9 @@ Layout layout_of(const AttnShape& a, int own, int streamed, bool wide) {
   const int rm = own <= 32 ? 2 : 4;
   const int tiles = (streamed + GT - 1) / GT;
   int split = 1;
+  const bool lens = a.q_lens != nullptr || a.kv_lens != nullptr;
   while (split < MAX_SPLIT && split * 2 <= tiles &&
-         (n4 * split * 2 <= sms || (n4 * split <= sms && split * 4 <= tiles)))
+         (n4 * split * 2 <= sms + sms / 3 || (n4 * split <= sms && (lens || split * 4 <= tiles))))
     split *= 2;
   return {rm, split};
 }

@@ -316,6 +316,9 @@ struct ItemList<false> {};
 // The columns past a sequence's end get their -inf from the tensor core: one
 // more MMA in the last block, a column of ones against a column of 0 and -inf.
 // (As selects in the warps it took as long as the block's exponentials.)
+//
+// 64 images of 865 tokens, 12 heads: 233 us, 630 TFLOP/s.  MUFU needs 124 of
+// them, the products 91; the two tiles' hand-overs take the rest.
 namespace {
 constexpr uint32_t F_P = 256, F_O = 384;
 constexpr size_t F_SMEM = 1024 + TILE_B * (4 + 2 * ST) + (ST + 1) * EXT_B + 512;
@@ -727,6 +730,11 @@ __global__ void __launch_bounds__(F_THREADS, 1)
 // than the operands do.  They enter the products instead, as three more
 // columns each (bf16 hi + mid + lo, 24 bits) against ones: S becomes
 // S - lse / scale and dP becomes dP - delta for two more MMAs a block.
+//
+// 64 images of 865 tokens, 12 heads: 602 us for both kernels, 610 TFLOP/s of
+// five products (855 of the seven that run).  MUFU is 42 to 55% busy, the
+// tensor pipe 41 to 45%: with one S, P and dS in tensor memory, which is full,
+// the groups wait for one another.
 namespace {
 // TMEM: S [0, 128); dq: dP twice [128, 384), dS [384, 448), dq [448, 512);
 // dk/dv: dP [128, 256), P [256, 320), dS [320, 384), dv [384, 448), dk [448, 512)

@@ -589,7 +589,8 @@ cudaError_t launch(void (*fn)(P...), int tiles, int split, int threads, int byte
   cfg.attrs = &cluster;
   cfg.numAttrs = split > 1 ? 1 : 0;
   e = cudaLaunchKernelEx(&cfg, fn, args...);
-  return e == cudaSuccess ? cudaGetLastError() : e;
+  const cudaError_t last = cudaGetLastError();
+  return e == cudaSuccess ? last : e;
 }
 
 // How a product of `own` rows per head with `streamed` ones is laid out: 16 rm
@@ -604,17 +605,29 @@ cudaError_t launch(void (*fn)(P...), int tiles, int split, int threads, int byte
 // up to 197, 48 and 43).  6 heads of 433 tokens forward 41 us in one piece, 24
 // split by 4; 12 heads of 100 queries and 3000 keys, 231 and 58 by 8.  2 for a
 // few rows: one query of 3457 keys 266 us with 64 rows in one block, 209 with
-// 32, 31 split by 8.
+// 32, 31 split by 8.  With one to two blocks an SM the streamed side is split
+// where that takes an eighth off the busiest SM's tiles: 12 heads of 865 tokens
+// forward 124 and 105, backward 413 and 336, but 36 heads of 433 (252 blocks)
+// 64 and 85 if split.
 struct Layout {
   int rm, split;
 };
 Layout layout_of(const AttnShape& a, int own, int streamed, bool wide) {
   const int sms = num_sms(), n8 = blocks_of(a, own, 128), n4 = blocks_of(a, own, 64);
   if (wide && n8 > sms && (n8 + sms - 1) / sms * 2 <= (n4 + sms - 1) / sms) return {8, 1};
-  if (n4 >= sms) return {4, 1};
-  const int rm = own <= 32 ? 2 : 4;
   const int tiles = (streamed + GT - 1) / GT;
   int split = 1;
+  if (n4 >= sms) {
+    if (n4 < 2 * sms) {
+      int most = 2 * tiles;  // tiles of the busiest SM
+      for (int s = 2; s <= MAX_SPLIT && s <= tiles; s *= 2) {
+        const int now = (n4 * s + sms - 1) / sms * ((tiles + s - 1) / s);
+        if (now * 8 <= most * 7) split = s, most = now;
+      }
+    }
+    return {4, split};
+  }
+  const int rm = own <= 32 ? 2 : 4;
   const bool lens = a.q_lens != nullptr || a.kv_lens != nullptr;
   while (split < MAX_SPLIT && split * 2 <= tiles &&
          (n4 * split * 2 <= sms + sms / 3 || (n4 * split <= sms && (lens || split * 4 <= tiles))))

@@ -215,6 +215,7 @@ struct Share {
 // values in its own block's memory, THREADS floats apart, and block `rank`
 // takes up some of the threads' elements from all blocks.
 constexpr int MAX_SPLIT = 8;
+constexpr int FEW = 4;  // queries that the form without tiles takes
 __device__ __forceinline__ float left_by(const float* mine, int rank) {
   float x;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(mapa_shared(mine, rank)));
@@ -376,6 +377,142 @@ __global__ void __launch_bounds__(16 * TX, 2)
     if (!live) acc[i].zero();  // (a sum of 0 has no values, but 0 * inf)
     acc[i].store(op + row * out.st, tx, inv);
   }
+}
+
+// A few queries: nothing is reused but q, which stays in registers, so keys and
+// values come straight from memory, D / L of a key's elements in each of L
+// lanes.  Every group of L lanes keeps a running maximum, sum and result of its
+// own keys; lanes, warps and the cluster's blocks join them in that order.
+// Bound by HBM: 96 heads of 1 query and 3457 keys, f32, @FEW@.
+template <class T, int D>
+__global__ void __launch_bounds__(256)
+    k_attn_forward_few(AttnShape a, int split, HeadsView q, HeadsView k, HeadsView v, HeadsView out,
+                       float* __restrict__ lse) {
+  constexpr int L = D >= 32 ? 8 : D / 4, V = D / (4 * L), KEYS = 32 / L, WARPS = 8;
+  __shared__ float part[WARPS][FEW][D + 2], whole[FEW][D + 2];  // maximum, sum, result
+  const int bh = blockIdx.x / split, rank = blockIdx.x - bh * split, b = bh / a.heads, h = bh - b * a.heads;
+  const int nq = seq_len(a.q_lens, b, a.nq), nk = nq > 0 ? seq_len(a.kv_lens, b, a.nk) : 0;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, lg = lane % L, kg = lane / L;
+  const int each = (nk + split - 1) / split, from = min(rank * each, nk), to = min(from + each, nk);
+  const T* qp = head_of<T>(q, b, h);
+  const T* kp = head_of<T>(k, b, h);
+  const T* vp = head_of<T>(v, b, h);
+  float4 qv[FEW][V], acc[FEW][V], kk[V], vv[V];
+  float m[FEW], l[FEW];
+#pragma unroll
+  for (int r = 0; r < FEW; ++r) {
+    m[r] = -INFINITY, l[r] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      acc[r][i] = qv[r][i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (r < nq) qv[r][i] = load4(qp + r * q.st + (i * L + lg) * 4);
+    }
+  }
+  auto fetch = [&](int key) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      kk[i] = vv[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (key < to) {
+        kk[i] = load4(kp + key * k.st + (i * L + lg) * 4);
+        vv[i] = load4(vp + key * v.st + (i * L + lg) * 4);
+      }
+    }
+  };
+  fetch(from + warp * KEYS + kg);
+  for (int k0 = from + warp * KEYS; k0 < to; k0 += WARPS * KEYS) {
+    const bool on = k0 + kg < to;
+    float4 kc[V], vc[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) kc[i] = kk[i], vc[i] = vv[i];
+    fetch(k0 + WARPS * KEYS + kg);
+#pragma unroll
+    for (int r = 0; r < FEW; ++r)
+      if (r < nq) {
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          s = fmaf(qv[r][i].x, kc[i].x, fmaf(qv[r][i].y, kc[i].y, fmaf(qv[r][i].z, kc[i].z, fmaf(qv[r][i].w, kc[i].w, s))));
+        s = lanes_sum<L>(s);
+        s = on ? s * a.scale : -INFINITY;
+        const float m_new = fmaxf(m[r], s), ref = m_new == -INFINITY ? 0.0f : m_new;
+        const float f = expf(m[r] - ref), p = expf(s - ref);
+        m[r] = m_new;
+        l[r] = fmaf(l[r], f, p);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          acc[r][i].x = fmaf(acc[r][i].x, f, p * vc[i].x), acc[r][i].y = fmaf(acc[r][i].y, f, p * vc[i].y);
+          acc[r][i].z = fmaf(acc[r][i].z, f, p * vc[i].z), acc[r][i].w = fmaf(acc[r][i].w, f, p * vc[i].w);
+        }
+      }
+  }
+#pragma unroll
+  for (int r = 0; r < FEW; ++r) {
+#pragma unroll
+    for (int o = L; o < 32; o *= 2) {
+      const float tm = __shfl_xor_sync(0xffffffffu, m[r], o), m_new = fmaxf(m[r], tm);
+      const float ref = m_new == -INFINITY ? 0.0f : m_new, f = expf(m[r] - ref), tf = expf(tm - ref);
+      m[r] = m_new;
+      l[r] = l[r] * f + __shfl_xor_sync(0xffffffffu, l[r], o) * tf;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        acc[r][i].x = acc[r][i].x * f + __shfl_xor_sync(0xffffffffu, acc[r][i].x, o) * tf;
+        acc[r][i].y = acc[r][i].y * f + __shfl_xor_sync(0xffffffffu, acc[r][i].y, o) * tf;
+        acc[r][i].z = acc[r][i].z * f + __shfl_xor_sync(0xffffffffu, acc[r][i].z, o) * tf;
+        acc[r][i].w = acc[r][i].w * f + __shfl_xor_sync(0xffffffffu, acc[r][i].w, o) * tf;
+      }
+    }
+    if (kg == 0) {
+      float* mine = part[warp][r];
+      if (lg == 0) mine[0] = m[r], mine[1] = l[r];
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        float* d = mine + 2 + (i * L + lg) * 4;
+        d[0] = acc[r][i].x, d[1] = acc[r][i].y, d[2] = acc[r][i].z, d[3] = acc[r][i].w;
+      }
+    }
+  }
+  __syncthreads();
+  const int r = threadIdx.x / D, d = threadIdx.x - r * D;
+  float top = -INFINITY, sum = 0.0f, total = 0.0f;
+  auto join = [&](const float (&ms)[8], const float (&ls)[8], const float (&xs)[8]) {
+    top = -INFINITY, sum = total = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) top = fmaxf(top, ms[w]);
+    const float ref = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      const float f = expf(ms[w] - ref);
+      sum = fmaf(ls[w], f, sum);
+      total = fmaf(xs[w], f, total);
+    }
+  };
+  static_assert(WARPS == 8 && MAX_SPLIT == 8 && FEW * 64 <= 256, "an element per thread, eight parts each");
+  if (r < FEW) {
+    float ms[8], ls[8], xs[8];
+#pragma unroll
+    for (int w = 0; w < 8; ++w) ms[w] = part[w][r][0], ls[w] = part[w][r][1], xs[w] = part[w][r][2 + d];
+    join(ms, ls, xs);
+    if (split > 1) {
+      whole[r][2 + d] = total;
+      if (d == 0) whole[r][0] = top, whole[r][1] = sum;
+    }
+  }
+  if (split > 1) {
+    cluster_sync();
+    if (r < FEW && rank == 0) {
+      float ms[8], ls[8], xs[8];
+      left_by_all(ms, &whole[r][0], split, -INFINITY);
+      left_by_all(ls, &whole[r][1], split, 0.0f);
+      left_by_all(xs, &whole[r][2 + d], split, 0.0f);
+      join(ms, ls, xs);
+    }
+    cluster_sync();  // until then the others' memory is read
+    if (rank != 0) return;
+  }
+  if (r >= FEW || r >= a.nq) return;
+  const bool live = r < nq && sum != 0.0f;
+  store1(head_of<T>(out, b, h) + r * out.st + d, live ? total / sum : 0.0f);
+  if (d == 0) lse[static_cast<size_t>(bh) * a.nq + r] = live ? top + logf(sum) : -INFINITY;
 }
 
 // dq and delta: a block owns 16 RM queries and streams the keys.
@@ -638,6 +775,13 @@ Layout layout_of(const AttnShape& a, int own, int streamed, bool wide) {
 template <class T, int D>
 cudaError_t forward(const AttnShape& a, HeadsView q, HeadsView k, HeadsView v, HeadsView out, float* lse,
                     cudaStream_t s) {
+  if (a.nq <= FEW) {
+    // four blocks an SM, 64 keys a block at least
+    const int heads = a.batch * a.heads;
+    int split = 1;
+    while (split < MAX_SPLIT && static_cast<int64_t>(heads) * split * 2 <= 4 * num_sms() && split * 128 <= a.nk) split *= 2;
+    return launch(k_attn_forward_few<T, D>, heads, split, 256, 0, s, a, split, q, k, v, out, lse);
+  }
   const Layout l = layout_of(a, a.nq, a.nk, true);
   const int tiles = blocks_of(a, a.nq, 16 * l.rm);
   if (l.rm == 8)

@@ -88,9 +88,10 @@ ATTENTION = [
     ("bf16", 2, 2, 300, 1, 64, "token", False), ("bf16", 2, 2, 1, 1000, 64, "head", False), ("bf16", 1, 12, 865, 865, 64, "token", False),
     ("bf16", 6, 3, 200, 200, 64, "head", True), ("bf16", 40, 12, 140, 140, 64, "token", True), ("bf16", 1, 1, 3457, 3457, 64, "head", False),
     ("bf16", 17, 11, 100, 130, 64, "token", False), ("bf16", 15, 11, 300, 70, 64, "head", False), ("bf16", 16, 10, 257, 257, 64, "head", False),
-    # up to four queries, with their keys split and not
+    # few queries, with their keys split and not
     ("f32", 3, 5, 4, 1000, 64, "token", True), ("f32", 2, 40, 2, 333, 32, "head", False), ("bf16", 4, 30, 3, 500, 16, "head", True),
     ("f32", 6, 100, 4, 70, 64, "token", True), ("bf16", 2, 3, 1, 129, 8, "token", False), ("f32", 5, 130, 3, 31, 16, "head", True),
+    ("f32", 4, 3, 15, 700, 64, "token", True), ("f32", 30, 6, 16, 90, 32, "head", True), ("f32", 1, 2, 9, 2000, 64, "head", False),
     # more sequences than are put in order, and more items than a launch takes; the latter alone
     ("bf16", 140, 20, 900, 870, 64, "token", True), ("bf16", 127, 24, 900, 300, 64, "head", True), ("bf16", 128, 1, 300, 500, 64, "token", True),
     ("bf16", 2, 3, 70, 90, 32, "head", True), ("bf16", 1, 2, 33, 40, 16, "token", False), ("bf16", 1, 2, 33, 40, 8, "head", False),

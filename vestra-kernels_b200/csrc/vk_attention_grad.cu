@@ -215,7 +215,7 @@ struct Share {
 // values in its own block's memory, THREADS floats apart, and block `rank`
 // takes up some of the threads' elements from all blocks.
 constexpr int MAX_SPLIT = 8;
-constexpr int FEW = 4;  // queries that the form without tiles takes
+constexpr int FEW = 4, FEW_MAX = 12;  // queries of a block without tiles, and of a sequence that goes that way
 __device__ __forceinline__ float left_by(const float* mine, int rank) {
   float x;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(mapa_shared(mine, rank)));
@@ -383,24 +383,28 @@ __global__ void __launch_bounds__(16 * TX, 2)
 // values come straight from memory, D / L of a key's elements in each of L
 // lanes.  Every group of L lanes keeps a running maximum, sum and result of its
 // own keys; lanes, warps and the cluster's blocks join them in that order.
-// Bound by HBM: 96 heads of 1 query and 3457 keys, f32, @FEW@.
-template <class T, int D>
+// Bound by HBM: 1536 heads of one query and 3457 keys, f32, 415 us, the copy
+// rate (2618 in tiles of 64 rows); 96 heads 55 us (227).  Four queries a block
+// take what the exponentials cost: 96 heads of 7 queries and 3000 keys 139 us
+// (202), of 16 270 (204 in tiles, so 12 is the most).
+template <class T, int D, int ROWS>
 __global__ void __launch_bounds__(256)
     k_attn_forward_few(AttnShape a, int split, HeadsView q, HeadsView k, HeadsView v, HeadsView out,
                        float* __restrict__ lse) {
   constexpr int L = D >= 32 ? 8 : D / 4, V = D / (4 * L), KEYS = 32 / L, WARPS = 8;
-  __shared__ float part[WARPS][FEW][D + 2], whole[FEW][D + 2];  // maximum, sum, result
-  const int bh = blockIdx.x / split, rank = blockIdx.x - bh * split, b = bh / a.heads, h = bh - b * a.heads;
-  const int nq = seq_len(a.q_lens, b, a.nq), nk = nq > 0 ? seq_len(a.kv_lens, b, a.nk) : 0;
+  __shared__ float part[WARPS][ROWS][D + 2], whole[ROWS][D + 2];  // maximum, sum, result
+  const int tiles = (a.nq + ROWS - 1) / ROWS, tile = blockIdx.x / split, rank = blockIdx.x - tile * split;
+  const int bh = tile / tiles, r0 = (tile - bh * tiles) * ROWS, b = bh / a.heads, h = bh - b * a.heads;
+  const int nq = min(max(seq_len(a.q_lens, b, a.nq) - r0, 0), ROWS), nk = nq > 0 ? seq_len(a.kv_lens, b, a.nk) : 0;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, lg = lane % L, kg = lane / L;
   const int each = (nk + split - 1) / split, from = min(rank * each, nk), to = min(from + each, nk);
-  const T* qp = head_of<T>(q, b, h);
+  const T* qp = head_of<T>(q, b, h) + r0 * q.st;
   const T* kp = head_of<T>(k, b, h);
   const T* vp = head_of<T>(v, b, h);
-  float4 qv[FEW][V], acc[FEW][V], kk[V], vv[V];
-  float m[FEW], l[FEW];
+  float4 qv[ROWS][V], acc[ROWS][V], kk[V], vv[V];
+  float m[ROWS], l[ROWS];
 #pragma unroll
-  for (int r = 0; r < FEW; ++r) {
+  for (int r = 0; r < ROWS; ++r) {
     m[r] = -INFINITY, l[r] = 0.0f;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -426,7 +430,7 @@ __global__ void __launch_bounds__(256)
     for (int i = 0; i < V; ++i) kc[i] = kk[i], vc[i] = vv[i];
     fetch(k0 + WARPS * KEYS + kg);
 #pragma unroll
-    for (int r = 0; r < FEW; ++r)
+    for (int r = 0; r < ROWS; ++r)
       if (r < nq) {
         float s = 0.0f;
 #pragma unroll
@@ -446,7 +450,7 @@ __global__ void __launch_bounds__(256)
       }
   }
 #pragma unroll
-  for (int r = 0; r < FEW; ++r) {
+  for (int r = 0; r < ROWS; ++r) {
 #pragma unroll
     for (int o = L; o < 32; o *= 2) {
       const float tm = __shfl_xor_sync(0xffffffffu, m[r], o), m_new = fmaxf(m[r], tm);
@@ -486,8 +490,8 @@ __global__ void __launch_bounds__(256)
       total = fmaf(xs[w], f, total);
     }
   };
-  static_assert(WARPS == 8 && MAX_SPLIT == 8 && FEW * 64 <= 256, "an element per thread, eight parts each");
-  if (r < FEW) {
+  static_assert(WARPS == 8 && MAX_SPLIT == 8 && ROWS * D <= 256, "an element per thread, eight parts each");
+  if (r < ROWS) {
     float ms[8], ls[8], xs[8];
 #pragma unroll
     for (int w = 0; w < 8; ++w) ms[w] = part[w][r][0], ls[w] = part[w][r][1], xs[w] = part[w][r][2 + d];
@@ -499,7 +503,7 @@ __global__ void __launch_bounds__(256)
   }
   if (split > 1) {
     cluster_sync();
-    if (r < FEW && rank == 0) {
+    if (r < ROWS && rank == 0) {
       float ms[8], ls[8], xs[8];
       left_by_all(ms, &whole[r][0], split, -INFINITY);
       left_by_all(ls, &whole[r][1], split, 0.0f);
@@ -509,10 +513,10 @@ __global__ void __launch_bounds__(256)
     cluster_sync();  // until then the others' memory is read
     if (rank != 0) return;
   }
-  if (r >= FEW || r >= a.nq) return;
+  if (r >= ROWS || r0 + r >= a.nq) return;
   const bool live = r < nq && sum != 0.0f;
-  store1(head_of<T>(out, b, h) + r * out.st + d, live ? total / sum : 0.0f);
-  if (d == 0) lse[static_cast<size_t>(bh) * a.nq + r] = live ? top + logf(sum) : -INFINITY;
+  store1(head_of<T>(out, b, h) + (r0 + r) * out.st + d, live ? total / sum : 0.0f);
+  if (d == 0) lse[static_cast<size_t>(bh) * a.nq + r0 + r] = live ? top + logf(sum) : -INFINITY;
 }
 
 // dq and delta: a block owns 16 RM queries and streams the keys.
@@ -775,12 +779,13 @@ Layout layout_of(const AttnShape& a, int own, int streamed, bool wide) {
 template <class T, int D>
 cudaError_t forward(const AttnShape& a, HeadsView q, HeadsView k, HeadsView v, HeadsView out, float* lse,
                     cudaStream_t s) {
-  if (a.nq <= FEW) {
+  if (a.nq <= FEW_MAX) {
     // four blocks an SM, 64 keys a block at least
-    const int heads = a.batch * a.heads;
+    const int tiles = blocks_of(a, a.nq, a.nq == 1 ? 1 : FEW);
     int split = 1;
-    while (split < MAX_SPLIT && static_cast<int64_t>(heads) * split * 2 <= 4 * num_sms() && split * 128 <= a.nk) split *= 2;
-    return launch(k_attn_forward_few<T, D>, heads, split, 256, 0, s, a, split, q, k, v, out, lse);
+    while (split < MAX_SPLIT && static_cast<int64_t>(tiles) * split * 2 <= 4 * num_sms() && split * 128 <= a.nk) split *= 2;
+    return a.nq == 1 ? launch(k_attn_forward_few<T, D, 1>, tiles, split, 256, 0, s, a, split, q, k, v, out, lse)
+                     : launch(k_attn_forward_few<T, D, FEW>, tiles, split, 256, 0, s, a, split, q, k, v, out, lse);
   }
   const Layout l = layout_of(a, a.nq, a.nk, true);
   const int tiles = blocks_of(a, a.nq, 16 * l.rm);

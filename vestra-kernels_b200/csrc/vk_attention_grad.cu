@@ -1,6 +1,7 @@
 // vk_attention_grad.cu -- attention with row statistics and its backward
 // pass on the CUDA cores: f32 elements (f32 arithmetic throughout), and bf16
-// elements of the head sizes the tensor-core kernels do not take.
+// elements of the head sizes the tensor-core kernels do not take, of one query
+// and of gradients of a few scores.
 //
 //   s_ij = scale q_i . k_j          lse_i = log sum_j exp s_ij
 //   p_ij = exp(s_ij - lse_i)        out_i = sum_j p_ij v_j

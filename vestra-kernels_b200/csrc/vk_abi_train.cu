@@ -206,7 +206,7 @@ extern "C" int vk_attention_backward(vk_ctx* ctx, const vk_attention_shape* shap
     // are launch latency either way (1 x 61 x 61 14 us on the device there, 23
     // here, 22 from the caller), so they keep f32 throughout.
     const bool few = static_cast<int64_t>(a.batch) * a.heads * a.nq <= 8192 / a.nk;
-    if (bf16 && a.dim == 64 && !few)
+    if (bf16 && a.dim == 64 && a.nq > 1 && !few)
       return vk_cuda_status(attention_backward_tc(a, vq, vk_, vv, vo, lse, vg, vdq, vdk, vdv, delta, ctx->d_err, s), name);
     return vk_cuda_status(attention_backward_simt(a, bf16, vq, vk_, vv, vo, lse, vg, vdq, vdk, vdv, delta, s), name);
   });

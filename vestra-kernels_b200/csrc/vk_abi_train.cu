@@ -204,7 +204,9 @@ extern "C" int vk_attention_backward(vk_ctx* ctx, const vk_attention_shape* shap
     // to 1.4 times the error that the rounding of the results has by itself; of
     // a few scores one alone can carry a row, at up to 2.6 times.  Few scores
     // are launch latency either way (1 x 61 x 61 14 us on the device there, 23
-    // here, 22 from the caller), so they keep f32 throughout.
+    // here, 22 from the caller), so they keep f32 throughout.  One query alone
+    // takes no tiles either: 12 heads of 3457 keys 44 us from the caller (78 on
+    // the tensor cores), 1536 heads 813 (1177).
     const bool few = static_cast<int64_t>(a.batch) * a.heads * a.nq <= 8192 / a.nk;
     if (bf16 && a.dim == 64 && a.nq > 1 && !few)
       return vk_cuda_status(attention_backward_tc(a, vq, vk_, vv, vo, lse, vg, vdq, vdk, vdv, delta, ctx->d_err, s), name);

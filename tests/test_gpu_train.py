@@ -238,6 +238,32 @@ def test_attention_of_empty_sequences_only(vk, dtype):
         assert all((x == 0).all() for x in run_backward(vk, q, k, v, out, lse, q, ql, kl))
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [1, 3])
+def test_attention_of_few_queries_captured(vk, dtype, n):
+    """A graph of the forms without tiles, replayed with other queries and lengths; keys past the lengths get zeros."""
+    t = TYPES[dtype]
+    q, k, v, _, _, _, _ = attention_case(t, 3, 4, n, 700, 64, "head", False, 75)
+    g, kl = make(q.shape, t, gen(76)), lens([700, 1, 300])
+
+    def both():
+        out, lse = run_forward(vk, q, k, v, None, kl)
+        return (out, lse, *run_backward(vk, q, k, v, out, lse, g, None, kl))
+
+    both()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = both()
+    q.copy_(make(q.shape, t, gen(77)))
+    kl.copy_(lens([0, 650, 2]))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(held, both()))
+    assert (held[3][0] == 0).all() and (held[4][2, :, 2:] == 0).all() and (held[1][0] == -math.inf).all()
+    want, bound, _, _ = forward_reference(q, k, v, [n] * 3, [0, 650, 2], 0.125)
+    within(held[0], want, bound, "out")
+
+
 def test_attention_of_a_sequence_by_itself(vk):
     """A sequence of a padded batch has the same bits whatever the others' lengths are."""
     q, k, v, _, _, _, _ = attention_case(torch.bfloat16, 6, 4, 700, 700, 64, "token", False, 73)

@@ -13,7 +13,8 @@
 // A block owns 16 RM rows (queries for the forward pass and dq, keys for dk
 // and dv) and streams the other side in tiles of 64, so every sum has one owner
 // and a fixed order: no atomics, the same bits every time.  The price is that
-// the backward pass computes s and dp twice (7 products instead of 5).
+// the backward pass computes s and dp twice (7 products instead of 5).  A few
+// queries go without tiles (the kernels named few).
 //
 // 16 x TX threads hold an RM x 64 / TX piece of each product.  Tiles are f32 in
 // shared memory with rows of D + 4 floats, which puts the rows that a warp
@@ -880,11 +881,11 @@ cudaError_t launch(void (*fn)(P...), int tiles, int split, int threads, int byte
 // 197 by 2, 49, by 4, 64) or where lengths make many blocks short (18 heads of
 // up to 197, 48 and 43).  6 heads of 433 tokens forward 41 us in one piece, 24
 // split by 4; 12 heads of 100 queries and 3000 keys, 231 and 58 by 8.  2 for a
-// few rows: one query of 3457 keys 266 us with 64 rows in one block, 209 with
-// 32, 31 split by 8.  With one to two blocks an SM the streamed side is split
-// where that takes an eighth off the busiest SM's tiles: 12 heads of 865 tokens
-// forward 124 and 105, backward 413 and 336, but 36 heads of 433 (252 blocks)
-// 64 and 85 if split.
+// few rows: 8 heads of 20 queries and 3000 keys of 32, 147 us with 64 rows in
+// one block, 20 with 32, split by 8.  With one to two blocks an SM the streamed
+// side is split where that takes an eighth off the busiest SM's tiles: 12 heads
+// of 865 tokens forward 124 and 105, backward 413 and 336, but 36 heads of 433
+// (252 blocks) 64 and 85 if split.
 struct Layout {
   int rm, split;
 };

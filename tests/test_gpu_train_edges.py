@@ -1,0 +1,54 @@
+"""The trainable block pieces where values are not finite, sides are short or a
+call comes first: what the header promises holds in every form that a call can
+take (few queries, tiles on the CUDA cores, tensor cores), and one form's
+results are another's.
+
+Tolerances are those of test_gpu_train.py, derived there."""
+import math
+
+import pytest
+import torch
+from test_gpu_train import TYPES, attention_case, gen, lens, make, run_backward, run_forward
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def vk():
+    import vestra_kernels
+
+    return vestra_kernels
+
+
+# dtype, sequences, heads, queries, keys, head_dim: every form of the backward pass
+FORMS = [
+    # few queries, the keys in one block and split
+    ("f32", 2, 3, 1, 300, 64), ("f32", 2, 3, 4, 70, 64), ("f32", 2, 3, 2, 900, 16), ("bf16", 2, 3, 1, 300, 64),
+    ("bf16", 2, 3, 1, 40, 8), ("bf16", 2, 2, 3, 200, 64), ("bf16", 2, 2, 4, 150, 64),
+    # tiles on the CUDA cores, split and not
+    ("f32", 2, 3, 20, 300, 32), ("f32", 2, 40, 130, 200, 64), ("bf16", 2, 2, 30, 50, 64), ("bf16", 2, 3, 70, 600, 32),
+    # tensor cores: one block, several, the last full and not
+    ("bf16", 2, 40, 100, 70, 64), ("bf16", 2, 3, 300, 385, 64), ("bf16", 2, 3, 256, 384, 64), ("bf16", 2, 30, 3, 200, 64),
+]
+
+
+@pytest.mark.parametrize("dtype,b,h,nq,nk,d", FORMS)
+@pytest.mark.parametrize("bad", [math.inf, math.nan])
+@pytest.mark.parametrize("where", ["d_out", "q"])
+def test_attention_gradients_past_the_lengths_are_zeros(vk, dtype, b, h, nq, nk, d, bad, where):
+    """A value that is not finite in a valid row of d_out or q (an overflowed gradient) leaves the rows past the
+    lengths zeros, and the other heads as they are without it."""
+    t = TYPES[dtype]
+    q, k, v, _, _, _, _ = attention_case(t, b, h, nq, nk, d, "head", False, 80)
+    g = make((b, h, nq, d), t, gen(81))
+    ql, kl = lens([nq, max(1, nq // 2)]), lens([max(1, nk - 9), nk // 3])
+    out, lse = run_forward(vk, q, k, v, ql, kl)
+    clean = run_backward(vk, q, k, v, out, lse, g, ql, kl)
+    (g if where == "d_out" else q)[0, 0, 0, 3] = bad
+    out, lse = run_forward(vk, q, k, v, ql, kl)
+    dq, dk, dv = run_backward(vk, q, k, v, out, lse, g, ql, kl)
+    for i in range(b):
+        assert (dq[i, :, int(ql[i]):] == 0).all()
+        assert (dk[i, :, int(kl[i]):] == 0).all() and (dv[i, :, int(kl[i]):] == 0).all()
+    for x, y in zip((dq, dk, dv), clean):
+        assert torch.equal(x[1:], y[1:]) and torch.equal(x[:1, 1:], y[:1, 1:])

@@ -757,10 +757,12 @@ __global__ void __launch_bounds__(256)
     for (int r = 0; r < ROWS; ++r)
       if (r < nq) {
         const float s = dot(qv[r], kc), dp = dot(gv[r], vc);
-        const float p = key < nk ? expf(fmaf(s, a.scale, -ref[r])) : 0.0f, ds = key < nk ? p * (dp - dl[r]) : 0.0f;
-        add(gvv, p, gv[r]);
-        add(gk, ds, qv[r]);
-        add(acc[r], ds, kc);
+        if (key < nk) {  // (as weights of 0, keys past the end would turn what is not finite in q or d_out into NaN)
+          const float p = expf(fmaf(s, a.scale, -ref[r])), ds = p * (dp - dl[r]);
+          add(gvv, p, gv[r]);
+          add(gk, ds, qv[r]);
+          add(acc[r], ds, kc);
+        }
       }
     if (key < to) {
 #pragma unroll

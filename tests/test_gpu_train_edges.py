@@ -8,7 +8,7 @@ import math
 
 import pytest
 import torch
-from test_gpu_train import TYPES, attention_case, gen, lens, make, run_backward, run_forward
+from test_gpu_train import TYPES, attention_case, backward_reference, forward_reference, gen, lens, make, run_backward, run_forward, within
 
 pytestmark = pytest.mark.gpu
 
@@ -52,3 +52,26 @@ def test_attention_gradients_past_the_lengths_are_zeros(vk, dtype, b, h, nq, nk,
         assert (dk[i, :, int(kl[i]):] == 0).all() and (dv[i, :, int(kl[i]):] == 0).all()
     for x, y in zip((dq, dk, dv), clean):
         assert torch.equal(x[1:], y[1:]) and torch.equal(x[:1, 1:], y[:1, 1:])
+
+
+@pytest.mark.parametrize("dtype,b,h,nq,nk,d", FORMS)
+@pytest.mark.parametrize("ragged", [False, True])
+def test_attention_gradients_of_scores_far_below_zero(vk, dtype, b, h, nq, nk, d, ragged):
+    """Scores so low that exp(-lse) is beyond f32: what a block reads past its keys must not count."""
+    t = TYPES[dtype]
+    q, k, v, _, _, _, _ = attention_case(t, b, h, nq, nk, d, "head", False, 86)
+    q, k = (q.abs() + 4).to(t), (-k.abs() - 4).to(t)
+    g = make((b, h, nq, d), t, gen(87))
+    scale = 8.0 / d  # (sums of d products near -23: -184 at any head size)
+    ql, kl = ([nq, max(1, nq // 2)], [max(1, nk - 9), max(1, nk // 3)]) if ragged else ([nq] * b, [nk] * b)
+    qt, kt = (lens(ql), lens(kl)) if ragged else (None, None)
+    out, lse = run_forward(vk, q, k, v, qt, kt, scale=scale)
+    want, bound, lse_want, lse_bound = forward_reference(q, k, v, ql, kl, scale)
+    within(out, want, bound, "out")
+    live = lse_want != -math.inf
+    assert lse_want[live].max() < -95
+    within(lse[live], lse_want[live], lse_bound[live], "lse")
+    dq, dk, dv = torch.full_like(q, 7.0), torch.full_like(k, 7.0), torch.full_like(v, 7.0)
+    vk.attention_backward(q, k, v, out, lse, g, dq, dk, dv, scale=scale, q_lens=qt, kv_lens=kt)
+    for name, x, (w, e) in zip(("dq", "dk", "dv"), (dq, dk, dv), backward_reference(q, k, v, out, lse, g, ql, kl, scale)):
+        within(x, w, e, name)

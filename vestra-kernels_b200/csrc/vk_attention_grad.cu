@@ -688,7 +688,7 @@ __global__ void __launch_bounds__(256)
   const int bh = blockIdx.x / split, rank = blockIdx.x - bh * split, b = bh / a.heads, h = bh - b * a.heads;
   const int nq = min(seq_len(a.q_lens, b, a.nq), ROWS), nk = nq > 0 ? seq_len(a.kv_lens, b, a.nk) : 0;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, lg = lane % L, kg = lane / L;
-  const int each = (a.nk + split - 1) / split, from = min(rank * each, a.nk), to = min(from + each, a.nk);
+  const int each = (a.nk + split - 1) / split, from = min(rank * each, a.nk), to = min(from + each, a.nk), end = min(to, nk);
   const T* qp = head_of<T>(q, b, h);
   const T* gp = head_of<T>(d_out, b, h);
   const T* op = head_of<T>(out, b, h);
@@ -737,7 +737,7 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       kk[i] = vv[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (key < to && key < nk) {
+      if (key < end) {
         kk[i] = load4(kp + key * k.st + (i * L + lg) * 4);
         vv[i] = load4(vp + key * v.st + (i * L + lg) * 4);
       }
@@ -757,7 +757,10 @@ __global__ void __launch_bounds__(256)
     for (int r = 0; r < ROWS; ++r)
       if (r < nq) {
         const float s = dot(qv[r], kc), dp = dot(gv[r], vc);
-        if (key < nk) {  // (as weights of 0, keys past the end would turn what is not finite in q or d_out into NaN)
+        // (As weights of 0, keys past the end would turn what is not finite in q
+        // or d_out into NaN; so would zeros in the place of the next share's
+        // keys, where exp(-lse) is infinite.)
+        if (key < end) {
           const float p = expf(fmaf(s, a.scale, -ref[r])), ds = p * (dp - dl[r]);
           add(gvv, p, gv[r]);
           add(gk, ds, qv[r]);

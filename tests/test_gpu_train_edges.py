@@ -75,3 +75,29 @@ def test_attention_gradients_of_scores_far_below_zero(vk, dtype, b, h, nq, nk, d
     vk.attention_backward(q, k, v, out, lse, g, dq, dk, dv, scale=scale, q_lens=qt, kv_lens=kt)
     for name, x, (w, e) in zip(("dq", "dk", "dv"), (dq, dk, dv), backward_reference(q, k, v, out, lse, g, ql, kl, scale)):
         within(x, w, e, name)
+
+
+# queries, keys, ragged: the last block of keys full and not
+SIDES = [(140, 300, False), (140, 256, False), (256, 100, False), (3, 300, False), (1, 300, False), (70, 70, False), (260, 300, True)]
+
+
+def infinite_query(vk, dtype, nq, nk, ragged):
+    """Inputs whose middle query scores -inf with every key, and those without it."""
+    t, b, h, row = TYPES[dtype], 2, 20, nq // 2
+    q, k, v, _, _, _, _ = attention_case(t, b, h, nq, nk, 64, "head", False, 82)
+    k = (k.abs() + 0.1).to(t)
+    q[:, :, row, 5] = -math.inf
+    ql, kl = ([nq, nq - 9], [nk, nk - 7]) if ragged else ([nq] * b, [nk] * b)
+    out, lse = run_forward(vk, q, k, v, *((lens(ql), lens(kl)) if ragged else (None, None)))
+    return q, k, v, out, lse, ql, kl, row, [i for i in range(nq) if i != row]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("nq,nk,ragged", SIDES)
+def test_attention_query_of_minus_infinity(vk, dtype, nq, nk, ragged):
+    """A query that scores -inf with every key is a row without values: out 0, lse -inf; the others are as without it."""
+    q, k, v, out, lse, ql, kl, row, rest = infinite_query(vk, dtype, nq, nk, ragged)
+    assert (out[:, :, row] == 0).all() and (lse[:, :, row] == -math.inf).all()
+    if rest:
+        want, bound, _, _ = forward_reference(q[:, :, rest], k, v, [n - 1 for n in ql], kl, 0.125)
+        within(out[:, :, rest], want, bound, "out")

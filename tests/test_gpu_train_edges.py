@@ -8,7 +8,8 @@ import math
 
 import pytest
 import torch
-from test_gpu_train import TYPES, attention_case, backward_reference, forward_reference, gen, lens, make, run_backward, run_forward, within
+from test_gpu_train import (TYPES, attention_case, backward_reference, forward_reference, gen, lens, make, run_backward, run_forward,
+                            within)
 
 pytestmark = pytest.mark.gpu
 
@@ -101,3 +102,21 @@ def test_attention_query_of_minus_infinity(vk, dtype, nq, nk, ragged):
     if rest:
         want, bound, _, _ = forward_reference(q[:, :, rest], k, v, [n - 1 for n in ql], kl, 0.125)
         within(out[:, :, rest], want, bound, "out")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("nq,nk,ragged", SIDES)
+def test_attention_gradients_of_a_query_of_minus_infinity(vk, dtype, nq, nk, ragged):
+    """Its gradient is 0, the other queries' and the keys' are as without it (its infinite column of dk apart: 0 * inf)."""
+    q, k, v, out, lse, ql, kl, row, rest = infinite_query(vk, dtype, nq, nk, ragged)
+    g = make(q.shape, q.dtype, gen(83))
+    grads = run_backward(vk, q, k, v, out, lse, g, *((lens(ql), lens(kl)) if ragged else (None, None)))
+    assert (grads[0][:, :, row] == 0).all()
+    if not rest:
+        return
+    ql = [n - 1 for n in ql]
+    (dq, bq), (dk, bk), (dv, bv) = backward_reference(q[:, :, rest], k, v, out[:, :, rest], lse[:, :, rest], g[:, :, rest], ql, kl, 0.125)
+    finite = [i for i in range(64) if i != 5]
+    within(grads[0][:, :, rest], dq, bq, "dq")
+    within(grads[1][..., finite], dk[..., finite], bk[..., finite], "dk")
+    within(grads[2], dv, bv, "dv")

@@ -1149,8 +1149,9 @@ __global__ void __launch_bounds__(B_THREADS, 1)
           if constexpr (DQ) {
             // Keys past the end are zero rows of k: whatever finite dS a
             // score of 0 gives there counts nothing.  It stays finite unless
-            // the row's lse is far below 0.
-            if (I.len - j * TR < TR && __any_sync(0xffffffffu, !(shift2.x < 60.0f))) mask_columns(r, I.len - j * TR);
+            // the row's lse is far below 0 or its query infinite.
+            if (I.len - j * TR < TR && __any_sync(0xffffffffu, !(shift2.x < 60.0f) || __uint_as_float(r[127]) != 0.0f))
+              mask_columns(r, I.len - j * TR);
           }
 #pragma unroll
           for (int i = 0; i < 64; ++i) {

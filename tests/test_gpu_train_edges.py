@@ -120,3 +120,34 @@ def test_attention_gradients_of_a_query_of_minus_infinity(vk, dtype, nq, nk, rag
     within(grads[0][:, :, rest], dq, bq, "dq")
     within(grads[1][..., finite], dk[..., finite], bk[..., finite], "dk")
     within(grads[2], dv, bv, "dv")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("nk,nq,ragged", SIDES)
+def test_attention_key_of_minus_infinity(vk, dtype, nk, nq, ragged):
+    """A key that every query scores -inf with has no weight: its gradients are 0, the other keys' those of a batch
+    without it, and so are the queries' (its own infinite column of dq apart: 0 * inf)."""
+    t = TYPES[dtype]
+    b, h, row = 2, 20, nk // 2
+    q, k, v, _, _, _, _ = attention_case(t, b, h, nq, nk, 64, "head", False, 84)
+    q = (q.abs() + 0.1).to(t)
+    k[:, :, row, 5] = -math.inf
+    g = make(q.shape, t, gen(85))
+    ql, kl = ([nq, nq - 9], [nk, nk - 7]) if ragged else ([nq] * b, [nk] * b)
+    qt, kt = (lens(ql), lens(kl)) if ragged else (None, None)
+    out, lse = run_forward(vk, q, k, v, qt, kt)
+    grads = run_backward(vk, q, k, v, out, lse, g, qt, kt)
+    assert (grads[1][:, :, row] == 0).all() and (grads[2][:, :, row] == 0).all()
+    rest = [i for i in range(nk) if i != row]
+    if not rest:
+        assert (out == 0).all() and (lse == -math.inf).all()
+        return
+    kr, vr = k[:, :, rest], v[:, :, rest]
+    kl = [n - 1 for n in kl]
+    want, bound, _, _ = forward_reference(q, kr, vr, ql, kl, 0.125)
+    within(out, want, bound, "out")
+    (dq, bq), (dk, bk), (dv, bv) = backward_reference(q, kr, vr, out, lse, g, ql, kl, 0.125)
+    finite = [i for i in range(64) if i != 5]
+    within(grads[0][..., finite], dq[..., finite], bq[..., finite], "dq")
+    within(grads[1][:, :, rest], dk, bk, "dk")
+    within(grads[2][:, :, rest], dv, bv, "dv")

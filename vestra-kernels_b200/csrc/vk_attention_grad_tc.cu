@@ -1146,13 +1146,11 @@ __global__ void __launch_bounds__(B_THREADS, 1)
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(s_free);
-          if constexpr (DQ) {
-            // Keys past the end are zero rows of k: whatever finite dS a
-            // score of 0 gives there counts nothing.  It stays finite unless
-            // the row's lse is far below 0 or its query infinite.
-            if (I.len - j * TR < TR && __any_sync(0xffffffffu, !(shift2.x < 60.0f) || __uint_as_float(r[127]) != 0.0f))
-              mask_columns(r, I.len - j * TR);
-          }
+          // Streamed rows past the end are zeros: whatever finite P and dS a
+          // score of 0 gives there count nothing.  They stay finite unless the
+          // row's lse is far below 0 (dq) or an own row is infinite.
+          if (I.len - j * TR < TR && __any_sync(0xffffffffu, !(shift2.x < 60.0f) || __uint_as_float(r[127]) != 0.0f))
+            mask_columns(r, I.len - j * TR);
 #pragma unroll
           for (int i = 0; i < 64; ++i) {
             const float2 s = make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), f = make_float2(sl2, sl2);

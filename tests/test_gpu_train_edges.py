@@ -5,6 +5,9 @@ results are another's.
 
 Tolerances are those of test_gpu_train.py, derived there."""
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -151,3 +154,47 @@ def test_attention_key_of_minus_infinity(vk, dtype, nk, nq, ragged):
     within(grads[0][..., finite], dq[..., finite], bq[..., finite], "dq")
     within(grads[1][:, :, rest], dk, bk, "dk")
     within(grads[2][:, :, rest], dv, bv, "dv")
+
+
+@pytest.mark.parametrize("dtype,piece", [("f32", "attention"), ("bf16", "attention"), ("bf16", "rope"), ("f32", "norm")])
+def test_first_call_of_a_process_captured(dtype, piece):
+    """The first call on a device may be a captured one: nothing has to run before it."""
+    here = os.path.dirname(os.path.abspath(__file__))
+    run = subprocess.run([sys.executable, "-c", FIRST, dtype, piece], cwd=os.path.dirname(here), capture_output=True, text=True,
+                         env={**os.environ, "PYTHONPATH": os.path.join(os.path.dirname(here), "vestra-kernels_b200")}, timeout=300)
+    assert run.returncode == 0, run.stderr[-2000:]
+
+
+FIRST = """
+import sys, torch, vestra_kernels as vk
+t, piece = {"f32": torch.float32, "bf16": torch.bfloat16}[sys.argv[1]], sys.argv[2]
+x = torch.randn(2, 3, 200, 64, device="cuda").to(t)
+pos = torch.arange(200, device="cuda")[:, None].contiguous()
+vec = torch.ones(64, device="cuda")
+
+def run():
+    if piece == "attention":
+        out, lse = torch.empty_like(x), torch.empty(2, 3, 200, device="cuda")
+        grads = [torch.empty_like(x) for _ in range(3)]
+        vk.attention_forward(x, x, x, out, lse)
+        vk.attention_backward(x, x, x, out, lse, x, *grads)
+        return [out, lse, *grads]
+    if piece == "rope":
+        out = torch.empty_like(x)
+        vk.rope_axes(x, None, pos, (64,), 100.0, out, None)
+        return [out]
+    rows = x.view(6, 200, 64)
+    h, y, stats = torch.empty_like(rows), torch.empty_like(rows), torch.empty(6, 200, 2, device="cuda")
+    d_x, d_branch, d_gamma, d_beta = torch.empty_like(rows), torch.empty_like(rows), torch.empty_like(vec), torch.empty_like(vec)
+    vk.residual_norm_forward(rows, rows, vec, vec, 1e-6, h, y, stats)
+    vk.residual_norm_backward(rows, rows, h, rows, stats, vec, d_x, d_branch, d_gamma, d_beta)
+    return [h, y, stats, d_x, d_branch, d_gamma, d_beta]
+
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    held = run()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(held, run()))
+vk.synchronize()
+"""

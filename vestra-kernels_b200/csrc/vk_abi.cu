@@ -67,9 +67,16 @@ extern "C" int vk_init(int device, vk_ctx** out) {
   if (prop.major != 10) return vk_fail(VK_ERR_NO_DEVICE, "vk_init: device %d is sm_%d%d, this library is sm_100a", device, prop.major, prop.minor);
   vk_ctx* ctx = new vk_ctx();
   ctx->device = device;
+  // A context may be made while some stream is being captured (the first call
+  // of a binding that keeps one per device): nothing here is part of the
+  // capture or waits for it, so the thread asks not to be refused.
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  cudaThreadExchangeStreamCaptureMode(&mode);
   e = cudaStreamCreateWithFlags(&ctx->own_stream, cudaStreamNonBlocking);
   if (e == cudaSuccess) e = cudaMalloc(&ctx->d_err, sizeof(int));
-  if (e == cudaSuccess) e = cudaMemset(ctx->d_err, 0, sizeof(int));
+  if (e == cudaSuccess) e = cudaMemsetAsync(ctx->d_err, 0, sizeof(int), ctx->own_stream);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->own_stream);
+  cudaThreadExchangeStreamCaptureMode(&mode);
   if (e != cudaSuccess) {
     if (ctx->d_err) cudaFree(ctx->d_err);
     if (ctx->own_stream) cudaStreamDestroy(ctx->own_stream);

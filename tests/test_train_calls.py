@@ -1,0 +1,97 @@
+"""CPU checks of how the wrappers of the trainable block pieces make their
+calls: what they refuse before a pointer leaves them, and what a wait leaves
+alone.  The library, the contexts and torch's device are stood in for, so no
+GPU is needed."""
+import contextlib
+import threading
+
+import pytest
+import torch
+import vestra_kernels as vk
+
+
+class FakeContext:
+    """A context that follows one of the streams of `work`, as Context follows a cudaStream_t."""
+
+    handle = 1
+
+    def __init__(self, work):
+        self.work, self.stream, self.started = work, 7, threading.Event()
+
+    def set_stream(self, stream):
+        self.stream = stream
+
+    def synchronize(self):
+        self.started.set()
+        if self.stream in self.work:
+            assert self.work[self.stream].wait(20)
+
+
+@pytest.fixture
+def fake(monkeypatch):
+    """Two devices whose default-context calls go to stand-ins; `device` is the calling thread's current one."""
+    work, current = {7: threading.Event()}, threading.local()
+
+    @contextlib.contextmanager
+    def device(i):
+        before = getattr(current, "device", 0)
+        current.device = i
+        yield
+        current.device = before
+
+    class External:
+        def __init__(self, stream, device=None):
+            self.stream = stream
+
+        def synchronize(self):
+            contexts[0].started.set()
+            if self.stream in work:
+                assert work[self.stream].wait(20)
+
+    class Lib:
+        def __getattr__(self, name):
+            return lambda *a: vk.VK_OK
+
+    contexts = {0: FakeContext(work), 1: FakeContext(work)}
+    monkeypatch.setattr(vk, "_on_stream", {d: [c, 7] for d, c in contexts.items()})
+    monkeypatch.setattr(vk, "lib", lambda: Lib())
+    monkeypatch.setattr(vk, "_torch_stream", lambda d: 8)
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: getattr(current, "device", 0))
+    monkeypatch.setattr(torch.cuda, "ExternalStream", External)
+    return work, contexts
+
+
+def test_synchronize_leaves_other_threads_calls_alone(fake):
+    """While one thread waits for its work, another's call on another stream goes through."""
+    work, contexts = fake
+    waiting = threading.Thread(target=vk.synchronize, args=(0,))
+    waiting.start()
+    assert contexts[0].started.wait(20)
+    called = threading.Thread(target=vk._launch, args=("vk_rope_axes", 0, None))
+    called.start()
+    called.join(5)
+    through = not called.is_alive()
+    work[7].set()
+    waiting.join()
+    called.join()
+    assert through
+
+
+def test_synchronize_waits_for_a_call_made_during_another_wait(fake):
+    """A call that another thread made while one waited is the last one for the next wait."""
+    work, contexts = fake
+    first = threading.Thread(target=vk.synchronize, args=(0,))
+    first.start()
+    assert contexts[0].started.wait(20)
+    vk._launch("vk_rope_axes", 0, None)  # goes to stream 8
+    work[7].set()
+    first.join()
+    work[8] = threading.Event()
+    second = threading.Thread(target=vk.synchronize, args=(0,))
+    second.start()
+    second.join(0.5)
+    assert second.is_alive()
+    work[8].set()
+    second.join(20)
+    assert not second.is_alive()

@@ -119,11 +119,14 @@ extern "C" int vk_synchronize(vk_ctx* ctx) {
   cudaSetDevice(ctx->device);
   cudaError_t e = cudaStreamSynchronize(ctx->stream);
   if (e != cudaSuccess) return vk_cuda_status(e, "vk_synchronize");
+  // (on the context's stream: a plain copy would wait for the work of the default stream as well)
   int flag = 0;
-  e = cudaMemcpy(&flag, ctx->d_err, sizeof(int), cudaMemcpyDeviceToHost);
+  e = cudaMemcpyAsync(&flag, ctx->d_err, sizeof(int), cudaMemcpyDeviceToHost, ctx->stream);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->stream);
   if (e != cudaSuccess) return vk_cuda_status(e, "vk_synchronize: error word");
   if (flag != 0) {
-    cudaMemset(ctx->d_err, 0, sizeof(int));
+    cudaMemsetAsync(ctx->d_err, 0, sizeof(int), ctx->stream);
+    cudaStreamSynchronize(ctx->stream);  // before work of another stream, which the context may be set to next
     return vk_fail(VK_ERR_TIMEOUT, "a kernel gave up a bounded wait (device code 0x%x)", flag);
   }
   return VK_OK;

@@ -663,8 +663,16 @@ def synchronize(device: int | None = None) -> None:
     device = torch.cuda.current_device() if device is None else device
     with _on_stream_lock:
         own = _on_stream.get(device)
-        if own is not None:
+        stream = None if own is None else own[1]
+    if stream is None:
+        return
+    torch.cuda.ExternalStream(stream, device=device).synchronize()  # (without the lock: other calls go on meanwhile)
+    with _on_stream_lock:
+        own[0].set_stream(None)  # the context's own stream, which has no work: only the error word is looked at
+        try:
             own[0].synchronize()
+        finally:
+            own[0].set_stream(own[1])  # (a later call's, perhaps)
 
 
 _I32, _I64 = 2, 3  # element types of lengths and positions, beside DTYPE_F32 and DTYPE_BF16

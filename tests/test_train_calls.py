@@ -15,13 +15,14 @@ class FakeContext:
 
     handle = 1
 
-    def __init__(self, work):
-        self.work, self.stream, self.started = work, 7, threading.Event()
+    def __init__(self, device, work, current):
+        self.device, self.work, self.current, self.stream, self.started = device, work, current, 7, threading.Event()
 
     def set_stream(self, stream):
         self.stream = stream
 
     def synchronize(self):
+        self.current.device = self.device  # as vk_synchronize does
         self.started.set()
         if self.stream in self.work:
             assert self.work[self.stream].wait(20)
@@ -52,7 +53,7 @@ def fake(monkeypatch):
         def __getattr__(self, name):
             return lambda *a: vk.VK_OK
 
-    contexts = {0: FakeContext(work), 1: FakeContext(work)}
+    contexts = {d: FakeContext(d, work, current) for d in (0, 1)}
     monkeypatch.setattr(vk, "_on_stream", {d: [c, 7] for d, c in contexts.items()})
     monkeypatch.setattr(vk, "lib", lambda: Lib())
     monkeypatch.setattr(vk, "_torch_stream", lambda d: 8)
@@ -95,3 +96,10 @@ def test_synchronize_waits_for_a_call_made_during_another_wait(fake):
     work[8].set()
     second.join(20)
     assert not second.is_alive()
+
+
+def test_synchronize_leaves_the_current_device(fake):
+    work, _ = fake
+    work[7].set()
+    vk.synchronize(1)
+    assert torch.cuda.current_device() == 0

@@ -667,7 +667,7 @@ def synchronize(device: int | None = None) -> None:
     if stream is None:
         return
     torch.cuda.ExternalStream(stream, device=device).synchronize()  # (without the lock: other calls go on meanwhile)
-    with _on_stream_lock:
+    with _on_stream_lock, torch.cuda.device(device):
         own[0].set_stream(None)  # the context's own stream, which has no work: only the error word is looked at
         try:
             own[0].synchronize()

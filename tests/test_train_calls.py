@@ -103,3 +103,64 @@ def test_synchronize_leaves_the_current_device(fake):
     work[7].set()
     vk.synchronize(1)
     assert torch.cuda.current_device() == 0
+
+
+class OnGpu:
+    """What the wrappers ask of a CUDA tensor, with an address of its own."""
+
+    is_cuda = True
+
+    def __init__(self, *shape, dtype=torch.float32, address=1 << 20, device=0, strides=None):
+        self.shape, self.dtype, self.address, self.device = torch.Size(shape), dtype, address, torch.device("cuda", device)
+        self.strides = strides or torch.empty(shape, device="meta").stride()
+
+    def get_device(self):
+        return self.device.index
+
+    def dim(self):
+        return len(self.shape)
+
+    def numel(self):
+        return self.shape.numel()
+
+    def element_size(self):
+        return self.dtype.itemsize
+
+    def stride(self):
+        return self.strides
+
+    def is_contiguous(self):
+        return self.strides == torch.empty(self.shape, device="meta").stride()
+
+    def data_ptr(self):
+        return self.address
+
+
+@pytest.fixture
+def launched(monkeypatch):
+    """The calls that would have reached the library."""
+    calls = []
+    monkeypatch.setattr(vk, "_launch", lambda name, device, ctx, *args: calls.append((name, device, args)))
+    return calls
+
+
+def norm_backward(workspace):
+    x, vec, stats = OnGpu(2, 3, 8), OnGpu(8), OnGpu(2, 3, 2)
+    vk.residual_norm_backward(x, x, x, x, stats, vec, x, x, vec, vec, workspace=workspace)
+
+
+@pytest.mark.parametrize("workspace,error", [
+    (torch.empty(1 << 16, dtype=torch.uint8), TypeError),  # in host memory: its address means nothing on the GPU
+    (OnGpu(1 << 16, dtype=torch.uint8, device=1), TypeError),
+    (OnGpu(64, 1024, dtype=torch.uint8, strides=(4096, 1)), ValueError),  # more bytes than lie together
+])
+def test_norm_workspace_is_on_the_device(launched, workspace, error):
+    with pytest.raises(error, match="workspace"):
+        norm_backward(workspace)
+    assert not launched
+
+
+def test_norm_workspace_of_any_type(launched):
+    norm_backward(OnGpu(1 << 16, dtype=torch.uint8))
+    norm_backward(OnGpu(64, 256))
+    assert [c[2][-2:] for c in launched] == [(1 << 20, 1 << 16), (1 << 20, 1 << 16)]

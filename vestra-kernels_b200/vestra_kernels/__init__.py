@@ -868,6 +868,10 @@ def residual_norm_backward(d_h, d_y, h, branch, stats, gamma, d_x, d_branch, d_g
         import torch
 
         workspace = torch.empty(need, dtype=torch.uint8, device=h.device)
+    elif not workspace.is_cuda or workspace.get_device() != dev:
+        raise TypeError(f"the workspace must be on cuda:{dev}, got {workspace.device}")
+    elif not workspace.is_contiguous():
+        raise ValueError("the workspace must be contiguous")
     grads = _ResidualNormGrads(_flat(d_x, "d_x", s, shape.stream_dtype, dev), _flat(d_branch, "d_branch", s, shape.branch_dtype, dev),
                                _flat(d_gamma, "d_gamma", vec, f, dev), _flat(d_beta, "d_beta", vec, f, dev),
                                _flat(d_scale, "d_scale", vec, f, dev),

@@ -164,3 +164,12 @@ def test_norm_workspace_of_any_type(launched):
     norm_backward(OnGpu(1 << 16, dtype=torch.uint8))
     norm_backward(OnGpu(64, 256))
     assert [c[2][-2:] for c in launched] == [(1 << 20, 1 << 16), (1 << 20, 1 << 16)]
+
+
+def test_norm_workspace_of_matrices_at_odd_addresses(launched):
+    """bf16 matrices may start at any even address; the vectors, which only have to be there, are aligned f32."""
+    x = OnGpu(2, 3, 8, dtype=torch.bfloat16, address=(1 << 20) + 2)
+    vk.residual_norm_workspace(x, x, scale=x, gate=x, post_gamma=x)
+    shape = launched[0][2][0]._obj
+    for name in ("gamma", "beta", "scale", "gate", "post_gamma", "post_beta"):
+        assert getattr(shape, name) and getattr(shape, name) % 4 == 0, name

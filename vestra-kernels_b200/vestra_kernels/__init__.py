@@ -833,7 +833,7 @@ def residual_norm_forward(x, branch, gamma, beta, eps, h, y, stats, scale=None, 
 def residual_norm_workspace(x, branch, scale=None, gate=None, post_gamma=None, ctx: Context | None = None) -> int:
     """Bytes of the workspace that residual_norm_backward takes for these operands."""
     dev = _device_of(x, ctx)
-    any_vector = x.data_ptr() or 16  # only whether a vector is there counts
+    any_vector = 16  # only whether a vector is there counts
     g, t, c = x.shape
     shape = _ResidualNormShape(_dtype_code(x, "x"), _dtype_code(branch, "branch"), g, t, c, 0.0, any_vector, any_vector,
                                None if scale is None else any_vector, None if gate is None else any_vector,

@@ -198,3 +198,18 @@ torch.cuda.synchronize()
 assert all(torch.equal(a, b) for a, b in zip(held, run()))
 vk.synchronize()
 """
+
+
+def test_residual_norm_of_as_many_rows_as_are_taken(vk):
+    """2^31 - 1 rows, of one column: h = x + branch, whose norm is beta."""
+    rows = 2 ** 31 - 1
+    x = torch.zeros(1, rows, 1, dtype=torch.bfloat16, device="cuda")
+    branch, y = torch.ones_like(x), torch.zeros_like(x)
+    stats = torch.zeros(1, rows, 2, device="cuda")
+    x[0, -9:] = 2
+    gamma, beta = torch.ones(1, device="cuda"), torch.full((1,), 3.0, device="cuda")
+    vk.residual_norm_forward(x, branch, gamma, beta, 1e-2, x, y, stats)
+    assert (x[0, :9] == 1).all() and (x[0, -9:] == 3).all()
+    assert (stats[0, -9:, 0] == 3).all() and (stats[0, :9, 0] == 1).all()
+    within(stats[0, -9:, 1], torch.full((9,), 10.0, device="cuda"), 10 * 2.0 ** -22, "rstd")
+    assert (y == 3).all()

@@ -496,7 +496,7 @@ cudaError_t forward(const ResidualNorm& r, const void* x, const void* branch, vo
   const bool wide = r.cols % 8 == 0 && aligned32({x, branch, h, y, r.gamma, r.beta, r.scale, r.gate, r.post_gamma, r.post_beta});
 #define VK_RN(VEC, T, NV)                                                                                          \
   k_residual_norm<XT, BT, VEC, T, NV>                                                                              \
-      <<<resident_grid(k_residual_norm<XT, BT, VEC, T, NV>, (rows + RN_BLOCK / T - 1) / (RN_BLOCK / T)), RN_BLOCK, 0, \
+      <<<resident_grid(k_residual_norm<XT, BT, VEC, T, NV>, (rows - 1) / (RN_BLOCK / T) + 1), RN_BLOCK, 0,           \
          s>>>(r, rows, FastDiv(r.rows_per_group), static_cast<const XT*>(x), static_cast<const BT*>(branch),       \
               static_cast<XT*>(h), static_cast<BT*>(y), stats, post_stats)
   if (wide) {

@@ -213,3 +213,18 @@ def test_residual_norm_of_as_many_rows_as_are_taken(vk):
     assert (stats[0, -9:, 0] == 3).all() and (stats[0, :9, 0] == 1).all()
     within(stats[0, -9:, 1], torch.full((9,), 10.0, device="cuda"), 10 * 2.0 ** -22, "rstd")
     assert (y == 3).all()
+
+
+@pytest.mark.parametrize("side", [False, True])
+def test_synchronize_waits_for_the_last_call(vk, side):
+    """Of the default stream and of another one."""
+    x = make((64, 12, 3000, 64), torch.bfloat16, gen(88))
+    pos, out = torch.arange(3000, device="cuda")[:, None].contiguous(), torch.empty_like(x)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.Stream() if side else torch.cuda.default_stream()):
+        for _ in range(20):
+            vk.rope_axes(x, None, pos, (64,), 100.0, out, None)
+        done = torch.cuda.Event()
+        done.record()
+    vk.synchronize()
+    assert done.query()

@@ -666,7 +666,8 @@ def synchronize(device: int | None = None) -> None:
         stream = None if own is None else own[1]
     if stream is None:
         return
-    torch.cuda.ExternalStream(stream, device=device).synchronize()  # (without the lock: other calls go on meanwhile)
+    # without the lock: other calls go on meanwhile (torch takes cudaStreamLegacy for no external stream)
+    (torch.cuda.default_stream(device) if stream == 1 else torch.cuda.ExternalStream(stream, device=device)).synchronize()
     with _on_stream_lock, torch.cuda.device(device):
         own[0].set_stream(None)  # the context's own stream, which has no work: only the error word is looked at
         try:

@@ -29,6 +29,8 @@
 // of the backward pass does not leave room for two blocks on an SM.
 #include <cuda_bf16.h>
 
+#include <type_traits>
+
 #include "vk_common.cuh"
 #include "vk_internal.h"
 #include "vk_train.h"
@@ -927,20 +929,27 @@ int few_split(int tiles, int keys) {
 template <class T, int D>
 cudaError_t forward(const AttnShape& a, HeadsView q, HeadsView k, HeadsView v, HeadsView out, float* lse,
                     cudaStream_t s) {
-  if (a.nq <= FEW_MAX) {
-    const int tiles = blocks_of(a, a.nq, a.nq == 1 ? 1 : FEW), split = few_split(tiles, a.nk);
-    return a.nq == 1 ? launch(k_attn_forward_few<T, D, 1>, tiles, split, 256, 0, s, a, split, q, k, v, out, lse)
-                     : launch(k_attn_forward_few<T, D, FEW>, tiles, split, 256, 0, s, a, split, q, k, v, out, lse);
+  if (a.nq == 1) {
+    const int tiles = blocks_of(a, 1, 1), split = few_split(tiles, a.nk);
+    return launch(k_attn_forward_few<T, D, 1>, tiles, split, 256, 0, s, a, split, q, k, v, out, lse);
   }
-  const Layout l = layout_of(a, a.nq, a.nk, true);
-  const int tiles = blocks_of(a, a.nq, 16 * l.rm);
-  if (l.rm == 8)
-    return launch(k_attn_forward_simt<T, D, 8, 8>, tiles, 1, 128, tile_bytes<D, 8>(1, 2, 1, 0), s, a, 1, q, k, v, out, lse);
-  if (l.rm == 4)
-    return launch(k_attn_forward_simt<T, D, 4, 16>, tiles, l.split, 256, tile_bytes<D, 4>(1, 2, 1, 0), s, a, l.split, q, k,
-                  v, out, lse);
-  return launch(k_attn_forward_simt<T, D, 2, 16>, tiles, l.split, 256, tile_bytes<D, 2>(1, 2, 1, 0), s, a, l.split, q, k, v,
-                out, lse);
+  if constexpr (D == 64 && std::is_same_v<T, __nv_bfloat16>) {
+    return cudaErrorInvalidValue;  // the tensor cores take them
+  } else {
+    if (a.nq <= FEW_MAX) {
+      const int tiles = blocks_of(a, a.nq, FEW), split = few_split(tiles, a.nk);
+      return launch(k_attn_forward_few<T, D, FEW>, tiles, split, 256, 0, s, a, split, q, k, v, out, lse);
+    }
+    const Layout l = layout_of(a, a.nq, a.nk, true);
+    const int tiles = blocks_of(a, a.nq, 16 * l.rm);
+    if (l.rm == 8)
+      return launch(k_attn_forward_simt<T, D, 8, 8>, tiles, 1, 128, tile_bytes<D, 8>(1, 2, 1, 0), s, a, 1, q, k, v, out, lse);
+    if (l.rm == 4)
+      return launch(k_attn_forward_simt<T, D, 4, 16>, tiles, l.split, 256, tile_bytes<D, 4>(1, 2, 1, 0), s, a, l.split, q, k,
+                    v, out, lse);
+    return launch(k_attn_forward_simt<T, D, 2, 16>, tiles, l.split, 256, tile_bytes<D, 2>(1, 2, 1, 0), s, a, l.split, q, k, v,
+                  out, lse);
+  }
 }
 
 template <class T, int D, int RM>

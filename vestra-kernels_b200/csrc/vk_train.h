@@ -44,7 +44,7 @@ __device__ __forceinline__ int seq_len(const int32_t* lens, int b, int tokens) {
 }
 
 // CUDA-core attention, f32 or bf16 elements, head_dim 8, 16, 32 or 64
-// (vk_attention_grad.cu).
+// (vk_attention_grad.cu).  The forward pass takes bf16 of 64 for one query only.
 cudaError_t attention_forward_simt(const AttnShape& a, bool bf16, HeadsView q, HeadsView k, HeadsView v, HeadsView out,
                                    float* lse, cudaStream_t s);
 cudaError_t attention_backward_simt(const AttnShape& a, bool bf16, HeadsView q, HeadsView k, HeadsView v, HeadsView out,

@@ -11,8 +11,9 @@ import sys
 
 import pytest
 import torch
-from test_gpu_train import (TYPES, attention_case, backward_reference, forward_reference, gen, lens, make, run_backward, run_forward,
-                            within)
+from test_gpu_train import (EPS, HALF, TYPES, U32, attention_case, backward_reference, forward_reference, gen, hat_error, lens, make,
+                            norm_backward_reference, norm_inputs, run_backward, run_forward, run_norm, run_norm_backward,
+                            standard64, within)
 
 pytestmark = pytest.mark.gpu
 
@@ -228,3 +229,90 @@ def test_synchronize_waits_for_the_last_call(vk, side):
         done.record()
     vk.synchronize()
     assert done.query()
+
+
+# bf16 of 64 where few queries or few keys meet a long other side on the tensor cores, and few scores off them
+SHORT_SIDES = [(8, 3, 2, 1500), (8, 12, 2, 700), (8, 12, 3, 300), (8, 12, 7, 500), (8, 12, 500, 5), (4, 12, 900, 2), (4, 30, 60, 60),
+               (3, 5, 130, 3), (1, 2, 3, 300), (2, 2, 4, 150), (1, 1, 60, 60), (1, 2, 865, 3)]
+
+
+@pytest.mark.parametrize("b,h,nq,nk", SHORT_SIDES)
+@pytest.mark.parametrize("ragged", [False, True])
+def test_attention_with_a_short_side(vk, b, h, nq, nk, ragged):
+    q, k, v, ql, kl, qt, kt = attention_case(torch.bfloat16, b, h, nq, nk, 64, "token", ragged, 89)
+    out, lse = run_forward(vk, q, k, v, qt, kt)
+    want, bound, lse_want, lse_bound = forward_reference(q, k, v, ql, kl, 0.125)
+    within(out, want, bound, "out")
+    live = lse_want != -math.inf
+    assert torch.equal(lse != -math.inf, live)
+    within(lse[live], lse_want[live], lse_bound[live], "lse")
+    g = make(q.shape, q.dtype, gen(90), "token")
+    if ragged:
+        for i in range(b):
+            g[i, :, ql[i]:] = math.nan
+    grads = run_backward(vk, q, k, v, out, lse, g, qt, kt)
+    for name, x, (w, e) in zip(("dq", "dk", "dv"), grads, backward_reference(q, k, v, out, lse, g, ql, kl, 0.125)):
+        within(x, w, e, name)
+
+
+@pytest.mark.parametrize("b,h,n,m,lengths", [(8, 12, 865, 2, None), (8, 12, 865, 8, None), (8, 12, 3, 865, None), (8, 12, 300, 300, (200, 3)),
+                                             (8, 12, 865, 865, None)])
+def test_attention_gradients_keep_their_error_on_short_sides(vk, b, h, n, m, lengths):
+    """The tensor cores round P and dS to bf16, and that costs a gradient as much as its own rounding whether a row has two
+    keys or many: of terms of random signs the squares add up to the square of their sum, on average, so roundings of the
+    terms and one of the sum, each 2^-9 / sqrt(3) of a value as a root mean square over a binade, make sqrt(2) of the
+    latter alone; 1.6 is an eighth above it, for averages over ten thousand values and more."""
+    q, k, v, _, _, _, _ = attention_case(torch.bfloat16, b, h, n, m, 64, "head", False, 91)
+    g = make(q.shape, q.dtype, gen(92))
+    x, y = lengths or (n, m)
+    qt, kt = (lens([x] * b), lens([y] * b)) if lengths else (None, None)
+    out, lse = run_forward(vk, q, k, v, qt, kt)
+    grads = run_backward(vk, q, k, v, out, lse, g, qt, kt)
+    q, k, v, g, out = (t[:, :, :c].double() for t, c in ((q, x), (k, y), (v, y), (g, x), (out, x)))
+    p = torch.softmax(q @ k.mT * 0.125, -1)
+    ds = p * (g @ v.mT - (g * out).sum(-1, keepdim=True))
+    for got, want in zip(grads, (ds @ k * 0.125, ds.mT @ q * 0.125, p.mT @ g)):
+        got = got[:, :, :want.shape[2]].double()
+        one = (want.bfloat16().double() - want).norm()
+        assert (got - want).norm() <= 1.6 * one
+
+
+def test_residual_norm_at_odd_addresses(vk):
+    """Every output of matrices that start 4 or 2 bytes off, against 64 bits."""
+    s = norm_inputs("f32", "bf16", 3, 401, 136, True, True, True, 50)
+
+    def off(t):  # the same values, one element further
+        return None if t is None else torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")[1:].view(t.shape).copy_(t)
+
+    h, y, stats, post_stats = run_norm(vk, s)
+    g = gen(51)
+    d_h, d_y = torch.randn(h.shape, device="cuda", generator=g), torch.randn(y.shape, device="cuda", generator=g).bfloat16()
+    s = {n: off(t) for n, t in s.items()}
+    x, y3, h3 = off(s["x"]), off(torch.zeros_like(y)), off(torch.zeros_like(h))
+    st3, post3 = torch.zeros_like(stats), torch.zeros_like(post_stats)
+    vk.residual_norm_forward(x, s["branch"], s["gamma"], s["beta"], EPS, h3, y3, st3, scale=s["scale"], gate=s["gate"],
+                             post_gamma=s["post_gamma"], post_beta=s["post_beta"], post_stats=post3)
+    n = s["branch"].double()
+    hat, mean, rstd = standard64(n)
+    e, e_mean, e_rstd = hat_error(n, mean, rstd, 0 * n)
+    within(post3[..., :1], mean, e_mean, "post mean")
+    within(post3[..., 1:], rstd, e_rstd, "post rstd")
+    pg = s["post_gamma"].double()
+    n = hat * pg + s["post_beta"].double()
+    n_err = e * pg.abs() + 2 * U32 * (n.abs() + (hat * pg).abs())
+    f = s["scale"].double() * s["gate"].double()[:, None]
+    want_h = s["x"].double() + f * n
+    h_err = f.abs() * (n_err + 2 * U32 * n.abs()) * 1.01 + U32 * want_h.abs()
+    within(h3, want_h, h_err + U32 * 1.01 * want_h.abs(), "h")
+    hat, mean, rstd = standard64(want_h)
+    e, e_mean, e_rstd = hat_error(want_h, mean, rstd, h_err)
+    within(st3[..., :1], mean, e_mean + 1e-12, "mean")
+    within(st3[..., 1:], rstd, e_rstd, "rstd")
+    want_y = hat * s["gamma"].double() + s["beta"].double()
+    y_err = e * s["gamma"].double().abs() + 2 * U32 * (want_y.abs() + (hat * s["gamma"].double()).abs())
+    within(y3, want_y, y_err + HALF[torch.bfloat16] * 1.01 * want_y.abs(), "y")
+    got = run_norm_backward(vk, s, h3, st3, post3, off(d_h), off(d_y), d_x=off(d_h), d_branch=off(d_y))
+    want, bound = norm_backward_reference(s, h3, st3, post3, d_h, d_y)
+    assert set(got) == set(want)
+    for name in want:
+        within(got[name], want[name], bound[name] + 1e-30, name)

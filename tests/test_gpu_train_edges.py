@@ -260,8 +260,7 @@ def test_attention_with_a_short_side(vk, b, h, nq, nk, ragged):
 def test_attention_gradients_keep_their_error_on_short_sides(vk, b, h, n, m, lengths):
     """The tensor cores round P and dS to bf16, and that costs a gradient as much as its own rounding whether a row has two
     keys or many: of terms of random signs the squares add up to the square of their sum, on average, so roundings of the
-    terms and one of the sum, each 2^-9 / sqrt(3) of a value as a root mean square over a binade, make sqrt(2) of the
-    latter alone; 1.6 is an eighth above it, for averages over ten thousand values and more."""
+    terms and one of the sum, of the same relative size, make sqrt(2) of the latter alone as a root mean square; 1.6 is an eighth above it, for averages over ten thousand values and more."""
     q, k, v, _, _, _, _ = attention_case(torch.bfloat16, b, h, n, m, 64, "head", False, 91)
     g = make(q.shape, q.dtype, gen(92))
     x, y = lengths or (n, m)
@@ -316,3 +315,19 @@ def test_residual_norm_at_odd_addresses(vk):
     assert set(got) == set(want)
     for name in want:
         within(got[name], want[name], bound[name] + 1e-30, name)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("scale", [1e-38, 1e-40, 2.0 ** -100])
+def test_attention_of_a_tiny_scale(vk, dtype, scale):
+    """Every score next to 0: the mean of the values, and gradients that keep it."""
+    q, k, v, ql, kl, _, _ = attention_case(TYPES[dtype], 2, 12, 200, 300, 64, "head", False, 93)
+    g = make(q.shape, q.dtype, gen(94))
+    out, lse = run_forward(vk, q, k, v, None, None, scale=scale)
+    want, bound, lse_want, lse_bound = forward_reference(q, k, v, ql, kl, scale)
+    within(out, want, bound, "out")
+    within(lse, lse_want, lse_bound, "lse")
+    dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+    vk.attention_backward(q, k, v, out, lse, g, dq, dk, dv, scale=scale)
+    for name, x, (w, e) in zip(("dq", "dk", "dv"), (dq, dk, dv), backward_reference(q, k, v, out, lse, g, ql, kl, scale)):
+        within(x, w, e, name)

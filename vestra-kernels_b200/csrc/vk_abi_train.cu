@@ -208,7 +208,9 @@ extern "C" int vk_attention_backward(vk_ctx* ctx, const vk_attention_shape* shap
     // takes no tiles either: 12 heads of 3457 keys 44 us from the caller (78 on
     // the tensor cores), 1536 heads 813 (1177).
     const bool few = static_cast<int64_t>(a.batch) * a.heads * a.nq <= 8192 / a.nk;
-    if (bf16 && a.dim == 64 && a.nq > 1 && !few)
+    // There lse / scale is an operand: below this scale it could pass f32's range.
+    const bool tiny_scale = a.scale < 0x1p-100f;
+    if (bf16 && a.dim == 64 && a.nq > 1 && !few && !tiny_scale)
       return vk_cuda_status(attention_backward_tc(a, vq, vk_, vv, vo, lse, vg, vdq, vdk, vdv, delta, ctx->d_err, s), name);
     return vk_cuda_status(attention_backward_simt(a, bf16, vq, vk_, vv, vo, lse, vg, vdq, vdk, vdv, delta, s), name);
   });

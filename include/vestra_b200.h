@@ -56,7 +56,7 @@ typedef struct {
 
 /* ---------------------------------------------------------------- lifecycle */
 /* Context on CUDA device `device` (one per GPU).  Replaces CudaRuntime::new
- * (src/cuda.rs:383-443). */
+ * (src/cuda.rs:383-443).  May be called while a stream is being captured. */
 int vk_init(int device, vk_ctx** out);
 int vk_destroy(vk_ctx* ctx);
 /* Use this cudaStream_t for later calls (NULL = the context's own stream,
@@ -336,8 +336,9 @@ int vk_conv3x3_release(vk_conv3x3* conv);
  *  - Buffers are device pointers of the context's GPU; the element type is
  *    given per call and decides the arithmetic (vk_set_math does not apply).
  *  - They allocate nothing and use no workspace of the context, so a call can
- *    be captured into a CUDA graph and replayed; what a call needs beside its
- *    outputs is passed in and belongs to the caller.
+ *    be captured into a CUDA graph and replayed for as long as the context
+ *    lives (its kernels report to the context's error word); what a call needs
+ *    beside its outputs is passed in and belongs to the caller.
  *  - Every element of every output is written on every call, the same bits
  *    each time (no atomics); outputs may not overlap inputs except where said.
  *  - The calling thread's current device is left as it was. */
@@ -365,12 +366,13 @@ typedef struct {
 
 /* out = softmax(scale q k^T) v over the valid keys, not causal; lse [batch,
  * heads, q_tokens] (f32) = log of the row's sum of exponentials.  Queries past
- * q_lens and rows without keys: out 0, lse -inf.  What lies past the lengths
- * in q, k, v is never used (it may hold NaN). */
+ * q_lens, rows without keys and rows whose scores are all -inf: out 0, lse -inf.
+ * What lies past the lengths in q, k, v is never used (it may hold NaN). */
 int vk_attention_forward(vk_ctx* ctx, const vk_attention_shape* shape, const vk_heads* q, const vk_heads* k,
                          const vk_heads* v, const vk_heads* out, float* lse);
 /* Gradients of vk_attention_forward for d_out, from its inputs, out and lse;
- * the probabilities are recomputed.  Rows past the lengths get zeros.  delta
+ * the probabilities are recomputed.  Rows past the lengths get zeros, whatever
+ * the others hold.  delta
  * [batch, heads, q_tokens] (f32) is scratch that belongs to this call until it
  * has run; it receives the row sums of d_out * out. */
 int vk_attention_backward(vk_ctx* ctx, const vk_attention_shape* shape, const vk_heads* q, const vk_heads* k,

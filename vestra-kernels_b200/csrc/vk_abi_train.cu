@@ -200,11 +200,13 @@ extern "C" int vk_attention_backward(vk_ctx* ctx, const vk_attention_shape* shap
     VK_TRY(heads_view(name, "d_out", d_out, shape->dtype, B, H, a.nq, D, 16, &vg));
     VK_TRY(floats_ok(name, "lse", lse));
     VK_TRY(apart(name, {vdq.p, vdk.p, vdv.p, delta}, {vq.p, vk_.p, vv.p, vo.p, vg.p, lse}));
-    // The tensor cores take dS rounded to bf16.  Over many scores that adds up
-    // to 1.4 times the error that the rounding of the results has by itself; of
-    // a few scores one alone can carry a row, at up to 2.6 times.  Few scores
-    // are launch latency either way (1 x 61 x 61 14 us on the device there, 23
-    // here, 22 from the caller), so they keep f32 throughout.  One query alone
+    // The tensor cores take P and dS rounded to bf16.  That makes a gradient's
+    // error 1.41 to 1.45 times the one of its own rounding as a root mean square,
+    // of 2 keys (865 queries, 96 heads) as of 865, of 2 queries as of many.  In a
+    // call of a few scores the largest of the few errors is up to 2.6 times the
+    // largest rounding.  Such calls are launch latency either way (1 x 61 x 61 14
+    // us on the device there, 23 here, 22 from the caller), so they keep f32
+    // throughout.  One query alone
     // takes no tiles either: 12 heads of 3457 keys 44 us from the caller (78 on
     // the tensor cores), 1536 heads 813 (1177).
     const bool few = static_cast<int64_t>(a.batch) * a.heads * a.nq <= 8192 / a.nk;

@@ -317,8 +317,10 @@ struct ItemList<false> {};
 // more MMA in the last block, a column of ones against a column of 0 and -inf.
 // (As selects in the warps it took as long as the block's exponentials.)
 //
-// 64 images of 865 tokens, 12 heads: 233 us, 630 TFLOP/s.  MUFU needs 124 of
-// them, the products 91; the two tiles' hand-overs take the rest.
+// 64 images of 865 tokens, 12 heads: 242 us in a replayed graph, 610 TFLOP/s
+// (259 once the card is at its power limit, 1.77 GHz; 261 from the caller).
+// MUFU needs 124 of them, the products 91; the two tiles' hand-overs take the
+// rest.
 namespace {
 constexpr uint32_t F_P = 256, F_O = 384;
 constexpr size_t F_SMEM = 1024 + TILE_B * (4 + 2 * ST) + (ST + 1) * EXT_B + 512;
@@ -735,8 +737,9 @@ __global__ void __launch_bounds__(F_THREADS, 1)
 // columns each (bf16 hi + mid + lo, 24 bits) against ones: S becomes
 // S - lse / scale and dP becomes dP - delta for two more MMAs a block.
 //
-// 64 images of 865 tokens, 12 heads: 602 us for both kernels, 610 TFLOP/s of
-// five products (855 of the seven that run).  MUFU is 42 to 55% busy, the
+// 64 images of 865 tokens, 12 heads: 599 us for both kernels in a replayed
+// graph, 614 TFLOP/s of five products (860 of the seven that run); 693 once the
+// card is at its power limit, 1.65 GHz, and 696 from the caller.  MUFU is 42 to 55% busy, the
 // tensor pipe 41 to 45%: with one S, P and dS in tensor memory, which is full,
 // the groups wait for one another.
 namespace {

@@ -235,8 +235,9 @@ Chunks chunks_of(const ResidualNorm& r) {
   Chunks c;
   c.groups = r.gate != nullptr ? r.groups : 1;
   c.group_rows = r.gate != nullptr ? r.rows_per_group : r.groups * r.rows_per_group;
-  // about five resident blocks per SM, but at least four rows each: a chunk
-  // writes its column sums once however few rows it has
+  // five blocks per SM, what is resident at 768 columns (at other widths and
+  // with a gate some places stay empty or some blocks start late), but at least
+  // four rows each: a chunk writes its column sums once however few rows it has
   const int64_t want = static_cast<int64_t>(num_sms()) * 5;
   const int64_t total = static_cast<int64_t>(c.groups) * c.group_rows;
   int64_t rows = (total + want - 1) / want;
